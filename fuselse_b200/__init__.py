@@ -20,6 +20,8 @@ memory with the copies overlapped.
 """
 from . import ext
 from .autograd import make_fuselse_logsumexp
+from .linear import linear_cross_entropy, linear_selective_log_softmax
 from .selective import selective_log_softmax
 
-__all__ = ["ext", "make_fuselse_logsumexp", "selective_log_softmax"]
+__all__ = ["ext", "make_fuselse_logsumexp", "selective_log_softmax", "linear_cross_entropy",
+           "linear_selective_log_softmax"]

@@ -66,6 +66,21 @@ SIGNATURES = {
     "fl_ipc_buffer_open": [c_int, c_void_p, POINTER(c_void_p)],
     "fl_ipc_buffer_close": [c_int, c_void_p],
     "fl_ipc_buffer_free": [c_int, c_void_p],
+    "fl_linear_loss_workspace": [c_int64, c_int64, c_int64, c_int64, c_int, POINTER(c_int64),
+                                 POINTER(c_int64)],
+    "fl_linear_loss_pack": [POINTER(c_uint16), POINTER(c_int64), c_int64, POINTER(c_uint16),
+                            POINTER(c_int), POINTER(c_int), POINTER(c_int), c_int64, c_int64, c_int64,
+                            c_int64, c_int64, _stream],
+    "fl_linear_loss_fwd": [POINTER(c_uint16), c_int64, POINTER(c_uint16), c_int64, c_int,
+                           POINTER(c_int64), POINTER(c_int), POINTER(c_int), POINTER(c_int), c_int64,
+                           c_int64, c_int64, c_int, c_float, _fp, _fp, c_void_p, c_int64,
+                           POINTER(c_int), _stream],
+    "fl_linear_loss_bwd": [_fp, POINTER(c_uint16), c_int64, POINTER(c_uint16), c_int64, c_int,
+                           POINTER(c_int64), POINTER(c_int), POINTER(c_int), POINTER(c_int), _fp,
+                           c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_int64,
+                           POINTER(c_uint16), POINTER(c_uint16), c_void_p, c_int64, _stream],
+    "fl_copy_rows16": [POINTER(c_uint16), POINTER(c_uint16), c_int64, c_int64, c_int64, c_int64,
+                       c_int64, c_int64, _stream],
     "fl_binary_version": [c_int, POINTER(c_int)],
 }
 

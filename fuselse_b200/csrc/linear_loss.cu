@@ -1,0 +1,930 @@
+// Losses over a vocabulary taken straight from hidden states and the output
+// projection, z = hidden @ weight^T, without keeping z (sm_100a).
+//
+//   forward   lse_i = LSE_v z_iv and z_{i,t_i}: one tensor-core product whose
+//             epilogue folds each 256 x 256 tile of z into (max, sum-exp) per
+//             row, then a small kernel that merges a row's pieces.
+//   backward  dz_iv = a_i softmax(z_i)_v - b_i [v = t_i], in pieces of the
+//             vocabulary: the product is recomputed, dz of the piece is written
+//             in 16 bits, and two more products take it to the gradients
+//             dW = dz^T hidden and dH = dz weight.
+//   Tokens without a target are packed away first, so every product runs over
+//   the remaining rows only.
+//
+// One persistent kernel does all four products: a CTA pair per 256 x 256 tile
+// (tcgen05.mma over two SMs, fp32 accumulators in tensor memory, two of them so
+// that one tile's epilogue overlaps the next tile's products), operands staged
+// by tensor-map copies 64 deep in K; warp 0 copies, warp 1 issues the products,
+// warps 4-11 are the epilogue.
+#include "common.cuh"
+#include "rows.cuh"
+#include "umma.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <algorithm>
+
+namespace fl {
+namespace {
+
+constexpr int kTile = 256;            // rows and columns of a CTA pair's tile
+constexpr int kHalfTile = 128;        // rows of A and of B staged by one CTA
+constexpr int kBlockK = 64;           // 128 bytes of a 16-bit operand
+constexpr int kGemmThreads = 384;     // 4 warps of roles, 8 epilogue warps
+constexpr int kEpiWarps = 8;
+constexpr uint32_t kOperandBytes = kHalfTile * kBlockK * 2;   // 16 KB
+constexpr uint32_t kStageBytes = 2 * kOperandBytes;
+constexpr uint32_t kStageTx = 2 * kStageBytes;                // both CTAs' copies
+constexpr uint32_t kStagingBuf = 4096;                        // 32 rows of 128 bytes
+constexpr uint32_t kTmemCols = 512;                           // two fp32 accumulators
+
+// What a product's epilogue does with a tile.
+enum Epi {
+    kEpiStats = 0,   // (max, sum-exp) of each row's 128-column pieces, target logits
+    kEpiGradZ = 1,   // dz of the tile in 16 bits
+    kEpiOut16 = 2,   // scaled, in 16 bits
+    kEpiSlab = 3,    // fp32 partial sums (stored, or added to what is there)
+};
+
+template <int EPI>
+struct GemmShape {
+    static constexpr bool kAMn = EPI == kEpiOut16;                    // A given as [k][m]
+    static constexpr bool kBMn = EPI == kEpiOut16 || EPI == kEpiSlab;  // B given as [k][n]
+    static constexpr int kStages = EPI == kEpiStats ? 7 : 5;
+    static constexpr uint32_t kStaging = EPI == kEpiStats ? 0 : kEpiWarps * 2 * kStagingBuf;
+    static constexpr uint32_t kSmem = kStages * kStageBytes + kStaging + 1024 + 256;
+};
+
+// meta words shared by the kernels of a call
+enum Meta { kMetaRows = 0, kMetaCount = 1, kMetaStop = 2 };
+
+struct GemmArgs {
+    int rows;              // rows of hidden (the packed count is meta[kMetaRows] when packed)
+    int packed;
+    int m_extent, n_extent, k_extent;  // of the product; the one that counts rows is -1
+    int b_offset;          // added to B's row coordinate
+    int out_row;           // added to the output's row coordinate
+    int splits;            // pieces of K, each with an output slab of its own
+    int slab_rows;
+    int add;               // add to the slab instead of storing it
+    uint32_t idesc;
+    int* meta;
+    const int64_t* target;
+    const int* src;        // packed row -> row of target
+    float2* part;          // [row][pieces] partial states
+    int pieces;
+    float* zt;
+    const float *lse, *a, *b, *inv_scale;
+    void* out;             // kEpiOut16: filled with NaN when a wait ran out
+    int64_t out_elems;
+};
+
+struct Unit {
+    int m, n, k0, k1, slab;
+};
+
+// Work unit u: K piece by K piece, tiles of a piece in groups of 8 tile rows,
+// so that the tiles in flight share operand rows through L2.
+constexpr int kGroupM = 8;
+__device__ __forceinline__ Unit decode_unit(int u, int mt, int nt, int splits, int kb) {
+    Unit t;
+    const int tiles = mt * nt;
+    t.slab = u / tiles;
+    const int r = u - t.slab * tiles;
+    const int group = r / (kGroupM * nt);
+    const int gm = min(kGroupM, mt - group * kGroupM);
+    const int q = r - group * kGroupM * nt;
+    t.m = group * kGroupM + q % gm;
+    t.n = q / gm;
+    t.k0 = static_cast<int>((int64_t)kb * t.slab / splits);
+    t.k1 = static_cast<int>((int64_t)kb * (t.slab + 1) / splits);
+    return t;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    uint32_t r;
+    if (BF16)
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                             uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+
+template <int EPI, bool BF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_out, const GemmArgs args) {
+    using Shape = GemmShape<EPI>;
+    constexpr int kStages = Shape::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ alignas(8) uint64_t bars[2 * kStages + 4];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int stop_flag;
+    volatile int* stop = &stop_flag;
+
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kStages;
+    const uint32_t acc_full0 = empty0 + 8 * kStages, acc_empty0 = acc_full0 + 16;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(acc_full0 + 8 * s, 1);
+            mbar_init(acc_empty0 + 8 * s, 2 * kEpiWarps);
+        }
+        mbar_init_fence();
+        tma_prefetch_map(&map_a);
+        tma_prefetch_map(&map_b);
+        if (EPI != kEpiStats) tma_prefetch_map(&map_out);
+    }
+    if (warp == 2) tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
+    if (threadIdx.x == 0) stop_flag = args.meta[kMetaStop];  // an earlier kernel of the call gave up
+    const int rows = args.packed ? args.meta[kMetaRows] : args.rows;
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // the other CTA's barriers exist from here on
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    const int m_ext = args.m_extent < 0 ? rows : args.m_extent;
+    const int k_ext = args.k_extent < 0 ? rows : args.k_extent;
+    const int mt = max(1, (m_ext + kTile - 1) / kTile);
+    const int nt = (args.n_extent + kTile - 1) / kTile;
+    const int kb_total = max(1, (k_ext + kBlockK - 1) / kBlockK);
+    const int units = mt * nt * args.splits;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    if (warp == 0) {
+        // ---- copies ----
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            for (int u = pair; u < units && !*stop; u += pairs) {
+                const Unit t = decode_unit(u, mt, nt, args.splits, kb_total);
+                const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * kTile + rank * kHalfTile;
+                for (int kb = t.k0; kb < t.k1; ++kb) {
+                    if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, stop)) break;
+                    const uint32_t bar = map_to_rank(full0 + 8 * stage, 0);
+                    const uint32_t sa = smem + stage * kStageBytes, sb = sa + kOperandBytes;
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * stage, kStageTx);
+                    const int k = kb * kBlockK;
+                    if (Shape::kAMn) {
+                        tma_load_pair(sa, &map_a, bar, ma, k);
+                        tma_load_pair(sa + kOperandBytes / 2, &map_a, bar, ma + 64, k);
+                    } else {
+                        tma_load_pair(sa, &map_a, bar, k, ma);
+                    }
+                    if (Shape::kBMn) {
+                        tma_load_pair(sb, &map_b, bar, nb, args.b_offset + k);
+                        tma_load_pair(sb + kOperandBytes / 2, &map_b, bar, nb + 64, args.b_offset + k);
+                    } else {
+                        tma_load_pair(sb, &map_b, bar, k, args.b_offset + nb);
+                    }
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---- products, issued by the pair's first CTA for both ----
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t lead_a = Shape::kAMn ? kOperandBytes / 2 : 16;
+            constexpr uint32_t lead_b = Shape::kBMn ? kOperandBytes / 2 : 16;
+            // 16 deep in K: 32 bytes along a K-major row, two 8-row groups of an MN-major tile
+            constexpr uint32_t step_a = Shape::kAMn ? 2048 >> 4 : 32 >> 4;
+            constexpr uint32_t step_b = Shape::kBMn ? 2048 >> 4 : 32 >> 4;
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+            for (int u = pair; u < units && !*stop; u += pairs) {
+                const Unit t = decode_unit(u, mt, nt, args.splits, kb_total);
+                if (t.k0 == t.k1) continue;
+                if (!mbar_wait(acc_empty0 + 8 * acc, acc_phase ^ 1, stop)) break;
+                tc_fence_after();
+                bool ok = true;
+                for (int kb = t.k0; kb < t.k1; ++kb) {
+                    ok = mbar_wait(full0 + 8 * stage, phase, stop);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t sa = smem + stage * kStageBytes;
+                    const uint64_t da = umma_desc(sa, lead_a), db = umma_desc(sa + kOperandBytes, lead_b);
+#pragma unroll
+                    for (int k = 0; k < kBlockK / 16; ++k)
+                        umma_pair(tmem + acc * kTile, da + k * step_a, db + k * step_b, args.idesc,
+                                  kb != t.k0 || k != 0);
+                    umma_commit_pair(empty0 + 8 * stage);
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                }
+                if (!ok) break;
+                umma_commit_pair(acc_full0 + 8 * acc);
+                if ((acc ^= 1) == 0) acc_phase ^= 1;
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ---- epilogue: warp quarter q reads lanes (rows) 32q.., half h columns 128h.. ----
+        const int q = warp & 3, h = (warp - 4) >> 2;
+        const uint32_t staging = smem + kStages * kStageBytes + (warp - 4) * 2 * kStagingBuf;
+        const uint32_t srow = lane * 128, sxor = lane & 7;
+        const uint32_t empty_leader = map_to_rank(acc_empty0, 0);
+        float scale = 1.0f;
+        if (EPI == kEpiOut16) scale = __ldg(args.inv_scale);
+        uint32_t acc = 0, acc_phase = 0;
+        for (int u = pair; u < units; u += pairs) {
+            const Unit t = decode_unit(u, mt, nt, args.splits, kb_total);
+            if (t.k0 == t.k1) continue;
+            const int row0 = t.m * kTile + rank * kHalfTile + q * 32, row = row0 + lane;
+            const int col0 = t.n * kTile + h * kHalfTile;
+            // a warp whose rows are all past the end has nothing to write, except that dz is
+            // defined (zero) on whole 64-row blocks: the weight gradient sums over those
+            const bool busy = EPI == kEpiGradZ ? row0 < max(64, (rows + 63) & ~63) : row0 < m_ext;
+            int64_t tcol = -1;
+            float lse = 0.0f, a = 0.0f, b = 0.0f;
+            if ((EPI == kEpiStats || EPI == kEpiGradZ) && row < rows) {
+                tcol = __ldg(args.target + (args.src ? __ldg(args.src + row) : row));
+                tcol = tcol < 0 ? -1 : tcol - (EPI == kEpiGradZ ? args.b_offset : 0) - col0;
+                if (EPI == kEpiGradZ) {
+                    lse = __ldg(args.lse + row);
+                    a = __ldg(args.a + row);
+                    b = __ldg(args.b + row);
+                }
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * acc, acc_phase, stop))) break;
+            tc_fence_after();
+            if (busy) {
+                const uint32_t base = tmem + acc * kTile + h * kHalfTile + (static_cast<uint32_t>(q * 32) << 16);
+                float m = -INFINITY, s = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32(base + 32 * c, r);
+                    tmem_wait_ld(r);
+                    const int cc = col0 + 32 * c;
+                    const bool here = tcol >= 32 * c && tcol < 32 * c + 32;  // the target's column
+                    if (EPI == kEpiStats) {
+                        float v[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+                        if (cc + 32 > args.n_extent) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (cc + j >= args.n_extent) v[j] = -INFINITY;
+                        }
+                        if (here) {
+                            float z = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (tcol == 32 * c + j) z = v[j];
+                            if (col0 + tcol < args.n_extent) args.zt[row] = z;
+                        }
+                        ms_fold<32>(m, s, v);
+                    } else if (EPI == kEpiGradZ || EPI == kEpiOut16) {
+                        float v[32];
+                        if (EPI == kEpiGradZ) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = a * exp_from(__uint_as_float(r[j]), lse);
+                            if (here) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (tcol == 32 * c + j) v[j] -= b;
+                            }
+                            // rows and columns past the end are zero whatever was staged there
+                            if (row >= rows || cc + 32 > args.n_extent) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (row >= rows || cc + j >= args.n_extent) v[j] = 0.0f;
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * scale;
+                        }
+                        const uint32_t buf = staging + (c >> 1) * kStagingBuf;
+                        if ((c & 1) == 0) {
+                            if (lane == 0) tma_store_wait_read<1>();
+                            __syncwarp();
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t chunk = (c & 1) * 4 + j;
+                            st_shared_v4(buf + srow + ((chunk ^ sxor) << 4),
+                                         pack16<BF16>(v[8 * j], v[8 * j + 1]),
+                                         pack16<BF16>(v[8 * j + 2], v[8 * j + 3]),
+                                         pack16<BF16>(v[8 * j + 4], v[8 * j + 5]),
+                                         pack16<BF16>(v[8 * j + 6], v[8 * j + 7]));
+                        }
+                        if ((c & 1) == 1) {
+                            fence_async_smem();
+                            __syncwarp();
+                            // a box that starts past the edge is not stored at all
+                            const int x = col0 + 64 * (c >> 1);
+                            if (lane == 0 && (EPI == kEpiGradZ ? row0 < args.rows : x < args.n_extent))
+                                tma_store(&map_out, buf, x, args.out_row + row0);
+                            if (lane == 0) tma_store_commit();
+                        }
+                    } else {
+                        const uint32_t buf = staging + (c & 1) * kStagingBuf;
+                        if (lane == 0) tma_store_wait_read<1>();
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            st_shared_v4(buf + srow + ((static_cast<uint32_t>(j) ^ sxor) << 4), r[4 * j],
+                                         r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            const int y = t.slab * args.slab_rows + row0;
+                            if (cc < args.n_extent) {
+                                if (args.add)
+                                    tma_reduce_add(&map_out, buf, cc, y);
+                                else
+                                    tma_store(&map_out, buf, cc, y);
+                            }
+                            tma_store_commit();
+                        }
+                    }
+                }
+                if (EPI == kEpiStats && row < rows)
+                    args.part[(int64_t)row * args.pieces + 2 * t.n + h] = make_float2(m, s);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty_leader + 8 * acc);
+            if ((acc ^= 1) == 0) acc_phase ^= 1;
+        }
+        if (EPI != kEpiStats && lane == 0) tma_store_wait_all();
+        __syncwarp();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (*stop) {
+        // Leave copies in flight the time to land, then mark the call's outputs.
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 2000000) __nanosleep(1000);
+        if (threadIdx.x == 0) args.meta[kMetaStop] = 1;
+        if (EPI == kEpiOut16) {
+            const int64_t per = (args.out_elems + gridDim.x - 1) / gridDim.x;
+            const int64_t e0 = per * blockIdx.x, e1 = min(args.out_elems, e0 + per);
+            for (int64_t i = e0 + threadIdx.x; i < e1; i += kGemmThreads)
+                static_cast<uint16_t*>(args.out)[i] = 0x7fff;  // NaN in both 16-bit types
+        }
+    }
+    cluster_sync_all();  // no arrival or operand read of the other CTA is left
+    if (warp == 2) tmem_free_pair(tmem, kTmemCols);
+}
+
+// ---------------------------------------------------------------------------
+// Packing: the rows that have a target, in order, as dense 16-byte-aligned rows
+// ---------------------------------------------------------------------------
+constexpr int kPackThreads = 256;
+
+// One warp copies D 16-bit elements and zeroes up to Dp.
+__device__ __forceinline__ void copy_row16(const uint16_t* s, uint16_t* d, int D, int Dp, int lane) {
+    if (((reinterpret_cast<uintptr_t>(s) | reinterpret_cast<uintptr_t>(d)) & 15u) == 0) {
+        const int nv = D / 8;
+        for (int i = lane; i < nv; i += 32)
+            reinterpret_cast<uint4*>(d)[i] = __ldg(reinterpret_cast<const uint4*>(s) + i);
+        for (int i = nv * 8 + lane; i < D; i += 32) d[i] = __ldg(s + i);
+    } else {
+        for (int i = lane; i < D; i += 32) d[i] = __ldg(s + i);
+    }
+    for (int i = D + lane; i < Dp; i += 32) d[i] = 0;
+}
+
+__device__ __forceinline__ int block_sum(int v, int* sh) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    int t = 0;
+#pragma unroll
+    for (int w = 0; w < kPackThreads / 32; ++w) t += sh[w];
+    return t;
+}
+
+// Each CTA takes a contiguous range of rows; it counts the kept rows before the
+// range itself (the targets are a few KB that L2 serves), so one launch does it.
+// pos[row] = packed position or -1, src[position] = row.
+__global__ void __launch_bounds__(kPackThreads) pack_rows_kernel(
+    const uint16_t* __restrict__ hidden, const int64_t* __restrict__ target, int64_t ignore,
+    uint16_t* __restrict__ packed, int* __restrict__ src, int* __restrict__ pos, int* __restrict__ meta,
+    int N, int D, int Dp, RowMap rm) {
+    __shared__ int sh[kPackThreads / 32];
+    __shared__ int list[kPackThreads];
+    const int r0 = static_cast<int>((int64_t)blockIdx.x * N / gridDim.x);
+    const int r1 = static_cast<int>((int64_t)(blockIdx.x + 1) * N / gridDim.x);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int before = 0;
+    for (int r = threadIdx.x; r < r0; r += kPackThreads) before += __ldg(target + r) != ignore;
+    int base = block_sum(before, sh);
+    for (int c = r0; c < r1; c += kPackThreads) {
+        const int r = c + threadIdx.x;
+        const bool keep = r < r1 && __ldg(target + r) != ignore;
+        const uint32_t ballot = __ballot_sync(0xffffffffu, keep);
+        __syncthreads();
+        if (lane == 0) sh[warp] = __popc(ballot);
+        __syncthreads();
+        int at = __popc(ballot & ((1u << lane) - 1)), n = 0;
+        for (int w = 0; w < kPackThreads / 32; ++w) {
+            if (w < warp) at += sh[w];
+            n += sh[w];
+        }
+        if (r < r1) pos[r] = keep ? base + at : -1;
+        if (keep) {
+            src[base + at] = r;
+            list[at] = r;
+        }
+        __syncthreads();
+        for (int i = warp; i < n; i += kPackThreads / 32)
+            copy_row16(hidden + rm(list[i]), packed + (int64_t)(base + i) * Dp, D, Dp, lane);
+        base += n;
+    }
+    if (blockIdx.x == gridDim.x - 1) {
+        // the weight gradient sums over whole blocks of 64 packed rows
+        const int end = min(N, max(kBlockK, (base + kBlockK - 1) / kBlockK * kBlockK));
+        for (int i = base + warp; i < end; i += kPackThreads / 32)
+            for (int j = lane; j < Dp; j += 32) packed[(int64_t)i * Dp + j] = 0;
+        if (threadIdx.x == 0) {
+            meta[kMetaRows] = base;
+            meta[kMetaCount] = 0;
+            meta[kMetaStop] = 0;
+        }
+    }
+}
+
+// Rows of D 16-bit elements to rows of Dp >= D (zero-filled) at stride Dp or,
+// with Dp < D, their first Dp elements.
+__global__ void __launch_bounds__(256) copy_rows16_kernel(const uint16_t* __restrict__ src,
+                                                          uint16_t* __restrict__ dst, int64_t rows, int D,
+                                                          int Dp, RowMap rm) {
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row < rows)
+        copy_row16(src + rm(row), dst + row * Dp, min(D, Dp), Dp, threadIdx.x & 31);
+}
+
+// ---------------------------------------------------------------------------
+// Forward: merge a row's pieces, form its value, reduce
+// ---------------------------------------------------------------------------
+enum Reduce { kLogp = 0, kNone = 1, kSum = 2, kMean = 3 };
+
+__global__ void __launch_bounds__(256) finish_forward_kernel(
+    const float2* __restrict__ part, int pieces, const float* __restrict__ zt,
+    const int64_t* __restrict__ target, const int* __restrict__ pos, int* meta, int64_t N, int64_t V,
+    float z_loss, int reduce, float* __restrict__ lse_out, float* values, float* __restrict__ out,
+    int* err) {
+    __shared__ double sums[8];
+    __shared__ int last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float nan = __int_as_float(0x7fc00000);
+    for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < N; row += (int64_t)gridDim.x * 8) {
+        const int64_t p = pos ? pos[row] : row;
+        float value = 0.0f;
+        if (p >= 0) {
+            float m = -INFINITY, s = 0.0f;
+            for (int i = lane; i < pieces; i += 32) {
+                const float2 v = __ldg(part + p * pieces + i);
+                ms_merge(m, s, v.x, v.y);
+            }
+            ms_warp_allreduce(m, s);
+            const float lse = ms_finalize(m, s, -INFINITY);
+            const int64_t t = __ldg(target + row);
+            const bool bad = t < 0 || t >= V;
+            if (lane == 0) {
+                lse_out[p] = lse;
+                if (bad && err) atomicOr(err, 1);
+            }
+            const float nll = bad || meta[kMetaStop] ? nan : lse - __ldg(zt + p);
+            value = reduce == kLogp ? -nll : nll;
+            if (z_loss != 0.0f) value += z_loss * lse * lse;
+        }
+        if (lane == 0) values[row] = value;
+    }
+    if (reduce == kLogp || reduce == kNone) return;  // values is the result
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(meta + kMetaCount, 1) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    // one CTA sums all rows in a fixed order, in 64 bits (long sums of like values)
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < N; i += 256) sum += __ldcg(values + i);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double total = 0.0;
+        for (int w = 0; w < 8; ++w) total += sums[w];
+        if (reduce == kMean) total /= meta[kMetaRows];
+        *out = static_cast<float>(total);
+        meta[kMetaCount] = 0;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Backward: row coefficients of dz, and the hidden gradient from its slabs
+// ---------------------------------------------------------------------------
+// dz = a softmax - b onehot, scaled by a power of two that brings the largest
+// coefficient to [2^13, 2^14): fp16 keeps its relative accuracy down to
+// probabilities of 1e-9 of it instead of flushing them.
+__global__ void __launch_bounds__(1024) coefficients_kernel(
+    const float* __restrict__ g, int reduce, float z_loss, const float* __restrict__ lse,
+    const int* __restrict__ src, const int* __restrict__ meta, int64_t N, float* __restrict__ a,
+    float* __restrict__ b, float* __restrict__ inv_scale) {
+    __shared__ float top[32];
+    const int64_t rows = src ? meta[kMetaRows] : N;
+    float g0 = 0.0f;
+    if (reduce == kSum) g0 = *g;
+    if (reduce == kMean) g0 = *g / static_cast<float>(rows);
+    auto coef = [&](int64_t r, float& ca, float& cb) {
+        cb = reduce >= kSum ? g0 : __ldg(g + (src ? src[r] : r));
+        if (reduce == kLogp) cb = -cb;
+        ca = z_loss != 0.0f ? cb * (1.0f + 2.0f * z_loss * lse[r]) : cb;
+    };
+    float big = 0.0f;
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+        float ca, cb;
+        coef(r, ca, cb);
+        big = fmaxf(big, fmaxf(fabsf(ca), fabsf(cb)));
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = big;
+    __syncthreads();
+    big = top[threadIdx.x & 31];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+    int e = 0;
+    if (big > 0.0f && big < INFINITY) e = min(max(14 - (ilogbf(big) + 1), -120), 120);
+    const float scale = scalbnf(1.0f, e);
+    if (threadIdx.x == 0) *inv_scale = scalbnf(1.0f, -e);
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+        float ca, cb;
+        coef(r, ca, cb);
+        a[r] = ca * scale;
+        b[r] = cb * scale;
+    }
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(256) finish_hidden_kernel(const float* __restrict__ slabs, int splits,
+                                                            int64_t slab_elems, const int* __restrict__ pos,
+                                                            const int* __restrict__ meta,
+                                                            const float* __restrict__ inv_scale, int D,
+                                                            int Dp, uint16_t* __restrict__ out) {
+    const int64_t row = blockIdx.x;
+    const int64_t p = pos ? pos[row] : row;
+    const float scale = meta[kMetaStop] ? __int_as_float(0x7fc00000) : *inv_scale;
+    uint16_t* o = out + row * D;
+    const float* s = slabs + p * Dp;
+    const bool wide = D % 4 == 0;
+    for (int j = 4 * (blockIdx.y * 256 + threadIdx.x); j < D; j += 4 * 256 * gridDim.y) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p >= 0) {
+            for (int k = 0; k < splits; ++k) {  // in the order of the vocabulary
+                const float4 w = __ldg(reinterpret_cast<const float4*>(s + k * slab_elems + j));
+                v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+            }
+            v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
+        }
+        const uint32_t lo = pack16<BF16>(v.x, v.y), hi = pack16<BF16>(v.z, v.w);
+        if (wide) {
+            *reinterpret_cast<uint2*>(o + j) = make_uint2(lo, hi);
+        } else {
+            const uint32_t w[2] = {lo, hi};
+            for (int i = 0; i < 4 && j + i < D; ++i) o[j + i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+constexpr int64_t kMaxExtent = INT32_MAX - 4 * kTile;
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// K pieces of the hidden gradient: as many as fill the CTA pairs best, at least
+// 8 blocks deep each and slabs of at most 64 MB in all (one slab is needed anyway).
+int choose_splits(int64_t tiles, int64_t kb, int64_t slab_bytes, int pairs) {
+    int best = 1;
+    double best_use = 0.0;
+    for (int s = 1; s <= 64; ++s) {
+        if (s > 1 && (kb / s < 8 || slab_bytes * s > (64 << 20))) break;
+        const int64_t units = tiles * s;
+        const double use = (double)units / (double)((units + pairs - 1) / pairs * pairs);
+        if (use > best_use * 1.02) best = s, best_use = use;
+    }
+    return best;
+}
+
+struct BwdPlan {
+    int64_t chunk;      // columns of a vocabulary piece, a multiple of 256
+    int splits;
+    int64_t slab_rows;
+    int64_t coef_off, slab_off, dz_off, bytes;
+};
+
+BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidden, int pairs) {
+    BwdPlan p;
+    const int64_t all = round_up(V, kTile);
+    // 512 MB of dz by default: the hidden gradient is added to once per piece
+    if (chunk <= 0) chunk = (256ll << 20) / std::max<int64_t>(N, 1);
+    p.chunk = std::min(all, std::max<int64_t>(kTile, chunk / kTile * kTile));
+    p.slab_rows = round_up(N, kTile);
+    const int64_t slab = p.slab_rows * Dp * 4;
+    p.splits = want_hidden ? choose_splits((p.slab_rows / kTile) * ((Dp + kTile - 1) / kTile),
+                                           p.chunk / kBlockK, slab, pairs)
+                           : 0;
+    p.coef_off = 256;
+    p.slab_off = p.coef_off + round_up(2 * N * 4, 256);
+    p.dz_off = p.slab_off + round_up(slab * p.splits, 256);
+    p.bytes = p.dz_off + round_up(N * p.chunk * 2, 256);
+    return p;
+}
+
+template <int EPI>
+int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GemmArgs& args,
+                   int64_t units, bool bf16, cudaStream_t stream, const char* what) {
+    auto kern = bf16 ? product_kernel<EPI, true> : product_kernel<EPI, false>;
+    constexpr uint32_t smem = GemmShape<EPI>::kSmem;
+    FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int64_t pairs = std::max<int64_t>(1, std::min<int64_t>(units, sm_count() / 2));
+    LaunchCfg lc(dim3((unsigned)(2 * pairs)), dim3(kGemmThreads), smem, stream, /*pdl=*/false);
+    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, a, b, out, args));
+    return check_launch(what);
+}
+
+constexpr CUtensorMapDataType kMap16[2] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16};
+
+int check_projection(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype, int64_t N,
+                     int64_t V, int64_t Dp, const char* what) {
+    FL_REQUIRE(dtype == 0 || dtype == 1, "%s: dtype must be 0 (fp16) or 1 (bf16)", what);
+    FL_REQUIRE(N >= 0 && V >= 1 && Dp >= 1, "%s: bad shape (%lld, %lld, %lld)", what, (long long)N,
+               (long long)V, (long long)Dp);
+    FL_REQUIRE(N <= kMaxExtent && V <= kMaxExtent && Dp <= (1 << 20), "%s: shape too large", what);
+    FL_REQUIRE(Dp % 8 == 0 && ldh % 8 == 0 && ldw % 8 == 0 && ldh >= Dp && ldw >= Dp,
+               "%s: rows must be a multiple of 8 elements apart and long", what);
+    FL_REQUIRE(ldh < (1ll << 38) && ldw < (1ll << 38), "%s: row stride too large", what);
+    FL_REQUIRE(N == 0 || (hidden && weight), "%s: NULL buffer", what);
+    FL_REQUIRE(aligned_to(hidden, 16) && aligned_to(weight, 16), "%s: operands must be 16-byte aligned", what);
+    // a unit index of the largest product (256 x 256 tiles times K pieces) fits 32 bits
+    FL_REQUIRE(((N + 255) / 256) * ((V + 255) / 256) <= INT32_MAX / 64 &&
+                   ((V + 255) / 256) * ((Dp + 255) / 256) <= INT32_MAX / 64 &&
+                   ((N + 255) / 256) * ((Dp + 255) / 256) <= INT32_MAX / 64,
+               "%s: shape too large", what);
+    return FL_OK;
+}
+
+int64_t fwd_bytes(int64_t N, int64_t V) {
+    return round_up(N * 2 * ((V + kTile - 1) / kTile) * 8, 256) + 2 * round_up(N * 4, 256);
+}
+
+}  // namespace
+}  // namespace fl
+
+using namespace fl;
+
+extern "C" int fl_linear_loss_workspace(int64_t N, int64_t V, int64_t D, int64_t vocab_chunk,
+                                        int want_hidden, int64_t* forward, int64_t* backward) {
+    clear_error();
+    const char* what = "fl_linear_loss_workspace";
+    if (int st = check_projection(nullptr, round_up(D, 8), nullptr, round_up(D, 8), 0, 0, V, round_up(D, 8),
+                                  what))
+        return st;
+    FL_REQUIRE(N >= 0 && N <= kMaxExtent && forward && backward, "%s: bad arguments", what);
+    FL_REQUIRE(vocab_chunk >= 0, "%s: vocab_chunk is negative", what);
+    *forward = fwd_bytes(N, V);
+    *backward = plan_bwd(N, V, round_up(D, 8), vocab_chunk, want_hidden != 0, sm_count() / 2).bytes;
+    return FL_OK;
+}
+
+extern "C" int fl_linear_loss_pack(const uint16_t* hidden, const int64_t* target, int64_t ignore_index,
+                                   uint16_t* packed, int* src, int* pos, int* meta, int64_t N, int64_t D,
+                                   int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
+                                   fl_stream_t stream) {
+    clear_error();
+    const char* what = "fl_linear_loss_pack";
+    FL_REQUIRE(N >= 0 && D >= 1 && N <= kMaxExtent && D <= (1 << 20), "%s: bad shape", what);
+    if (N == 0) return FL_OK;
+    FL_REQUIRE(hidden && target && packed && src && pos && meta, "%s: NULL buffer", what);
+    FL_REQUIRE(aligned_to(hidden, 2) && aligned_to(target, 8) && aligned_to(packed, 16) &&
+                   aligned_to(src, 4) && aligned_to(pos, 4) && aligned_to(meta, 4),
+               "%s: misaligned buffer", what);
+    RowMap rm = RowMap::dense(D);
+    if (rows_per_group >= 0) {
+        FL_REQUIRE(rows_per_group >= 1 && group_stride >= 0 && row_stride >= 0, "%s: bad row layout", what);
+        rm = RowMap{rows_per_group, group_stride, row_stride};
+    }
+    if (int st = bind_device(stream, packed)) return st;
+    const int64_t grid = std::min<int64_t>(N, 2 * sm_count());
+    LaunchCfg lc(dim3((unsigned)grid), dim3(kPackThreads), 0, reinterpret_cast<cudaStream_t>(stream), false);
+    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, pack_rows_kernel, hidden, target, ignore_index, packed, src, pos, meta,
+                               (int)N, (int)D, (int)round_up(D, 8), rm));
+    return check_launch(what);
+}
+
+extern "C" int fl_copy_rows16(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t D, int64_t Dp,
+                              int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
+                              fl_stream_t stream) {
+    clear_error();
+    const char* what = "fl_copy_rows16";
+    FL_REQUIRE(rows >= 0 && D >= 1 && Dp >= 1 && D <= (1 << 20) && Dp <= (1 << 20), "%s: bad shape", what);
+    if (rows == 0) return FL_OK;
+    FL_REQUIRE(src && dst && aligned_to(src, 2) && aligned_to(dst, 2), "%s: NULL or misaligned buffer", what);
+    RowMap rm = RowMap::dense(D);
+    if (rows_per_group >= 0) {
+        FL_REQUIRE(rows_per_group >= 1 && group_stride >= 0 && row_stride >= 0, "%s: bad row layout", what);
+        rm = RowMap{rows_per_group, group_stride, row_stride};
+    }
+    if (int st = bind_device(stream, dst)) return st;
+    const int64_t grid = (rows + 7) / 8;
+    FL_REQUIRE(grid <= INT32_MAX, "%s: too many rows", what);
+    LaunchCfg lc(dim3((unsigned)grid), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), false);
+    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, copy_rows16_kernel, src, dst, rows, (int)D, (int)Dp, rm));
+    return check_launch(what);
+}
+
+extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t ldh, const uint16_t* weight, int64_t ldw,
+                                  int dtype, const int64_t* target, const int* src, const int* pos, int* meta,
+                                  int64_t N, int64_t V, int64_t D, int reduce, float z_loss, float* lse,
+                                  float* out, void* workspace, int64_t workspace_bytes, int* err_flag,
+                                  fl_stream_t stream) {
+    clear_error();
+    const char* what = "fl_linear_loss_fwd";
+    if (int st = check_projection(hidden, ldh, weight, ldw, dtype, N, V, D, what)) return st;
+    FL_REQUIRE(reduce >= kLogp && reduce <= kMean, "%s: unknown reduction %d", what, reduce);
+    FL_REQUIRE((src == nullptr) == (pos == nullptr), "%s: src and pos come together", what);
+    FL_REQUIRE(src || reduce < kSum, "%s: a reduced loss needs packed rows", what);
+    if (N == 0) return FL_OK;
+    FL_REQUIRE(target && meta && lse && out && workspace, "%s: NULL buffer", what);
+    FL_REQUIRE(aligned_to(target, 8) && aligned_to(lse, 4) && aligned_to(out, 4) && aligned_to(err_flag, 4) &&
+                   aligned_to(workspace, 256),
+               "%s: misaligned buffer", what);
+    FL_REQUIRE(workspace_bytes >= fwd_bytes(N, V), "%s: workspace of %lld bytes, %lld needed", what,
+               (long long)workspace_bytes, (long long)fwd_bytes(N, V));
+    if (int st = bind_device(stream, lse)) return st;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const int64_t tiles_n = (V + kTile - 1) / kTile;
+    float2* part = static_cast<float2*>(workspace);
+    float* zt = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(N * 2 * tiles_n * 8, 256));
+    float* values = reduce < kSum ? out
+                                  : reinterpret_cast<float*>(reinterpret_cast<char*>(zt) + round_up(N * 4, 256));
+    if (!src) FL_CUDA(cudaMemsetAsync(meta, 0, 16, s));
+    CUtensorMap a, b;
+    if (int st = make_tensor_map(&a, kMap16[dtype], 2, hidden, D, N, ldh, kBlockK, kHalfTile)) return st;
+    if (int st = make_tensor_map(&b, kMap16[dtype], 2, weight, D, V, ldw, kBlockK, kHalfTile)) return st;
+    GemmArgs g = {};
+    g.rows = (int)N;
+    g.packed = src != nullptr;
+    g.m_extent = -1;
+    g.n_extent = (int)V;
+    g.k_extent = (int)D;
+    g.splits = 1;
+    g.idesc = umma_idesc(dtype == 1, false, false);
+    g.meta = meta;
+    g.target = target;
+    g.src = src;
+    g.part = part;
+    g.pieces = (int)(2 * tiles_n);
+    g.zt = zt;
+    if (int st = launch_product<kEpiStats>(a, b, a, g, ((N + kTile - 1) / kTile) * tiles_n, dtype == 1, s, what))
+        return st;
+    const int64_t grid = std::min<int64_t>((N + 7) / 8, 8ll * sm_count());
+    LaunchCfg lc(dim3((unsigned)grid), dim3(256), 0, s, false);
+    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, finish_forward_kernel, (const float2*)part, g.pieces, (const float*)zt,
+                               target, pos, meta, N, V, z_loss, reduce, lse, values, out, err_flag));
+    return check_launch(what);
+}
+
+extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int64_t ldh,
+                                  const uint16_t* weight, int64_t ldw, int dtype, const int64_t* target,
+                                  const int* src, const int* pos, int* meta, const float* lse, int64_t N,
+                                  int64_t V, int64_t D, int64_t hidden_cols, int reduce, float z_loss,
+                                  int64_t vocab_chunk, uint16_t* grad_hidden, uint16_t* grad_weight,
+                                  void* workspace, int64_t workspace_bytes, fl_stream_t stream) {
+    clear_error();
+    const char* what = "fl_linear_loss_bwd";
+    if (int st = check_projection(hidden, ldh, weight, ldw, dtype, N, V, D, what)) return st;
+    FL_REQUIRE(reduce >= kLogp && reduce <= kMean, "%s: unknown reduction %d", what, reduce);
+    FL_REQUIRE((src == nullptr) == (pos == nullptr) && (src || reduce < kSum), "%s: bad packing", what);
+    FL_REQUIRE(vocab_chunk >= 0, "%s: vocab_chunk is negative", what);
+    FL_REQUIRE(hidden_cols >= 1 && hidden_cols <= D, "%s: bad hidden_cols", what);
+    if (!grad_hidden && !grad_weight) return FL_OK;
+    FL_REQUIRE(grad_weight == nullptr || aligned_to(grad_weight, 16), "%s: misaligned buffer", what);
+    if (N == 0) {
+        if (!grad_weight) return FL_OK;
+        if (int st = bind_device(stream, grad_weight)) return st;
+        FL_CUDA(cudaMemsetAsync(grad_weight, 0, (size_t)(V * D * 2), reinterpret_cast<cudaStream_t>(stream)));
+        return FL_OK;
+    }
+    FL_REQUIRE(grad && target && meta && lse && workspace, "%s: NULL buffer", what);
+    FL_REQUIRE(aligned_to(grad, 4) && aligned_to(target, 8) && aligned_to(lse, 4) &&
+                   aligned_to(grad_hidden, 8) && aligned_to(workspace, 256),
+               "%s: misaligned buffer", what);
+    if (int st = bind_device(stream, workspace)) return st;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const int pairs = sm_count() / 2;
+    const BwdPlan plan = plan_bwd(N, V, D, vocab_chunk, grad_hidden != nullptr, pairs);
+    FL_REQUIRE(workspace_bytes >= plan.bytes, "%s: workspace of %lld bytes, %lld needed", what,
+               (long long)workspace_bytes, (long long)plan.bytes);
+    FL_REQUIRE(plan.slab_rows * std::max(plan.splits, 1) <= kMaxExtent, "%s: shape too large", what);
+    char* ws = static_cast<char*>(workspace);
+    float* inv_scale = reinterpret_cast<float*>(ws);
+    float* ca = reinterpret_cast<float*>(ws + plan.coef_off);
+    float* cb = ca + N;
+    float* slabs = reinterpret_cast<float*>(ws + plan.slab_off);
+    uint16_t* dz = reinterpret_cast<uint16_t*>(ws + plan.dz_off);
+    const bool bf16 = dtype == 1;
+    {
+        LaunchCfg lc(dim3(1), dim3(1024), 0, s, false);
+        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, coefficients_kernel, grad, reduce, z_loss, lse, src,
+                                   (const int*)meta, N, ca, cb, inv_scale));
+        if (int st = check_launch(what)) return st;
+    }
+    // operand and output views: hidden and weight by rows and by columns, dz both ways
+    CUtensorMap h_k, w_k, dz_out, dz_mn, h_mn, dw_out, dz_k, w_mn, slab_out;
+    if (int st = make_tensor_map(&h_k, kMap16[dtype], 2, hidden, D, N, ldh, kBlockK, kHalfTile)) return st;
+    if (int st = make_tensor_map(&w_k, kMap16[dtype], 2, weight, D, V, ldw, kBlockK, kHalfTile)) return st;
+    if (int st = make_tensor_map(&dz_out, kMap16[dtype], 2, dz, plan.chunk, N, plan.chunk, 64, 32)) return st;
+    if (grad_weight) {
+        if (int st = make_tensor_map(&dz_mn, kMap16[dtype], 2, dz, plan.chunk, N, plan.chunk, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&h_mn, kMap16[dtype], 2, hidden, D, N, ldh, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&dw_out, kMap16[dtype], 2, grad_weight, D, V, D, 64, 32)) return st;
+    }
+    if (grad_hidden) {
+        if (int st = make_tensor_map(&dz_k, kMap16[dtype], 2, dz, plan.chunk, N, plan.chunk, kBlockK, kHalfTile))
+            return st;
+        if (int st = make_tensor_map(&w_mn, kMap16[dtype], 2, weight, D, V, ldw, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&slab_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, slabs, D,
+                                     plan.slab_rows * plan.splits, D, 32, 32))
+            return st;
+    }
+    GemmArgs base = {};
+    base.rows = (int)N;
+    base.packed = src != nullptr;
+    base.splits = 1;
+    base.meta = meta;
+    const int64_t mt = (N + kTile - 1) / kTile, dt = (D + kTile - 1) / kTile;
+    for (int64_t v0 = 0; v0 < V; v0 += plan.chunk) {
+        const int64_t cv = std::min(plan.chunk, V - v0), ct = (cv + kTile - 1) / kTile;
+        GemmArgs g = base;
+        g.m_extent = -1;
+        g.n_extent = (int)cv;
+        g.k_extent = (int)D;
+        g.b_offset = (int)v0;
+        g.idesc = umma_idesc(bf16, false, false);
+        g.target = target;
+        g.src = src;
+        g.lse = lse;
+        g.a = ca;
+        g.b = cb;
+        if (int st = launch_product<kEpiGradZ>(h_k, w_k, dz_out, g, mt * ct, bf16, s, what)) return st;
+        if (grad_weight) {
+            g = base;
+            g.m_extent = (int)cv;
+            g.n_extent = (int)D;
+            g.k_extent = -1;
+            g.out_row = (int)v0;
+            g.idesc = umma_idesc(bf16, true, true);
+            g.inv_scale = inv_scale;
+            g.out = grad_weight;
+            g.out_elems = V * D;
+            if (int st = launch_product<kEpiOut16>(dz_mn, h_mn, dw_out, g, ct * dt, bf16, s, what)) return st;
+        }
+        if (grad_hidden) {
+            g = base;
+            g.m_extent = -1;
+            g.n_extent = (int)D;
+            g.k_extent = (int)cv;
+            g.b_offset = (int)v0;
+            g.splits = plan.splits;
+            g.slab_rows = (int)plan.slab_rows;
+            g.add = v0 > 0;
+            g.idesc = umma_idesc(bf16, false, true);
+            if (int st = launch_product<kEpiSlab>(dz_k, w_mn, slab_out, g, mt * dt * plan.splits, bf16, s, what))
+                return st;
+        }
+    }
+    if (grad_hidden) {
+        auto kern = bf16 ? finish_hidden_kernel<true> : finish_hidden_kernel<false>;
+        const int64_t gy = std::min<int64_t>(8, (hidden_cols + 1023) / 1024);
+        LaunchCfg lc(dim3((unsigned)N, (unsigned)gy), dim3(256), 0, s, false);
+        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, (const float*)slabs, plan.splits, plan.slab_rows * D, pos,
+                                   (const int*)meta, (const float*)inv_scale, (int)hidden_cols, (int)D,
+                                   grad_hidden));
+        return check_launch(what);
+    }
+    return FL_OK;
+}

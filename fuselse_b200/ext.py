@@ -175,6 +175,156 @@ def selective_logsoftmax_backward(grad_output: torch.Tensor, x: torch.Tensor, ls
 
 
 # --------------------------------------------------------------------------
+# Losses from hidden states and the output projection (no reference kernel)
+# --------------------------------------------------------------------------
+_DTYPE16 = {torch.float16: 0, torch.bfloat16: 1}
+_LOSS_LOGP = 0
+
+
+def check_linear_loss(what: str, hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor) -> None:
+    """The argument checks of linear_cross_entropy and linear_selective_log_softmax."""
+    for t, name in ((hidden, "hidden"), (weight, "weight"), (target, "target")):
+        _check(isinstance(t, torch.Tensor), f"{what}: {name} must be a tensor")
+    _check(hidden.dtype in _DTYPE16 and weight.dtype == hidden.dtype,
+           f"{what}: hidden and weight must both be fp16 or both bf16 "
+           f"(got {hidden.dtype} and {weight.dtype})")
+    _check(target.dtype in (torch.int64, torch.int32), f"{what}: the targets must be int64 or int32")
+    _check(hidden.dim() >= 1 and weight.dim() == 2, f"{what}: hidden (..., D) and weight (V, D) expected")
+    _check(hidden.shape[-1] == weight.shape[1],
+           f"{what}: hidden has {hidden.shape[-1]} columns, weight {weight.shape[1]}")
+    _check(weight.shape[0] >= 1 and weight.shape[1] >= 1, f"{what}: weight is empty")
+    _check(target.shape == hidden.shape[:-1],
+           f"{what}: targets of shape {tuple(hidden.shape[:-1])} expected, got {tuple(target.shape)}")
+    _check(hidden.is_cuda and weight.is_cuda and target.is_cuda, f"{what}: the tensors must be CUDA")
+    _check(weight.device == hidden.device and target.device == hidden.device,
+           f"{what}: the tensors must be on one device")
+
+
+def _u16(t):
+    return ptr(t, ctypes.c_uint16)
+
+
+def _tma_rows(t: torch.Tensor) -> bool:
+    """Whether (R, D) rows can be copied by a tensor map as they lie."""
+    return (t.shape[1] % 8 == 0 and t.stride(1) == 1 and t.data_ptr() % 16 == 0
+            and (t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])))
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _padded_rows(t: torch.Tensor) -> torch.Tensor:
+    """(R, D) rows as dense rows of D rounded up to 8 elements."""
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        t = t.contiguous()
+    R, D = t.shape
+    out = torch.empty((R, (D + 7) // 8 * 8), dtype=t.dtype, device=t.device)
+    if R:
+        call("fl_copy_rows16", _u16(t), _u16(out), R, D, out.shape[1], R, 0, t.stride(0), _stream(t))
+    return out
+
+
+def linear_loss_workspace_bytes(N: int, V: int, D: int, vocab_chunk: int = 0,
+                                want_hidden: bool = True) -> tuple[int, int]:
+    """Bytes of scratch that linear_loss_forward and linear_loss_backward allocate."""
+    fwd, bwd = ctypes.c_int64(), ctypes.c_int64()
+    call("fl_linear_loss_workspace", N, V, D, vocab_chunk, int(want_hidden), ctypes.byref(fwd),
+         ctypes.byref(bwd))
+    return fwd.value, bwd.value
+
+
+def linear_loss_forward(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduce: int,
+                        ignore_index: int | None = None, z_loss: float = 0.0, err_flag=None):
+    """(out, state): reduce 0 log-probabilities, 1 losses (both like target), 2 their
+    sum, 3 their mean over the kept rows.  Rows whose target is `ignore_index` are
+    left out (None: all rows are kept; needed by 2 and 3).  state is
+    (packed, padded, src, pos, meta, lse) for linear_loss_backward: packed / padded
+    are None where hidden / weight are used as they lie."""
+    check_linear_loss("linear_loss_forward", hidden, weight, target)
+    V, D = weight.shape
+    N, shape = target.numel(), target.shape
+    dev = hidden.device
+    with torch.cuda.device(dev):
+        stream = _stream(hidden)
+        target = target.reshape(-1).to(torch.int64).contiguous()
+        padded = None if _tma_rows(weight) else _padded_rows(weight)
+        w = weight if padded is None else padded
+        packed = src = pos = None
+        lay = row_layout(hidden)
+        if lay is None:  # neither packing nor the products can address these rows
+            hidden = packed = hidden.reshape(N, D).contiguous()
+            lay = row_layout(hidden)
+        meta = torch.empty(4, dtype=torch.int32, device=dev)
+        lse = torch.empty(N, dtype=torch.float32, device=dev)
+        one_level = lay[3] == 0  # the rows are one stride apart
+        rows = hidden.as_strided((N, D), (lay[4], 1)) if one_level and N else None
+        if ignore_index is not None:
+            packed = torch.empty((N, w.shape[1]), dtype=hidden.dtype, device=dev)
+            src, pos = torch.empty((2, N), dtype=torch.int32, device=dev).unbind(0)
+            call("fl_linear_loss_pack", _u16(hidden), ptr(target, ctypes.c_int64), ignore_index,
+                 _u16(packed), ptr(src, ctypes.c_int), ptr(pos, ctypes.c_int), ptr(meta, ctypes.c_int),
+                 N, D, lay[2], lay[3], lay[4], stream)
+            rows = packed
+        elif N and not (rows is not None and _tma_rows(rows)):
+            packed = torch.empty((N, w.shape[1]), dtype=hidden.dtype, device=dev)
+            call("fl_copy_rows16", _u16(hidden), _u16(packed), N, D, w.shape[1], lay[2], lay[3], lay[4],
+                 stream)
+            rows = packed
+        out = torch.empty(shape if reduce < 2 else (), dtype=torch.float32, device=dev)
+        if N == 0:
+            if reduce >= 2:
+                out.fill_(float("nan") if reduce == 3 else 0.0)
+        else:
+            need, _ = linear_loss_workspace_bytes(N, V, D)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            call("fl_linear_loss_fwd", _u16(rows), _row_stride(rows), _u16(w), _row_stride(w),
+                 _DTYPE16[hidden.dtype], ptr(target, ctypes.c_int64), ptr(src, ctypes.c_int),
+                 ptr(pos, ctypes.c_int), ptr(meta, ctypes.c_int), N, V, w.shape[1], reduce, z_loss,
+                 ptr(lse), ptr(out), ctypes.c_void_p(ws.data_ptr()), need,
+                 ptr(err_flag, ctypes.c_int), stream)
+    return out, (packed, padded, src, pos, meta, lse)
+
+
+def linear_loss_backward(grad_output: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor,
+                         target: torch.Tensor, src, pos, meta: torch.Tensor, lse: torch.Tensor,
+                         hidden_cols: int, reduce: int, z_loss: float = 0.0, vocab_chunk: int = 0,
+                         want_hidden: bool = True, want_weight: bool = True):
+    """(grad_hidden (N, hidden_cols), grad_weight (V, hidden_cols)) of linear_loss_forward,
+    None where not wanted; hidden and weight as its state gives them (the packed or padded
+    copies where it made any)."""
+    V, Dp = weight.shape
+    N, D = target.numel(), hidden_cols
+    dev = weight.device
+    if not (want_hidden or want_weight):
+        return None, None
+    with torch.cuda.device(dev):
+        stream = _stream(weight)
+        g = grad_output.to(torch.float32).reshape(-1).contiguous()
+        _check(g.numel() == (1 if reduce >= 2 else N), "grad_output does not match the forward's output")
+        target = target.reshape(-1).to(torch.int64).contiguous()
+        grad_hidden = torch.empty((N, D), dtype=weight.dtype, device=dev) if want_hidden else None
+        grad_weight = torch.empty((V, Dp), dtype=weight.dtype, device=dev) if want_weight else None
+        if N:
+            lay = row_layout(hidden)
+            rows = hidden.as_strided((N, Dp), (lay[4], 1))
+            _, need = linear_loss_workspace_bytes(N, V, Dp, vocab_chunk, want_hidden)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            call("fl_linear_loss_bwd", ptr(g), _u16(rows), _row_stride(rows), _u16(weight),
+                 _row_stride(weight), _DTYPE16[weight.dtype], ptr(target, ctypes.c_int64),
+                 ptr(src, ctypes.c_int), ptr(pos, ctypes.c_int), ptr(meta, ctypes.c_int), ptr(lse), N, V,
+                 Dp, D, reduce, z_loss, vocab_chunk, _u16(grad_hidden), _u16(grad_weight),
+                 ctypes.c_void_p(ws.data_ptr()), need, stream)
+        elif want_weight:
+            grad_weight.zero_()
+        if want_weight and Dp != D:
+            cut = torch.empty((V, D), dtype=weight.dtype, device=dev)
+            call("fl_copy_rows16", _u16(grad_weight), _u16(cut), V, Dp, D, -1, 0, 0, stream)
+            grad_weight = cut
+    return grad_hidden, grad_weight
+
+
+# --------------------------------------------------------------------------
 # In-place layouts: strided rows and dim != -1 (no contiguous copy)
 # --------------------------------------------------------------------------
 def row_layout(x: torch.Tensor):

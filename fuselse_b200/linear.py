@@ -1,0 +1,101 @@
+"""Vocabulary losses straight from hidden states and the output projection.
+
+With z = hidden @ weight.T, (N, V) logits that are never kept:
+
+    linear_cross_entropy(hidden, weight, target)         the training loss, as
+        cross_entropy(z, target), optionally with z_loss * lse(z)^2 per token
+    linear_selective_log_softmax(hidden, weight, index)  z[i, index[i]] - lse(z[i]),
+        what selective_log_softmax gives on z: per-token log-probabilities for
+        scoring and for policy-gradient training
+
+Both read the operands once per pass in tensor-core tiles whose epilogue folds
+the logits into each row's log-sum-exp; the backward recomputes the tiles in
+pieces of the vocabulary and takes each piece to the gradients of hidden and
+weight.  No reference counterpart: the reference's callers hold the logits
+(experiment_rlhf_logsumexp/run_rlhf.py:145-157).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import ext
+
+_REDUCTIONS = {"none": 1, "sum": 2, "mean": 3}
+_LOGP = 0
+
+
+class LinearLoss(torch.autograd.Function):
+    """hidden (..., D), weight (V, D), target (...) -> loss or log-probabilities."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err_flag):
+        out, state = ext.linear_loss_forward(hidden, weight, target, reduce=reduce,
+                                             ignore_index=ignore_index, z_loss=z_loss, err_flag=err_flag)
+        packed, padded, src, pos, meta, lse = state
+        # an operand used as it lies is saved as the input it is, a copy as what it is
+        ctx.save_for_backward(hidden if packed is None else packed, weight if padded is None else padded,
+                              target, src, pos, meta, lse)
+        ctx.shapes = hidden.shape, weight.shape
+        ctx.config = reduce, z_loss, vocab_chunk
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        hidden, weight, target, src, pos, meta, lse = ctx.saved_tensors
+        reduce, z_loss, vocab_chunk = ctx.config
+        grad_hidden, grad_weight = ext.linear_loss_backward(
+            grad_output, hidden, weight, target, src, pos, meta, lse, hidden_cols=ctx.shapes[0][-1],
+            reduce=reduce, z_loss=z_loss, vocab_chunk=vocab_chunk,
+            want_hidden=ctx.needs_input_grad[0], want_weight=ctx.needs_input_grad[1])
+        if grad_hidden is not None:
+            grad_hidden = grad_hidden.view(ctx.shapes[0])
+        return grad_hidden, grad_weight, None, None, None, None, None, None
+
+
+def _apply(what, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, check_index):
+    ext.check_linear_loss(what, hidden, weight, target)
+    if vocab_chunk is None:
+        vocab_chunk = 0
+    elif isinstance(vocab_chunk, bool) or not isinstance(vocab_chunk, int) or vocab_chunk < 1:
+        raise RuntimeError(f"{what}: vocab_chunk must be a positive int or None")
+    target = target.to(torch.int64)
+    err = torch.zeros(1, dtype=torch.int32, device=hidden.device) if check_index else None
+    out = LinearLoss.apply(hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err)
+    if check_index and int(err.item()):
+        raise RuntimeError(f"{what}: index out of range for {weight.shape[0]} classes")
+    return out
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *,
+                         ignore_index: int = -100, reduction: str = "mean", z_loss: float = 0.0,
+                         vocab_chunk: int | None = None, check_index: bool = False) -> torch.Tensor:
+    """Cross entropy of softmax(hidden @ weight.T) against `target`, fp32.
+
+    hidden (..., D) and weight (V, D) are CUDA fp16 or bf16 (the same), target
+    (...) integer.  Per token lse - z[target] + z_loss * lse^2; tokens whose
+    target is `ignore_index` give 0, take no part in the mean and are left out
+    of every product (their hidden states may hold anything).  reduction "mean"
+    (over the other tokens; NaN without any), "sum" or "none" (target.shape).
+    A target outside [0, V) gives NaN; with `check_index=True` it raises
+    RuntimeError instead (one device sync).  Gradients have the dtype of their
+    operands; the backward holds the logits' gradient of `vocab_chunk`
+    vocabulary entries at a time (None: at most 512 MB)."""
+    if reduction not in _REDUCTIONS:
+        raise RuntimeError(f"linear_cross_entropy: unknown reduction {reduction!r}")
+    return _apply("linear_cross_entropy", hidden, weight, target, _REDUCTIONS[reduction],
+                  int(ignore_index), float(z_loss), vocab_chunk, check_index)
+
+
+def linear_selective_log_softmax(hidden: torch.Tensor, weight: torch.Tensor, index: torch.Tensor, *,
+                                 vocab_chunk: int | None = None,
+                                 check_index: bool = False) -> torch.Tensor:
+    """Log-probabilities of `index` under softmax(hidden @ weight.T), fp32, shape
+    index.shape: selective_log_softmax(hidden @ weight.T, index) without the logits.
+
+    hidden (..., D) and weight (V, D) are CUDA fp16 or bf16 (the same), index
+    (...) integer.  An index outside [0, V) yields NaN; with `check_index=True`
+    it raises RuntimeError instead (one device sync).  Gradients and
+    `vocab_chunk` as in linear_cross_entropy."""
+    return _apply("linear_selective_log_softmax", hidden, weight, index, _LOGP, None, 0.0,
+                  vocab_chunk, check_index)

@@ -1,0 +1,73 @@
+"""Inputs, 64-bit formulas and error bounds of the linear_* loss tests.
+
+Bounds.  u = eps / 2 of the 16-bit type is one rounding.  A logit is a sum of D
+exact products in fp32: |dz| <= D 2^-23 (|h| @ |w|) (2^-23: the tensor cores may
+truncate).  The log-sum-exp is off by at most the largest logit error of its row
+plus its own arithmetic, held to 1e-5 max(|lse|, 1) as the other LSE tests hold
+it.  softmax is then off by a factor exp(e) with e the sum of the two, plus the
+exponential's 2^-22.  The logits' gradient is rounded once (u of its value),
+the products with weight and hidden add V or N terms of fp32 (2^-23 each), and
+the result is rounded once more; an fp16 result below its normal range by at
+most half its spacing, 2^-25.
+"""
+import torch
+
+F64 = torch.float64
+
+
+def make(N, D, V, dtype, seed=0, spread=2.0, dev="cuda"):
+    g = torch.Generator(device="cpu").manual_seed(seed + 7 * N + 11 * D + 13 * V)
+    w = (torch.randn(V, D, generator=g) * (spread / D ** 0.5)).to(dtype)
+    t = torch.randint(0, V, (N,), generator=g)
+    if N >= 3:
+        t[0], t[1], t[2] = 0, V - 1, V // 2
+    h = torch.randn(N, D, generator=g) + 2.0 * torch.rand(N, 1, generator=g) * w[t].float()
+    up = torch.randn(N, generator=g)
+    return h.to(dtype).to(dev), w.to(dev), t.to(dev), up.to(dev)
+
+
+def reference(h, w, t, coef, z_loss=0.0, sign=1.0):
+    """64-bit per-row value sign * (lse - z_t) + z_loss lse^2 and, for row coefficients
+    coef = d loss / d value, the gradients; with the elementwise error bounds above."""
+    N, D = h.shape
+    V = w.shape[0]
+    u = torch.finfo(h.dtype).eps / 2
+    tiny = 2.0 ** -25 if h.dtype == torch.float16 else 0.0
+    hd, wd = h.to(F64), w.to(F64)
+    z = hd @ wd.t()
+    lse = torch.logsumexp(z, -1)
+    rows = torch.arange(N, device=h.device)
+    nll = lse - z[rows, t]
+    value = sign * nll + z_loss * lse ** 2
+    zerr = D * 2.0 ** -23 * (hd.abs() @ wd.abs().t())
+    lerr = zerr.amax(-1) + 1e-5 * lse.abs().clamp_min(1.0)
+    verr = lerr + zerr[rows, t] + 2.0 ** -23 * z.abs().amax(-1) + 2 * z_loss * lse.abs() * lerr \
+        + 2.0 ** -22 * value.abs()
+    p = torch.exp(z - lse[:, None])
+    a = coef * (sign + 2 * z_loss * lse)
+    b = coef * sign
+    dz = a[:, None] * p
+    dz[rows, t] -= b
+    perr = a.abs()[:, None] * p * (torch.expm1(zerr + lerr[:, None]) + 2.0 ** -22) \
+        + (2 * coef.abs() * z_loss * lerr)[:, None] * p
+    derr = perr + u * dz.abs() + 2.0 ** -22 * dz.abs()
+    dh, dw = dz @ wd, dz.t() @ hd
+    dherr = (derr + V * 2.0 ** -23 * dz.abs()) @ wd.abs() + u * dh.abs() + tiny
+    dwerr = (derr + N * 2.0 ** -23 * dz.abs()).t() @ hd.abs() + u * dw.abs() + tiny
+    return {"value": value, "lse": lse, "grad_hidden": dh, "grad_weight": dw, "value_err": verr,
+            "grad_hidden_err": dherr, "grad_weight_err": dwerr}
+
+
+def within(got, want, bound, what):
+    err = (got.to(F64) - want).abs()
+    ok = err <= bound
+    assert bool(ok.all()), (f"{what}: {int((~ok).sum())} of {ok.numel()} off, worst {err.max().item():.3g} "
+                            f"where {bound.flatten()[err.argmax()].item():.3g} is allowed")
+
+
+def rms_close(got, want, dtype, what, roundings=2.0):
+    """Independent roundings of the summands and of the result: their rms is below one
+    u each, so two together stay below 2 u of the whole's norm."""
+    u = torch.finfo(dtype).eps / 2
+    err = (got.to(F64) - want).norm() / want.norm().clamp_min(1e-300)
+    assert err <= roundings * u, f"{what}: rms error {err.item():.3g}, {roundings * u:.3g} allowed"

@@ -1,0 +1,368 @@
+"""linear_cross_entropy and linear_selective_log_softmax against 64-bit formulas
+(bounds derived in linear_loss_cases.py): sizes around every tile edge, both
+16-bit types, reductions, ignored tokens, strides, vocabulary pieces, graphs,
+streams, and special values."""
+import pytest
+import torch
+
+import fuselse_b200
+from fuselse_b200 import linear_cross_entropy, linear_selective_log_softmax
+from tests.linear_loss_cases import F64, make, reference, rms_close, within
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _logp_case(h, w, t, up, **kw):
+    h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+    logp = linear_selective_log_softmax(h, w, t, **kw)
+    gh, gw = torch.autograd.grad(logp, (h, w), up)
+    return logp.detach(), gh, gw
+
+
+def _check_logp(h, w, t, up, got, rms=True):
+    ref = reference(h, w, t, up.to(F64), sign=-1.0)
+    logp, gh, gw = got
+    assert logp.dtype == torch.float32 and gh.dtype == h.dtype and gw.dtype == w.dtype
+    within(logp, ref["value"], ref["value_err"], "logp")
+    within(gh, ref["grad_hidden"], ref["grad_hidden_err"], "grad_hidden")
+    within(gw, ref["grad_weight"], ref["grad_weight_err"], "grad_weight")
+    if rms:
+        rms_close(gh, ref["grad_hidden"], h.dtype, "grad_hidden")
+        rms_close(gw, ref["grad_weight"], w.dtype, "grad_weight")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("N,D,V", [(128, 64, 256), (256, 128, 512), (300, 200, 1000)])
+def test_logp_forward(N, D, V, dtype):
+    h, w, t, _ = make(N, D, V, dtype)
+    ref = reference(h, w, t, torch.ones(N, dtype=F64, device="cuda"), sign=-1.0)
+    within(linear_selective_log_softmax(h, w, t), ref["value"], ref["value_err"], "logp")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("N,D,V", [
+    (256, 256, 512), (1, 8, 1), (1, 1, 3), (2, 7, 5), (1, 64, 256), (17, 63, 255), (127, 65, 257),
+    (128, 128, 256), (129, 72, 300), (255, 200, 511), (256, 64, 513), (257, 320, 1000),
+    (300, 1000, 4099), (1023, 520, 2051), (64, 4096, 777), (5, 2048, 50257), (65, 129, 16032)])
+def test_logp_and_gradients(N, D, V, dtype):
+    h, w, t, up = make(N, D, V, dtype)
+    _check_logp(h, w, t, up, _logp_case(h, w, t, up), rms=V > 8)
+
+
+@pytest.mark.parametrize("chunk", [1, 256, 600, 1024, 1 << 20])
+def test_vocab_pieces(chunk):
+    h, w, t, up = make(200, 136, 2300, BF16)
+    _check_logp(h, w, t, up, _logp_case(h, w, t, up, vocab_chunk=chunk))
+
+
+def test_pieces_and_k_splits_agree_with_whole():
+    """Few rows: the hidden gradient is summed in K pieces, by vocabulary pieces too."""
+    h, w, t, up = make(33, 264, 40000, FP16)
+    _check_logp(h, w, t, up, _logp_case(h, w, t, up))
+    _check_logp(h, w, t, up, _logp_case(h, w, t, up, vocab_chunk=8192))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("N,D,V,drop,z_loss", [
+    (1, 16, 33, 0.0, 0.0), (40, 64, 300, 0.3, 1e-2), (300, 136, 1111, 0.5, 0.0),
+    (700, 77, 515, 0.9, 1e-3), (513, 256, 2048, 0.02, 0.0)])
+def test_cross_entropy(N, D, V, drop, z_loss, reduction, dtype):
+    h, w, t, up = make(N, D, V, dtype, seed=3)
+    g = torch.Generator(device="cpu").manual_seed(N)
+    dropped = (torch.rand(N, generator=g) < drop).cuda()
+    dropped[0] = False
+    live = ~dropped
+    target = torch.where(dropped, torch.full_like(t, -100), t)
+    scale = 64.0 if dtype == FP16 else 1.0
+    if reduction == "none":
+        upstream = up * scale
+        coef = up[live].to(F64) * scale
+    else:
+        upstream = torch.tensor(scale * 1.5, device="cuda")
+        coef = torch.full((int(live.sum()),), scale * 1.5, dtype=F64, device="cuda")
+        if reduction == "mean":
+            coef = coef / int(live.sum())
+    ref = reference(h[live], w, t[live], coef, z_loss=z_loss)
+    hg, wg = h.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(hg, wg, target, reduction=reduction, z_loss=z_loss)
+    gh, gw = torch.autograd.grad(loss, (hg, wg), upstream)
+    assert loss.dtype == torch.float32
+    if reduction == "none":
+        within(loss[live], ref["value"], ref["value_err"], "loss")
+        assert (loss[dropped] == 0).all()
+    else:
+        n = int(live.sum()) if reduction == "mean" else 1
+        within(loss, ref["value"].sum() / n, ref["value_err"].sum() / n + 2.0 ** -23 * ref["value"].sum().abs() / n,
+               "loss")
+    # the mean's coefficient is itself a rounded quotient
+    within(gh[live], ref["grad_hidden"], ref["grad_hidden_err"], "grad_hidden")
+    within(gw, ref["grad_weight"], ref["grad_weight_err"], "grad_weight")
+    assert (gh[dropped] == 0).all()
+
+
+def test_garbage_in_ignored_rows_stays_out():
+    h, w, t, up = make(400, 104, 700, BF16, seed=5)
+    clean = h.clone()
+    drop = torch.zeros(400, dtype=torch.bool, device="cuda")
+    drop[::3] = True
+    t = torch.where(drop, torch.full_like(t, 7777), t)
+    outs = []
+    for fill in (0.0, float("nan"), float("inf")):
+        x = clean.clone()
+        x[drop] = fill
+        x.requires_grad_()
+        wg = w.detach().requires_grad_()
+        loss = linear_cross_entropy(x, wg, t, ignore_index=7777)
+        outs.append((loss.detach(), *torch.autograd.grad(loss, (x, wg))))
+    for other in outs[1:]:
+        for a, b in zip(outs[0], other):
+            assert torch.equal(a, b)
+    assert all(torch.isfinite(a).all() for a in outs[0])
+
+
+@pytest.mark.parametrize("n", [1, 70, 600])
+def test_every_token_ignored(n):
+    h, w, t, up = make(n, 72, 300, BF16)
+    t = torch.full_like(t, -100)
+    h[:] = float("nan")
+    hg, wg = h.requires_grad_(), w.requires_grad_()
+    for reduction, want in (("mean", float("nan")), ("sum", 0.0)):
+        loss = linear_cross_entropy(hg, wg, t, reduction=reduction)
+        assert (loss.isnan() if want != want else loss == want)
+        gh, gw = torch.autograd.grad(loss, (hg, wg))
+        assert (gh == 0).all() and (gw == 0).all()
+    assert (linear_cross_entropy(hg, wg, t, reduction="none") == 0).all()
+
+
+def test_no_tokens():
+    w = torch.randn(50, 16, device="cuda", dtype=BF16, requires_grad=True)
+    h = torch.empty(2, 0, 16, device="cuda", dtype=BF16, requires_grad=True)
+    t = torch.empty(2, 0, dtype=torch.int64, device="cuda")
+    logp = linear_selective_log_softmax(h, w, t)
+    assert logp.shape == (2, 0)
+    loss = linear_cross_entropy(h, w, t, reduction="sum")
+    gh, gw = torch.autograd.grad(loss, (h, w))
+    assert loss == 0 and gh.shape == h.shape and (gw == 0).all()
+    assert linear_cross_entropy(h, w, t).isnan()
+
+
+def test_out_of_range_targets():
+    h, w, t, up = make(100, 64, 300, BF16)
+    bad = t.clone()
+    bad[5], bad[40], bad[77] = -1, 300, 1 << 40
+    rows = torch.tensor([5, 40, 77], device="cuda")
+    logp, gh, gw = _logp_case(h, w, bad, up)
+    assert logp[rows].isnan().all()
+    ok = torch.ones(100, dtype=torch.bool, device="cuda")
+    ok[rows] = False
+    ref = reference(h, w, t, up.to(F64), sign=-1.0)
+    within(logp[ok], ref["value"][ok], ref["value_err"][ok], "logp")
+    # no one-hot term in those rows: d z = -g softmax
+    hd, wd = h.to(F64), w.to(F64)
+    p = torch.softmax(hd @ wd.t(), -1)
+    within(gh[rows], (-up.to(F64)[:, None] * p)[rows] @ wd, ref["grad_hidden_err"][rows] + 1e-3, "grad_hidden")
+    assert torch.isfinite(gw).all()
+    assert linear_cross_entropy(h, w, bad).isnan()
+    for fn in (linear_selective_log_softmax, linear_cross_entropy):
+        with pytest.raises(RuntimeError, match="out of range"):
+            fn(h, w, bad, check_index=True)
+    linear_cross_entropy(h, w, torch.full_like(t, -100), check_index=True)
+
+
+@pytest.mark.parametrize("layout", ["sliced", "column_offset", "transposed", "expanded", "three_level"])
+def test_hidden_layouts(layout):
+    B, T, D, V = 3, 41, 72, 300
+    g = torch.Generator(device="cpu").manual_seed(9)
+    big = torch.randn(B, T + 1, 2 * D, generator=g).to(BF16).cuda()
+    if layout == "sliced":
+        h = big[:, :-1, :D].contiguous()
+        h = torch.cat([h, h[:, :1]], 1)[:, :-1]
+    elif layout == "column_offset":
+        h = big[:, :-1, 3:3 + D]        # rows not 16-byte aligned
+    elif layout == "transposed":
+        h = big[0].t()[:D].t()[None, :T].expand(1, T, D).transpose(0, 1)
+    elif layout == "expanded":
+        h = big[:1, :1, :D].expand(B, T, D)
+    else:
+        h = big.view(B, 1, T + 1, 2 * D).expand(B, 2, T + 1, 2 * D)[:, :, 1:, :D]
+    t = torch.randint(0, V, h.shape[:-1], generator=g).cuda()
+    w = (torch.randn(V, D, generator=g) / 4).to(BF16).cuda()
+    up = torch.randn(h.shape[:-1], generator=g).cuda()
+    hg, wg = h.detach().requires_grad_(), w.requires_grad_()
+    flat = h.reshape(-1, D).contiguous()
+    ref = reference(flat, w.detach(), t.reshape(-1), up.reshape(-1).to(F64), sign=-1.0)
+    for fn, sign in ((linear_selective_log_softmax, 1.0),
+                     (lambda *a: linear_cross_entropy(*a, reduction="none"), -1.0)):
+        out = fn(hg, wg, t)
+        assert out.shape == t.shape
+        gh, gw = torch.autograd.grad(out, (hg, wg), up * sign)
+        within(sign * out.reshape(-1), ref["value"], ref["value_err"], "value")
+        assert gh.shape == h.shape
+        within(gh.reshape(-1, D), ref["grad_hidden"], ref["grad_hidden_err"], "grad_hidden")
+        within(gw, ref["grad_weight"], ref["grad_weight_err"], "grad_weight")
+
+
+@pytest.mark.parametrize("case", ["strided_rows", "odd_offset", "transposed"])
+def test_weight_layouts(case):
+    N, D, V = 50, 80, 333
+    h, w, t, up = make(N, D, V, FP16)
+    if case == "strided_rows":
+        buf = torch.zeros(V, D + 8, device="cuda", dtype=FP16)
+        view = buf[:, :D]
+    elif case == "odd_offset":
+        buf = torch.zeros(V * D + 1, device="cuda", dtype=FP16)
+        view = buf[1:].view(V, D)
+    else:
+        buf = torch.zeros(D, V, device="cuda", dtype=FP16)
+        view = buf.t()
+    view.copy_(w)
+    _check_logp(h, w, t, up, _logp_case(h, view, t, up))
+
+
+def test_only_one_gradient_wanted():
+    h, w, t, up = make(90, 64, 500, BF16)
+    _, gh, gw = _logp_case(h, w, t, up)
+    hg = h.detach().requires_grad_()
+    (g1,) = torch.autograd.grad(linear_selective_log_softmax(hg, w, t), (hg,), up)
+    wg = w.detach().requires_grad_()
+    (g2,) = torch.autograd.grad(linear_selective_log_softmax(h, wg, t), (wg,), up)
+    assert torch.equal(g1, gh) and torch.equal(g2, gw)
+    assert not linear_selective_log_softmax(h, w, t).requires_grad
+
+
+def test_equal_calls_give_equal_bits_and_backward_twice():
+    h, w, t, _ = make(300, 520, 5000, BF16)
+    hg, wg = h.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(hg, wg, t)
+    first = torch.autograd.grad(loss, (hg, wg), retain_graph=True)
+    second = torch.autograd.grad(loss, (hg, wg))
+    again = linear_cross_entropy(hg, wg, t)
+    assert torch.equal(loss, again)
+    assert torch.equal(first[0], second[0]) and torch.equal(first[1], second[1])
+
+
+def test_gradient_against_differences():
+    """Central differences of the 64-bit loss along random directions."""
+    h, w, t, _ = make(20, 32, 90, BF16)
+    hg, wg = h.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(hg, wg, t, z_loss=1e-2)
+    gh, gw = torch.autograd.grad(loss, (hg, wg))
+
+    def f(hd, wd):
+        z = hd @ wd.t()
+        lse = torch.logsumexp(z, -1)
+        return (lse - z[torch.arange(20, device="cuda"), t] + 1e-2 * lse ** 2).mean()
+
+    hd, wd = h.detach().to(F64), w.detach().to(F64)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for _ in range(4):
+        dh = torch.randn(20, 32, generator=g, device="cuda", dtype=F64)
+        dw = torch.randn(90, 32, generator=g, device="cuda", dtype=F64)
+        e = 1e-5
+        want = (f(hd + e * dh, wd + e * dw) - f(hd - e * dh, wd - e * dw)) / (2 * e)
+        got = (gh.to(F64) * dh).sum() + (gw.to(F64) * dw).sum()
+        # each gradient element: two roundings of 2^-8 at most, independent along the direction
+        bound = 4 * 2.0 ** -8 * ((gh.to(F64) * dh).norm() + (gw.to(F64) * dw).norm())
+        assert (got - want).abs() <= bound + 1e-8
+
+
+def test_extreme_logits():
+    """Logits of +-1e4 and rows that one entry owns: finite losses, no overflow."""
+    N, D, V = 64, 64, 1000
+    h, w, t, up = make(N, D, V, BF16, spread=2.0)
+    h = (h * 1000).contiguous()
+    ref = reference(h, w, t, up.to(F64), sign=-1.0)
+    logp, gh, gw = _logp_case(h, w, t, up)
+    within(logp, ref["value"], ref["value_err"], "logp")
+    assert torch.isfinite(gh).all() and torch.isfinite(gw).all()
+
+
+def test_nan_and_inf_rows_stay_in_their_rows():
+    h, w, t, up = make(300, 64, 700, BF16)
+    clean = linear_selective_log_softmax(h, w, t)
+    h2 = h.clone()
+    h2[3, 5] = float("nan")
+    h2[200] = float("inf")
+    out = linear_selective_log_softmax(h2, w, t)
+    keep = torch.ones(300, dtype=torch.bool, device="cuda")
+    keep[3] = keep[200] = False
+    assert out[3].isnan() and out[200].isnan()
+    assert torch.equal(out[keep], clean[keep])
+
+
+def test_int32_targets_and_shapes():
+    h, w, t, _ = make(12, 64, 300, BF16)
+    a = linear_selective_log_softmax(h.view(3, 4, 64), w, t.view(3, 4).int())
+    b = linear_selective_log_softmax(h, w, t)
+    assert a.shape == (3, 4) and torch.equal(a.reshape(-1), b)
+    one = linear_selective_log_softmax(h[0], w, t[0])
+    assert one.shape == () and one == linear_selective_log_softmax(h[:1], w, t[:1])[0]
+
+
+def test_other_stream():
+    h, w, t, up = make(300, 256, 3000, BF16)
+    want = _logp_case(h, w, t, up)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = _logp_case(h, w, t, up)
+    torch.cuda.current_stream().wait_stream(s)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    cases = [make(500, 256, 4000, BF16, seed=s) for s in range(2)]
+    want = [_logp_case(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for s, c in zip(streams, cases):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(_logp_case(*c))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_captured_step_replays_on_new_data():
+    h, w, t, _ = make(300, 128, 1500, BF16, seed=1)
+    h2, w2, t2, _ = make(300, 128, 1500, BF16, seed=2)
+    t2[::4] = -100
+    hg, wg, tg = h.clone().requires_grad_(), w.clone().requires_grad_(), t.clone()
+
+    def step():
+        loss = linear_cross_entropy(hg, wg, tg)
+        return (loss.detach(), *torch.autograd.grad(loss, (hg, wg)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for hh, ww, tt in ((h, w, t), (h2, w2, t2)):
+        with torch.no_grad():
+            hg.copy_(hh), wg.copy_(ww), tg.copy_(tt)
+        graph.replay()
+        got = [o.clone() for o in out]
+        want = step()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    torch.cuda.synchronize()
+
+
+def test_matches_selective_on_logits():
+    """The same values as selective_log_softmax gives on kept fp32 logits."""
+    h, w, t, _ = make(64, 128, 1000, BF16)
+    z = h.float() @ w.float().t()
+    want = fuselse_b200.selective_log_softmax(z, t)
+    lse = torch.logsumexp(z, -1).abs().clamp_min(1.0)
+    got = linear_selective_log_softmax(h, w, t)
+    zerr = 128 * 2.0 ** -23 * (h.float().abs() @ w.float().abs().t()).amax(-1)
+    assert ((got - want).abs() <= 2e-5 * lse + 2 * zerr).all()
