@@ -13,6 +13,9 @@ libfuselse_b200.so (include/fuselse_b200.h).  `fuselse_b200.distributed`
 shards rows across GPUs and combines vocab-sharded rows over NCCL or the
 library's own NVLink exchange.  `selective_log_softmax(logits, index)` is the
 fused per-token log-probability (target gather + LSE in one pass).
+`linear_cross_entropy` and `linear_selective_log_softmax` take hidden states and
+the output projection and keep no logits; `topk_distillation_loss` trains a
+student on a teacher's top logits.
 `fuselse_b200.pc` has the pyjuice `SumLayer._forward_sparse` hook and a
 differentiable sparse sum layer (its backward on the device too), and
 `fuselse_b200.host` runs the forward and backward on rows held in pinned host
@@ -20,8 +23,9 @@ memory with the copies overlapped.
 """
 from . import ext
 from .autograd import make_fuselse_logsumexp
+from .distill import topk_distillation_loss
 from .linear import linear_cross_entropy, linear_selective_log_softmax
 from .selective import selective_log_softmax
 
 __all__ = ["ext", "make_fuselse_logsumexp", "selective_log_softmax", "linear_cross_entropy",
-           "linear_selective_log_softmax"]
+           "linear_selective_log_softmax", "topk_distillation_loss"]

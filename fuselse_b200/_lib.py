@@ -81,6 +81,12 @@ SIGNATURES = {
                            POINTER(c_uint16), POINTER(c_uint16), c_void_p, c_int64, _stream],
     "fl_copy_rows16": [POINTER(c_uint16), POINTER(c_uint16), c_int64, c_int64, c_int64, c_int64,
                        c_int64, c_int64, _stream],
+    "fl_topk_distill_fwd": [c_void_p, c_int, c_void_p, c_int, POINTER(c_int64), c_int64, c_int64,
+                            c_int64, c_int64, c_int64, c_int64, c_float, c_int, _fp, _fp, _fp, _fp,
+                            _fp, POINTER(c_int), _stream],
+    "fl_topk_distill_bwd": [_fp, c_void_p, c_int, c_void_p, c_int, POINTER(c_int64), c_int64, c_int64,
+                            c_int64, c_int64, c_int64, c_int64, c_float, c_int, _fp, _fp, _fp,
+                            c_void_p, _stream],
     "fl_binary_version": [c_int, POINTER(c_int)],
 }
 

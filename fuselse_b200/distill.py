@@ -1,0 +1,63 @@
+"""Distillation from a teacher's top logits.
+
+A teacher that is too large to run beside its student is stored as its top K
+logits of each token.  `topk_distillation_loss(logits, teacher_logits,
+teacher_index)` is T^2 KL(p || q) with p the softmax of the kept teacher logits
+/ T and q = softmax(logits / T) over the whole vocabulary: one pass over the
+student's logits forward (their log-sum-exp and the K gathers together), one
+fused pass backward, T (q - p).  No reference counterpart.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import ext
+
+_REDUCTIONS = {"none": 1, "sum": 2, "mean": 3}
+
+
+class TopkDistillation(torch.autograd.Function):
+    """Student logits whose rows are read in place -> loss."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, teacher_index, temperature, reduce, err_flag):
+        out, (lse, tlse, count) = ext.topk_distill_forward(logits, teacher_logits, teacher_index,
+                                                           temperature, reduce, err_flag)
+        ctx.save_for_backward(logits, teacher_logits, teacher_index, lse, tlse, count)
+        ctx.config = temperature, reduce
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        temperature, reduce = ctx.config
+        grad = ext.topk_distill_backward(grad_output, *ctx.saved_tensors, temperature=temperature,
+                                         reduce=reduce)
+        return grad, None, None, None, None, None
+
+
+def topk_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
+                           *, temperature: float = 1.0, reduction: str = "mean",
+                           check_index: bool = False) -> torch.Tensor:
+    """T^2 KL(teacher || student), fp32, from the teacher's top logits.
+
+    logits (..., V) are the student's (CUDA fp32, fp16 or bf16; sliced rows are
+    read in place), teacher_logits (..., K) the teacher's kept logits (any of
+    the three types; no gradient) at columns teacher_index (..., K), K <= 1024.
+    An index of -1 or a logit of -inf is padding; a row without any entry gives
+    0, takes no part in the mean and gets a zero gradient, whatever its logits
+    hold.  reduction "mean" (over the other rows; NaN without any), "sum" or
+    "none" (logits.shape[:-1]).  Any other index outside [0, V) makes its row
+    NaN; with `check_index=True` it raises RuntimeError instead (one device sync)."""
+    if reduction not in _REDUCTIONS:
+        raise RuntimeError(f"topk_distillation_loss: unknown reduction {reduction!r}")
+    temperature = float(temperature)
+    ext.check_topk_distill("topk_distillation_loss", logits, teacher_logits, teacher_index, temperature)
+    if ext.row_layout(logits) is None:
+        logits = logits.contiguous()
+    err = torch.zeros(1, dtype=torch.int32, device=logits.device) if check_index else None
+    out = TopkDistillation.apply(logits, teacher_logits.detach(), teacher_index, temperature,
+                                 _REDUCTIONS[reduction], err)
+    if check_index and int(err.item()):
+        raise RuntimeError(f"topk_distillation_loss: index out of range for {logits.shape[-1]} classes")
+    return out

@@ -325,6 +325,84 @@ def linear_loss_backward(grad_output: torch.Tensor, hidden: torch.Tensor, weight
 
 
 # --------------------------------------------------------------------------
+# Distillation from a teacher's top logits (no reference kernel)
+# --------------------------------------------------------------------------
+_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+MAX_TOP = 1024
+
+
+def check_topk_distill(what: str, logits: torch.Tensor, teacher_logits: torch.Tensor,
+                       teacher_index: torch.Tensor, temperature: float) -> None:
+    """The argument checks of topk_distillation_loss."""
+    for t, name in ((logits, "logits"), (teacher_logits, "teacher_logits"),
+                    (teacher_index, "teacher_index")):
+        _check(isinstance(t, torch.Tensor), f"{what}: {name} must be a tensor")
+    _check(logits.dtype in _DTYPE and teacher_logits.dtype in _DTYPE,
+           f"{what}: logits must be fp32, fp16 or bf16 (got {logits.dtype} and {teacher_logits.dtype})")
+    _check(teacher_index.dtype in (torch.int64, torch.int32), f"{what}: teacher_index must be int64 or int32")
+    _check(logits.dim() >= 1 and logits.shape[-1] >= 1, f"{what}: logits (..., V) expected")
+    _check(teacher_logits.shape == teacher_index.shape,
+           f"{what}: teacher_logits and teacher_index must have one shape")
+    _check(teacher_logits.shape[:-1] == logits.shape[:-1] and teacher_logits.dim() == logits.dim(),
+           f"{what}: teacher entries of shape {tuple(logits.shape[:-1])} + (K,) expected, "
+           f"got {tuple(teacher_logits.shape)}")
+    _check(1 <= teacher_logits.shape[-1] <= MAX_TOP, f"{what}: 1 to {MAX_TOP} teacher entries per row")
+    # 1 / T and T^2 are formed in fp32
+    _check(2.0 ** -60 <= temperature <= 2.0 ** 60, f"{what}: temperature must be positive and finite")
+    _check(logits.is_cuda and teacher_logits.is_cuda and teacher_index.is_cuda,
+           f"{what}: the tensors must be CUDA")
+    _check(teacher_logits.device == logits.device and teacher_index.device == logits.device,
+           f"{what}: the tensors must be on one device")
+
+
+def topk_distill_forward(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
+                         temperature: float = 1.0, reduce: int = 1, err_flag=None):
+    """(out, state): reduce 1 per-row losses (logits.shape[:-1]), 2 their sum, 3 their
+    mean over the rows that keep a teacher entry.  logits rows are read in place
+    (row_layout must address them); state is (lse, teacher_lse, count) for
+    topk_distill_backward."""
+    check_topk_distill("topk_distill_forward", logits, teacher_logits, teacher_index, temperature)
+    lay = row_layout(logits)
+    _check(lay is not None, "logits rows cannot be addressed in place (more than two leading stride levels)")
+    N, V, rpg, gs, rs = lay
+    K, dev = teacher_logits.shape[-1], logits.device
+    tl, ti = teacher_logits.contiguous(), teacher_index.to(torch.int64).contiguous()
+    with torch.cuda.device(dev):
+        # the results share no storage with what the backward keeps: a caller may change them in place
+        lse, tlse = torch.empty((2, N), dtype=torch.float32, device=dev).unbind(0)
+        values = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+        out = torch.empty((), dtype=torch.float32, device=dev) if reduce >= 2 else None
+        count = torch.empty((), dtype=torch.float32, device=dev) if reduce == 3 else None
+        if N == 0 and out is not None:
+            out.fill_(float("nan") if reduce == 3 else 0.0)
+        elif N:
+            call("fl_topk_distill_fwd", ctypes.c_void_p(logits.data_ptr()), _DTYPE[logits.dtype],
+                 ctypes.c_void_p(tl.data_ptr()), _DTYPE[tl.dtype], ptr(ti, ctypes.c_int64), N, V, K, rpg,
+                 gs, rs, temperature, reduce, ptr(lse), ptr(tlse), ptr(values), ptr(out),
+                 ptr(count), ptr(err_flag, ctypes.c_int), _stream(logits))
+    return values if out is None else out, (lse, tlse, count)
+
+
+def topk_distill_backward(grad_output: torch.Tensor, logits: torch.Tensor, teacher_logits: torch.Tensor,
+                          teacher_index: torch.Tensor, lse: torch.Tensor, teacher_lse: torch.Tensor, count,
+                          temperature: float = 1.0, reduce: int = 1) -> torch.Tensor:
+    """Dense gradient of logits, of their shape and dtype."""
+    N, V, rpg, gs, rs = row_layout(logits)
+    K, dev = teacher_logits.shape[-1], logits.device
+    tl, ti = teacher_logits.contiguous(), teacher_index.to(torch.int64).contiguous()
+    with torch.cuda.device(dev):
+        g = grad_output.to(torch.float32).reshape(-1).contiguous()
+        _check(g.numel() == (N if reduce == 1 else 1), "grad_output does not match the forward's output")
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        if N:
+            call("fl_topk_distill_bwd", ptr(g), ctypes.c_void_p(logits.data_ptr()), _DTYPE[logits.dtype],
+                 ctypes.c_void_p(tl.data_ptr()), _DTYPE[tl.dtype], ptr(ti, ctypes.c_int64), N, V, K, rpg,
+                 gs, rs, temperature, reduce, ptr(lse), ptr(teacher_lse), ptr(count),
+                 ctypes.c_void_p(grad.data_ptr()), _stream(logits))
+    return grad
+
+
+# --------------------------------------------------------------------------
 # In-place layouts: strided rows and dim != -1 (no contiguous copy)
 # --------------------------------------------------------------------------
 def row_layout(x: torch.Tensor):

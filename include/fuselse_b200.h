@@ -400,6 +400,34 @@ int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int64_t ldh,
                        int64_t vocab_chunk, uint16_t* grad_hidden, uint16_t* grad_weight,
                        void* workspace, int64_t workspace_bytes, fl_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Distillation from a teacher's top logits: x (N, V) student logits (rows
+ * strided as fl_lse_f32_fwd_strided; rows_per_group < 0: dense), K <= 1024
+ * teacher logits per row at columns teacher_index (int64), both dense (N, K).
+ * dtype and teacher_dtype 0: fp32, 1: fp16, 2: bf16; fp32 arithmetic.
+ *   p = softmax(teacher / T) over the entries whose index is not -1 and whose
+ *       logit is not -inf,  q = softmax(x / T)
+ *   values[row] = T^2 sum_j p_j (log p_j - log q_j);  0 where nothing is kept
+ *   reduce 1: values is the result; 2, 3: out[0] = their sum, their mean over
+ *   the rows that keep an entry (0 / 0 if none), *count (3) the number of those.
+ * An index outside [0, V) other than -1 makes its row NaN and, when err_flag
+ * is not NULL, sets *err_flag |= 1.  lse and teacher_lse (N,) are kept for
+ * the backward:  gx = grad * T * (q - p), grad one float for reduce 2 and 3
+ * (divided by *count for 3), (N,) for 1; gx (N, V) dense, of x's
+ * dtype; zero in rows that keep nothing.  Columns named twice count twice.
+ * No reference counterpart.
+ * ---------------------------------------------------------------------- */
+int fl_topk_distill_fwd(const void* x, int dtype, const void* teacher_logits, int teacher_dtype,
+                        const int64_t* teacher_index, int64_t N, int64_t V, int64_t K,
+                        int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
+                        float temperature, int reduce, float* lse, float* teacher_lse, float* values,
+                        float* out, float* count, int* err_flag, fl_stream_t stream);
+int fl_topk_distill_bwd(const float* grad, const void* x, int dtype, const void* teacher_logits,
+                        int teacher_dtype, const int64_t* teacher_index, int64_t N, int64_t V,
+                        int64_t K, int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
+                        float temperature, int reduce, const float* lse, const float* teacher_lse,
+                        const float* count, void* gx, fl_stream_t stream);
+
 /* Rows of D 16-bit elements (strided as fl_lse_f32_fwd_strided, rows_per_group
  * < 0: dense) to dense rows of Dp: zero-filled if Dp > D, cut if Dp < D. */
 int fl_copy_rows16(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t D, int64_t Dp,

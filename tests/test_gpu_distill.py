@@ -1,0 +1,303 @@
+"""topk_distillation_loss against the definition in 64 bits.
+
+Bounds, with u32 = 2^-24 and u the rounding of the logits' type.  lse(z / T) is
+held to 1e-5 max(|lse|, 1) as in the other LSE tests, and so is the teacher's;
+a row's loss T^2 sum p (gap) is off by T^2 times the two, the roundings of the
+scaled logits (2^-23 of their size) and 2^-21 of each term.  A gradient element
+c (q - p) is off by c (q e_lse + p e_teacher) with e the errors of the exponents,
+plus the exponentials' 2^-22, plus one rounding u (fp16: or half its smallest
+spacing, 2^-25).
+"""
+import math
+
+import pytest
+import torch
+
+from fuselse_b200 import topk_distillation_loss
+
+pytestmark = pytest.mark.gpu
+F64 = torch.float64
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def make(N, V, K, dtype, seed=0, pad=0.3, tdtype=None):
+    g = torch.Generator(device="cpu").manual_seed(seed + N + 3 * V + 7 * K)
+    z = (2 * torch.randn(N, V, generator=g)).to(dtype)
+    index = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(N)])
+    t = (2 * torch.randn(N, K, generator=g)).to(tdtype or dtype)
+    drop = torch.rand(N, K, generator=g) < pad
+    drop[:, 0] = False
+    index = torch.where(drop, torch.full_like(index, -1), index)
+    if N > 2:
+        index[1] = -1          # a row without entries
+        t[2, -1] = -math.inf   # an entry of no probability
+    return z.cuda(), t.cuda(), index.cuda()
+
+
+def reference(z, t, index, T, coef, dtype):
+    N, V = z.shape
+    u = torch.finfo(dtype).eps / 2
+    zd, td = z.to(F64) / T, t.to(F64) / T
+    keep = (index != -1) & (td != -math.inf)
+    live = keep.any(-1)
+    td = td.masked_fill(~keep, -math.inf)
+    tl = torch.logsumexp(td, -1)
+    tl = torch.where(live, tl, torch.zeros_like(tl))
+    lse = torch.logsumexp(zd, -1)
+    p = torch.where(keep, torch.exp(td - tl[:, None]), torch.zeros_like(td))
+    slot = index.clamp(min=0)
+    zt = zd.gather(-1, slot)
+    gap = torch.where(keep, td - tl[:, None] - zt + lse[:, None], torch.zeros_like(td))
+    value = T * T * (p * gap).sum(-1) * live
+    e_lse = 1e-5 * lse.abs().clamp_min(1) + 2.0 ** -23 * zd.abs().amax(-1)
+    e_tl = 1e-5 * tl.abs().clamp_min(1) + 2.0 ** -23 * torch.where(keep, td, torch.zeros_like(td)).abs().amax(-1)
+    size = torch.where(keep, td.abs() + zt.abs(), torch.zeros_like(td)) + tl.abs()[:, None] + lse.abs()[:, None]
+    terms = p * (2.0 ** -21 * (gap.abs() + size) + gap.abs() * (e_tl[:, None] + 2.0 ** -21))
+    verr = T * T * (terms.sum(-1) + e_lse + e_tl) * live
+    c = (coef * T * live)[:, None]
+    q = torch.exp(zd - lse[:, None])
+    dense = torch.zeros_like(zd).scatter_add_(-1, slot, torch.where(keep, p, torch.zeros_like(p)))
+    grad = c * (q - dense)
+    ez = torch.expm1(e_lse[:, None] + 2.0 ** -23 * zd.abs()) + 2.0 ** -21
+    ep = torch.expm1(e_tl[:, None] + 2.0 ** -22) + 2.0 ** -21
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-37
+    gerr = c.abs() * (q * ez + dense * ep) + (u + 2.0 ** -22) * grad.abs() + tiny
+    grad[~live] = 0
+    return value, verr, grad, gerr, live
+
+
+def close(got, want, bound, what):
+    err = (got.to(F64) - want).abs()
+    ok = err <= bound
+    assert bool(ok.all()), f"{what}: {int((~ok).sum())} off, worst {err.max().item():.3g}"
+
+
+def run(z, t, index, T, reduction, upstream):
+    z = z.detach().requires_grad_()
+    loss = topk_distillation_loss(z, t, index, temperature=T, reduction=reduction)
+    (g,) = torch.autograd.grad(loss, (z,), upstream)
+    return loss.detach(), g
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,K", [
+    (1, 1, 1), (2, 3, 2), (5, 7, 7), (3, 8, 4), (17, 255, 33), (9, 257, 100), (4, 1024, 1024),
+    (300, 1000, 20), (700, 515, 5), (3, 4099, 64), (2, 50257, 300), (4, 128256, 50), (64, 16032, 32)])
+@pytest.mark.parametrize("T,reduction", [(1.0, "none"), (2.5, "mean"), (0.7, "sum")])
+def test_loss_and_gradient(N, V, K, dtype, T, reduction):
+    z, t, index = make(N, V, K, dtype)
+    g = torch.Generator(device="cpu").manual_seed(5)
+    if reduction == "none":
+        up = torch.randn(N, generator=g).cuda()
+        coef = up.to(F64)
+    else:
+        up = torch.tensor(3.0, device="cuda")
+        coef = torch.full((N,), 3.0, dtype=F64, device="cuda")
+    value, verr, grad, gerr, live = reference(z, t, index, T, coef, dtype)
+    if reduction == "mean":
+        n = int(live.sum())
+        grad, gerr = grad / n, gerr / n + (2.0 ** -25 if dtype == torch.float16 else 0)
+    loss, got = run(z, t, index, T, reduction, up)
+    assert loss.dtype == torch.float32 and got.dtype == dtype and got.shape == z.shape
+    if reduction == "none":
+        close(loss, value, verr, "loss")
+    else:
+        n = int(live.sum()) if reduction == "mean" else 1
+        close(loss, value.sum() / n, verr.sum() / n + 2.0 ** -23 * value.sum().abs() / n, "loss")
+    close(got, grad, gerr, "gradient")
+    if N > 2:
+        assert (got[1] == 0).all()
+
+
+@pytest.mark.parametrize("tdtype", TYPES)
+def test_teacher_of_another_type(tdtype):
+    z, t, index = make(20, 700, 16, torch.bfloat16, tdtype=tdtype)
+    coef = torch.ones(20, dtype=F64, device="cuda")
+    value, verr, grad, gerr, _ = reference(z, t, index, 1.5, coef, torch.bfloat16)
+    loss, got = run(z, t, index.int(), 1.5, "none", torch.ones(20, device="cuda"))
+    close(loss, value, verr, "loss")
+    close(got, grad, gerr, "gradient")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_columns_named_twice(dtype):
+    z, t, index = make(40, 300, 24, dtype, pad=0.0)
+    index[:, 8:16] = index[:, :8]
+    index[:, 16:24] = index[:, :8]
+    index[3] = 7                     # one column for all entries
+    t[4, 8] = t[4, 0]                # equal probabilities too
+    coef = torch.ones(40, dtype=F64, device="cuda")
+    value, verr, grad, gerr, _ = reference(z, t, index, 1.0, coef, dtype)
+    a = run(z, t, index, 1.0, "none", torch.ones(40, device="cuda"))
+    close(a[0], value, verr, "loss")
+    close(a[1], grad, gerr, "gradient")
+    b = run(z, t, index, 1.0, "none", torch.ones(40, device="cuda"))
+    assert torch.equal(a[1], b[1])
+
+
+def test_rows_that_keep_nothing():
+    z, t, index = make(6, 500, 8, torch.float32, pad=0.0)
+    z[1] = float("nan")
+    z[3, 7] = float("inf")
+    index[3] = -1
+    t[4] = -math.inf
+    loss, g = run(z, t, index, 1.0, "none", torch.ones(6, device="cuda"))
+    for r in (1, 3, 4):
+        assert loss[r] == 0 and (g[r] == 0).all()
+    mean, gm = run(z, t, index, 1.0, "mean", torch.tensor(1.0, device="cuda"))
+    assert torch.allclose(mean, loss[[0, 2, 5]].double().mean().float(), rtol=2.0 ** -22, atol=0)
+    index[:] = -1
+    empty, ge = run(z, t, index, 1.0, "mean", torch.tensor(1.0, device="cuda"))
+    assert empty.isnan() and (ge == 0).all()
+    total, _ = run(z, t, index, 1.0, "sum", torch.tensor(1.0, device="cuda"))
+    assert total == 0
+
+
+def test_special_student_values():
+    z, t, index = make(5, 400, 4, torch.float32, pad=0.0)
+    index[1] = index[0]
+    t[2] = t[0]
+    z[0, 11] = -math.inf                       # masked entry away from the teacher's
+    index[0] = torch.tensor([1, 2, 3, 4], device="cuda")
+    z[1, index[1, 0]] = -math.inf              # masked where the teacher has mass
+    z[3, 9] = float("nan")
+    z[4] = -math.inf
+    loss, g = run(z, t, index, 1.0, "none", torch.ones(5, device="cuda"))
+    assert torch.isfinite(loss[0]) and g[0, 11] == 0 and torch.isfinite(g[0]).all()
+    assert loss[1] == math.inf and torch.isfinite(g[1]).all()
+    assert loss[3].isnan() and loss[4].isnan()
+    t2 = t.clone()
+    t2[2, 1] = -math.inf
+    z2 = z.clone()
+    z2[2, index[2, 1]] = -math.inf             # 0 log 0: neither side has mass
+    assert torch.isfinite(topk_distillation_loss(z2, t2, index, reduction="none")[2])
+
+
+def test_index_out_of_range():
+    z, t, index = make(10, 100, 4, torch.bfloat16, pad=0.0)
+    clean, _ = run(z, t, index, 1.0, "none", torch.ones(10, device="cuda"))
+    for bad in (100, -2, 1 << 40):
+        i2 = index.clone()
+        i2[5, 2] = bad
+        loss, g = run(z, t, i2, 1.0, "none", torch.ones(10, device="cuda"))
+        assert loss[5].isnan() and torch.isfinite(g).all()
+        keep = torch.arange(10, device="cuda") != 5
+        assert torch.equal(loss[keep], clean[keep])
+        with pytest.raises(RuntimeError, match="out of range"):
+            topk_distillation_loss(z, t, i2, check_index=True)
+    topk_distillation_loss(z, t, index, check_index=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["sliced", "column_offset", "expanded", "columns"])
+def test_layouts(layout, dtype):
+    g = torch.Generator(device="cpu").manual_seed(2)
+    base = (2 * torch.randn(3, 12, 1001, generator=g)).to(dtype).cuda()
+    z = {"sliced": base[:, :-1], "column_offset": base[:, :-1, 3:], "expanded": base[:1, :1].expand(3, 11, 1001),
+         "columns": base[:, :-1].transpose(0, 2).contiguous().transpose(0, 2)}[layout]
+    index = torch.randint(0, z.shape[-1], (3, 11, 9), generator=g).cuda()
+    t = torch.randn(3, 11, 9, generator=g).cuda()
+    flat = z.reshape(33, -1)
+    coef = torch.ones(33, dtype=F64, device="cuda")
+    value, verr, grad, gerr, _ = reference(flat, t.view(33, 9), index.view(33, 9), 1.0, coef, dtype)
+    loss, got = run(z, t, index, 1.0, "none", torch.ones(3, 11, device="cuda"))
+    assert loss.shape == (3, 11)
+    close(loss.view(33), value, verr, "loss")
+    close(got.reshape(33, -1), grad, gerr, "gradient")
+
+
+def test_result_may_change_in_place_before_the_backward():
+    z, t, index = make(6, 300, 5, torch.float32, pad=0.0)
+    z.requires_grad_()
+    for reduction in ("none", "mean", "sum"):
+        (want,) = torch.autograd.grad(2 * topk_distillation_loss(z, t, index, reduction=reduction).sum(), (z,))
+        loss = topk_distillation_loss(z, t, index, reduction=reduction)
+        loss.mul_(2)
+        (got,) = torch.autograd.grad(loss.sum(), (z,))
+        assert torch.equal(got, want)
+
+
+def test_gradient_against_differences():
+    z, t, index = make(6, 40, 5, torch.float32)
+    z = z.requires_grad_()
+    loss = topk_distillation_loss(z, t, index, temperature=1.7, reduction="sum")
+    (grad,) = torch.autograd.grad(loss, (z,))
+
+    def f(zd):
+        coef = torch.ones(6, dtype=F64, device="cuda")
+        return reference(zd, t, index, 1.7, coef, torch.float32)[0].sum()
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for _ in range(4):
+        d = torch.randn(6, 40, generator=g, device="cuda", dtype=F64)
+        e = 1e-5
+        want = (f(z.detach().to(F64) + e * d) - f(z.detach().to(F64) - e * d)) / (2 * e)
+        assert ((grad.to(F64) * d).sum() - want).abs() <= 1e-4 * (grad.to(F64) * d).abs().sum()
+
+
+def test_no_rows():
+    z = torch.empty(2, 0, 30, device="cuda", requires_grad=True)
+    t, i = torch.empty(2, 0, 4, device="cuda"), torch.empty(2, 0, 4, device="cuda", dtype=torch.int64)
+    assert topk_distillation_loss(z, t, i).isnan()
+    loss = topk_distillation_loss(z, t, i, reduction="sum")
+    (g,) = torch.autograd.grad(loss, (z,))
+    assert loss == 0 and g.shape == z.shape
+    assert topk_distillation_loss(z, t, i, reduction="none").shape == (2, 0)
+
+
+def test_streams_and_graphs():
+    a, b = make(50, 3000, 30, torch.bfloat16, seed=1), make(50, 3000, 30, torch.bfloat16, seed=9)
+    z, t, index = (x.clone() for x in a)
+    z.requires_grad_()
+    one = torch.ones((), device="cuda")
+
+    def step():
+        loss = topk_distillation_loss(z, t, index, temperature=2.0)
+        (g,) = torch.autograd.grad(loss, (z,), one)
+        return loss.detach(), g
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = step()
+    torch.cuda.current_stream().wait_stream(side)
+    want = step()
+    assert all(torch.equal(x, y) for x, y in zip(first, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for case in (a, b):
+        with torch.no_grad():
+            z.copy_(case[0]), t.copy_(case[1]), index.copy_(case[2])
+        graph.replay()
+        got = [o.clone() for o in out]
+        assert all(torch.equal(x, y) for x, y in zip(got, step()))
+    torch.cuda.synchronize()
+
+
+def test_together_with_the_vocabulary_losses():
+    """A distillation step: labels through the projection without logits, the teacher
+    on the logits of some tokens, both gradients into one weight."""
+    from fuselse_b200 import linear_cross_entropy
+    g = torch.Generator(device="cpu").manual_seed(4)
+    h = torch.randn(96, 64, generator=g).to(torch.bfloat16).cuda().requires_grad_()
+    w = (torch.randn(500, 64, generator=g) / 4).to(torch.bfloat16).cuda().requires_grad_()
+    target = torch.randint(0, 500, (96,), generator=g).cuda()
+    target[::5] = -100
+    t, index = torch.randn(32, 8, generator=g).cuda(), torch.randint(0, 500, (32, 8), generator=g).cuda()
+    loss = linear_cross_entropy(h, w, target) + 0.5 * topk_distillation_loss(
+        h[:32] @ w.t(), t, index, temperature=2.0)
+    loss.backward()
+    hd, wd = h.detach().to(F64).requires_grad_(), w.detach().to(F64).requires_grad_()
+    z = hd @ wd.t()
+    p = torch.zeros(32, 500, dtype=F64, device="cuda").scatter_add_(-1, index, torch.softmax(t.to(F64) / 2, -1))
+    lq = torch.log_softmax(z[:32] / 2, -1)
+    kl = 4 * (torch.softmax(t.to(F64) / 2, -1) * (torch.log_softmax(t.to(F64) / 2, -1) - lq.gather(-1, index))).sum(-1).mean()
+    want = torch.nn.functional.cross_entropy(z, target) + 0.5 * kl
+    want.backward()
+    # the logits between the two are rounded to bf16: each by 2^-8 of its size at most, which
+    # moves a KL of their softmax by no more than twice the largest such step times T
+    zmax = z.detach().abs().max().item()
+    assert abs(loss.item() - want.item()) <= 0.5 * 2 * 2 * 2.0 ** -8 * zmax + 1e-4
+    for got, ref in ((h.grad, hd.grad), (w.grad, wd.grad)):
+        assert (got.to(F64) - ref).norm() <= 0.05 * ref.norm()
