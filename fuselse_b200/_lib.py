@@ -66,26 +66,22 @@ SIGNATURES = {
     "fl_ipc_buffer_open": [c_int, c_void_p, POINTER(c_void_p)],
     "fl_ipc_buffer_close": [c_int, c_void_p],
     "fl_ipc_buffer_free": [c_int, c_void_p],
-    "fl_linear_loss_workspace": [c_int64, c_int64, c_int64, c_int64, c_int, POINTER(c_int64),
-                                 POINTER(c_int64)],
-    "fl_linear_loss_pack": [POINTER(c_uint16), POINTER(c_int64), c_int64, POINTER(c_uint16),
-                            POINTER(c_int), POINTER(c_int), POINTER(c_int), c_int64, c_int64, c_int64,
-                            c_int64, c_int64, _stream],
-    "fl_linear_loss_fwd": [POINTER(c_uint16), c_int64, POINTER(c_uint16), c_int64, c_int,
-                           POINTER(c_int64), POINTER(c_int), POINTER(c_int), POINTER(c_int), c_int64,
-                           c_int64, c_int64, c_int, c_float, _fp, _fp, c_void_p, c_int64,
-                           POINTER(c_int), _stream],
-    "fl_linear_loss_bwd": [_fp, POINTER(c_uint16), c_int64, POINTER(c_uint16), c_int64, c_int,
-                           POINTER(c_int64), POINTER(c_int), POINTER(c_int), POINTER(c_int), _fp,
-                           c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_int64,
-                           POINTER(c_uint16), POINTER(c_uint16), c_void_p, c_int64, _stream],
-    "fl_copy_rows16": [POINTER(c_uint16), POINTER(c_uint16), c_int64, c_int64, c_int64, c_int64,
-                       c_int64, c_int64, _stream],
-    "fl_topk_distill_fwd": [c_void_p, c_int, c_void_p, c_int, POINTER(c_int64), c_int64, c_int64,
-                            c_int64, c_int64, c_int64, c_int64, c_float, c_int, _fp, _fp, _fp, _fp,
-                            _fp, POINTER(c_int), _stream],
-    "fl_topk_distill_bwd": [_fp, c_void_p, c_int, c_void_p, c_int, POINTER(c_int64), c_int64, c_int64,
-                            c_int64, c_int64, c_int64, c_int64, c_float, c_int, _fp, _fp, _fp,
+    # addresses as plain integers: these entry points are called once or twice per training step
+    # of small batches, where forming typed pointers would be a good part of the call
+    "fl_linear_loss_sizes": [c_int64, c_int64, c_int64, c_int, c_int64, c_int, POINTER(c_int64),
+                             POINTER(c_int64), POINTER(c_int64)],
+    "fl_linear_loss_fwd": [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int,
+                           c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_void_p, c_int64, c_void_p,
+                           c_void_p, c_int64, c_void_p, _stream],
+    "fl_linear_loss_bwd": [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int,
+                           c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_float, c_int64, c_void_p,
+                           c_int64, c_void_p, c_void_p, c_void_p, c_int64, _stream],
+    "fl_copy_rows16": [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _stream],
+    "fl_topk_distill_fwd": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                            c_int64, c_int64, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                            c_void_p, c_void_p, _stream],
+    "fl_topk_distill_bwd": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64,
+                            c_int64, c_int64, c_int64, c_float, c_int, c_void_p, c_void_p, c_void_p,
                             c_void_p, _stream],
     "fl_binary_version": [c_int, POINTER(c_int)],
 }

@@ -668,27 +668,85 @@ int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
 
 constexpr CUtensorMapDataType kMap16[2] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16};
 
-int check_projection(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype, int64_t N,
-                     int64_t V, int64_t Dp, const char* what) {
-    FL_REQUIRE(dtype == 0 || dtype == 1, "%s: dtype must be 0 (fp16) or 1 (bf16)", what);
-    FL_REQUIRE(N >= 0 && V >= 1 && Dp >= 1, "%s: bad shape (%lld, %lld, %lld)", what, (long long)N,
-               (long long)V, (long long)Dp);
-    FL_REQUIRE(N <= kMaxExtent && V <= kMaxExtent && Dp <= (1 << 20), "%s: shape too large", what);
-    FL_REQUIRE(Dp % 8 == 0 && ldh % 8 == 0 && ldw % 8 == 0 && ldh >= Dp && ldw >= Dp,
-               "%s: rows must be a multiple of 8 elements apart and long", what);
-    FL_REQUIRE(ldh < (1ll << 38) && ldw < (1ll << 38), "%s: row stride too large", what);
-    FL_REQUIRE(N == 0 || (hidden && weight), "%s: NULL buffer", what);
-    FL_REQUIRE(aligned_to(hidden, 16) && aligned_to(weight, 16), "%s: operands must be 16-byte aligned", what);
-    // a unit index of the largest product (256 x 256 tiles times K pieces) fits 32 bits
-    FL_REQUIRE(((N + 255) / 256) * ((V + 255) / 256) <= INT32_MAX / 64 &&
-                   ((V + 255) / 256) * ((Dp + 255) / 256) <= INT32_MAX / 64 &&
-                   ((N + 255) / 256) * ((Dp + 255) / 256) <= INT32_MAX / 64,
-               "%s: shape too large", what);
-    return FL_OK;
-}
-
 int64_t fwd_bytes(int64_t N, int64_t V) {
     return round_up(N * 2 * ((V + kTile - 1) / kTile) * 8, 256) + 2 * round_up(N * 4, 256);
+}
+
+// What a forward leaves for its backward: meta, the rows' lse, the packing's
+// two maps (kPackKept) and the packed rows (kPackAll, kPackKept).
+enum Pack { kPackNone = 0, kPackAll = 1, kPackKept = 2 };
+
+struct State {
+    int* meta;
+    float* lse;
+    int *src, *pos;
+    uint16_t* packed;
+    int64_t bytes;
+};
+
+State lay_state(void* base, int64_t N, int64_t Dp, int pack) {
+    State s = {};
+    char* p = static_cast<char*>(base);
+    int64_t at = 256;
+    auto take = [&](int64_t bytes) {
+        char* q = p + at;
+        at += round_up(bytes, 256);
+        return q;
+    };
+    s.meta = reinterpret_cast<int*>(p);
+    s.lse = reinterpret_cast<float*>(take(N * 4));
+    if (pack == kPackKept) {
+        s.src = reinterpret_cast<int*>(take(N * 4));
+        s.pos = reinterpret_cast<int*>(take(N * 4));
+    }
+    if (pack != kPackNone) s.packed = reinterpret_cast<uint16_t*>(take(N * Dp * 2));
+    s.bytes = at;
+    return s;
+}
+
+struct Call {
+    const uint16_t* hidden;
+    RowMap rows;
+    int64_t ldh;  // kPackNone: the rows' distance
+    int64_t Dp;
+};
+
+// The checks that both directions share; forms the row layout.
+int check_call(Call* c, const uint16_t* hidden, int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
+               const uint16_t* weight, int64_t ldw, int dtype, const int64_t* target, int pack, int64_t N,
+               int64_t V, int64_t D, int reduce, const void* state, int64_t state_bytes, const char* what) {
+    FL_REQUIRE(N >= 0 && V >= 1 && D >= 1, "%s: bad shape (%lld, %lld, %lld)", what, (long long)N, (long long)V,
+               (long long)D);
+    FL_REQUIRE(dtype == 0 || dtype == 1, "%s: dtype must be 0 (fp16) or 1 (bf16)", what);
+    FL_REQUIRE(N <= kMaxExtent && V <= kMaxExtent && D <= (1 << 20), "%s: shape too large", what);
+    c->Dp = round_up(D, 8);
+    // a unit index of the largest product (256 x 256 tiles times K pieces) fits 32 bits
+    const int64_t tn = (N + kTile - 1) / kTile, tv = (V + kTile - 1) / kTile, td = (D + kTile - 1) / kTile;
+    FL_REQUIRE(std::max({tn * tv, tv * td, tn * td}) <= INT32_MAX / 64, "%s: shape too large", what);
+    FL_REQUIRE(pack >= kPackNone && pack <= kPackKept, "%s: unknown packing %d", what, pack);
+    FL_REQUIRE(reduce >= kLogp && reduce <= kMean, "%s: unknown reduction %d", what, reduce);
+    FL_REQUIRE(reduce < kSum || pack == kPackKept, "%s: a reduced loss needs packing 2", what);
+    c->rows = RowMap::dense(D);
+    c->ldh = D;
+    if (rows_per_group >= 0) {
+        FL_REQUIRE(rows_per_group >= 1 && group_stride >= 0 && row_stride >= 0, "%s: bad row layout", what);
+        c->rows = RowMap{rows_per_group, group_stride, row_stride};
+        c->ldh = row_stride;
+    }
+    FL_REQUIRE(ldw >= c->Dp && ldw % 8 == 0 && ldw < (1ll << 38) && aligned_to(weight, 16),
+               "%s: weight rows must be 16-byte aligned, a multiple of 8 elements apart", what);
+    FL_REQUIRE(pack != kPackNone || N == 0 ||
+                   (D % 8 == 0 && c->ldh % 8 == 0 && c->ldh >= D && c->ldh < (1ll << 38) &&
+                    (rows_per_group < 0 || rows_per_group >= N) && aligned_to(hidden, 16)),
+               "%s: unpacked hidden rows must be 16-byte aligned, a multiple of 8 elements long and apart", what);
+    FL_REQUIRE(N == 0 || (weight && target && state), "%s: NULL buffer", what);
+    FL_REQUIRE(aligned_to(hidden, 2) && aligned_to(target, 8) && aligned_to(state, 256), "%s: misaligned buffer",
+               what);
+    FL_REQUIRE(N == 0 || state_bytes >= lay_state(nullptr, N, c->Dp, pack).bytes,
+               "%s: state of %lld bytes, %lld needed", what, (long long)state_bytes,
+               (long long)lay_state(nullptr, N, c->Dp, pack).bytes);
+    c->hidden = hidden;
+    return FL_OK;
 }
 
 }  // namespace
@@ -696,43 +754,20 @@ int64_t fwd_bytes(int64_t N, int64_t V) {
 
 using namespace fl;
 
-extern "C" int fl_linear_loss_workspace(int64_t N, int64_t V, int64_t D, int64_t vocab_chunk,
-                                        int want_hidden, int64_t* forward, int64_t* backward) {
+extern "C" int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int pack, int64_t vocab_chunk,
+                                    int want_hidden, int64_t* state, int64_t* forward, int64_t* backward) {
     clear_error();
-    const char* what = "fl_linear_loss_workspace";
-    if (int st = check_projection(nullptr, round_up(D, 8), nullptr, round_up(D, 8), 0, 0, V, round_up(D, 8),
-                                  what))
+    const char* what = "fl_linear_loss_sizes";
+    Call c;
+    if (int st = check_call(&c, nullptr, -1, 0, 0, nullptr, round_up(std::max<int64_t>(D, 1), 8), 0, nullptr, pack,
+                            0, V, D, kLogp, nullptr, 0, what))
         return st;
-    FL_REQUIRE(N >= 0 && N <= kMaxExtent && forward && backward, "%s: bad arguments", what);
-    FL_REQUIRE(vocab_chunk >= 0, "%s: vocab_chunk is negative", what);
+    FL_REQUIRE(N >= 0 && N <= kMaxExtent && vocab_chunk >= 0 && state && forward && backward,
+               "%s: bad arguments", what);
+    *state = lay_state(nullptr, N, c.Dp, pack).bytes;
     *forward = fwd_bytes(N, V);
-    *backward = plan_bwd(N, V, round_up(D, 8), vocab_chunk, want_hidden != 0, sm_count() / 2).bytes;
+    *backward = plan_bwd(N, V, c.Dp, vocab_chunk, want_hidden != 0, sm_count() / 2).bytes;
     return FL_OK;
-}
-
-extern "C" int fl_linear_loss_pack(const uint16_t* hidden, const int64_t* target, int64_t ignore_index,
-                                   uint16_t* packed, int* src, int* pos, int* meta, int64_t N, int64_t D,
-                                   int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
-                                   fl_stream_t stream) {
-    clear_error();
-    const char* what = "fl_linear_loss_pack";
-    FL_REQUIRE(N >= 0 && D >= 1 && N <= kMaxExtent && D <= (1 << 20), "%s: bad shape", what);
-    if (N == 0) return FL_OK;
-    FL_REQUIRE(hidden && target && packed && src && pos && meta, "%s: NULL buffer", what);
-    FL_REQUIRE(aligned_to(hidden, 2) && aligned_to(target, 8) && aligned_to(packed, 16) &&
-                   aligned_to(src, 4) && aligned_to(pos, 4) && aligned_to(meta, 4),
-               "%s: misaligned buffer", what);
-    RowMap rm = RowMap::dense(D);
-    if (rows_per_group >= 0) {
-        FL_REQUIRE(rows_per_group >= 1 && group_stride >= 0 && row_stride >= 0, "%s: bad row layout", what);
-        rm = RowMap{rows_per_group, group_stride, row_stride};
-    }
-    if (int st = bind_device(stream, packed)) return st;
-    const int64_t grid = std::min<int64_t>(N, 2 * sm_count());
-    LaunchCfg lc(dim3((unsigned)grid), dim3(kPackThreads), 0, reinterpret_cast<cudaStream_t>(stream), false);
-    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, pack_rows_kernel, hidden, target, ignore_index, packed, src, pos, meta,
-                               (int)N, (int)D, (int)round_up(D, 8), rm));
-    return check_launch(what);
 }
 
 extern "C" int fl_copy_rows16(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t D, int64_t Dp,
@@ -756,46 +791,63 @@ extern "C" int fl_copy_rows16(const uint16_t* src, uint16_t* dst, int64_t rows, 
     return check_launch(what);
 }
 
-extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t ldh, const uint16_t* weight, int64_t ldw,
-                                  int dtype, const int64_t* target, const int* src, const int* pos, int* meta,
-                                  int64_t N, int64_t V, int64_t D, int reduce, float z_loss, float* lse,
+extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group, int64_t group_stride,
+                                  int64_t row_stride, const uint16_t* weight, int64_t ldw, int dtype,
+                                  const int64_t* target, int pack, int64_t ignore_index, int64_t N, int64_t V,
+                                  int64_t D, int reduce, float z_loss, void* state, int64_t state_bytes,
                                   float* out, void* workspace, int64_t workspace_bytes, int* err_flag,
                                   fl_stream_t stream) {
     clear_error();
     const char* what = "fl_linear_loss_fwd";
-    if (int st = check_projection(hidden, ldh, weight, ldw, dtype, N, V, D, what)) return st;
-    FL_REQUIRE(reduce >= kLogp && reduce <= kMean, "%s: unknown reduction %d", what, reduce);
-    FL_REQUIRE((src == nullptr) == (pos == nullptr), "%s: src and pos come together", what);
-    FL_REQUIRE(src || reduce < kSum, "%s: a reduced loss needs packed rows", what);
+    Call c;
+    if (int st = check_call(&c, hidden, rows_per_group, group_stride, row_stride, weight, ldw, dtype, target, pack,
+                            N, V, D, reduce, state, state_bytes, what))
+        return st;
     if (N == 0) return FL_OK;
-    FL_REQUIRE(target && meta && lse && out && workspace, "%s: NULL buffer", what);
-    FL_REQUIRE(aligned_to(target, 8) && aligned_to(lse, 4) && aligned_to(out, 4) && aligned_to(err_flag, 4) &&
-                   aligned_to(workspace, 256),
+    FL_REQUIRE(hidden && out && workspace, "%s: NULL buffer", what);
+    FL_REQUIRE(aligned_to(out, 4) && aligned_to(err_flag, 4) && aligned_to(workspace, 256),
                "%s: misaligned buffer", what);
     FL_REQUIRE(workspace_bytes >= fwd_bytes(N, V), "%s: workspace of %lld bytes, %lld needed", what,
                (long long)workspace_bytes, (long long)fwd_bytes(N, V));
-    if (int st = bind_device(stream, lse)) return st;
+    if (int st = bind_device(stream, state)) return st;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const State keep = lay_state(state, N, c.Dp, pack);
+    const uint16_t* h = hidden;
+    int64_t ldh = c.ldh;
+    if (pack == kPackKept) {
+        LaunchCfg lc(dim3((unsigned)std::min<int64_t>(N, 2 * sm_count())), dim3(kPackThreads), 0, s, false);
+        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, pack_rows_kernel, hidden, target, ignore_index, keep.packed, keep.src,
+                                   keep.pos, keep.meta, (int)N, (int)D, (int)c.Dp, c.rows));
+        if (int st = check_launch(what)) return st;
+    } else {
+        FL_CUDA(cudaMemsetAsync(keep.meta, 0, 16, s));
+        if (pack == kPackAll) {
+            LaunchCfg lc(dim3((unsigned)((N + 7) / 8)), dim3(256), 0, s, false);
+            FL_CUDA(cudaLaunchKernelEx(&lc.cfg, copy_rows16_kernel, hidden, keep.packed, N, (int)D, (int)c.Dp,
+                                       c.rows));
+            if (int st = check_launch(what)) return st;
+        }
+    }
+    if (pack != kPackNone) h = keep.packed, ldh = c.Dp;
     const int64_t tiles_n = (V + kTile - 1) / kTile;
     float2* part = static_cast<float2*>(workspace);
     float* zt = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(N * 2 * tiles_n * 8, 256));
     float* values = reduce < kSum ? out
                                   : reinterpret_cast<float*>(reinterpret_cast<char*>(zt) + round_up(N * 4, 256));
-    if (!src) FL_CUDA(cudaMemsetAsync(meta, 0, 16, s));
     CUtensorMap a, b;
-    if (int st = make_tensor_map(&a, kMap16[dtype], 2, hidden, D, N, ldh, kBlockK, kHalfTile)) return st;
-    if (int st = make_tensor_map(&b, kMap16[dtype], 2, weight, D, V, ldw, kBlockK, kHalfTile)) return st;
+    if (int st = make_tensor_map(&a, kMap16[dtype], 2, h, c.Dp, N, ldh, kBlockK, kHalfTile)) return st;
+    if (int st = make_tensor_map(&b, kMap16[dtype], 2, weight, c.Dp, V, ldw, kBlockK, kHalfTile)) return st;
     GemmArgs g = {};
     g.rows = (int)N;
-    g.packed = src != nullptr;
+    g.packed = pack == kPackKept;
     g.m_extent = -1;
     g.n_extent = (int)V;
-    g.k_extent = (int)D;
+    g.k_extent = (int)c.Dp;
     g.splits = 1;
     g.idesc = umma_idesc(dtype == 1, false, false);
-    g.meta = meta;
+    g.meta = keep.meta;
     g.target = target;
-    g.src = src;
+    g.src = keep.src;
     g.part = part;
     g.pieces = (int)(2 * tiles_n);
     g.zt = zt;
@@ -804,42 +856,45 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t ldh, const uin
     const int64_t grid = std::min<int64_t>((N + 7) / 8, 8ll * sm_count());
     LaunchCfg lc(dim3((unsigned)grid), dim3(256), 0, s, false);
     FL_CUDA(cudaLaunchKernelEx(&lc.cfg, finish_forward_kernel, (const float2*)part, g.pieces, (const float*)zt,
-                               target, pos, meta, N, V, z_loss, reduce, lse, values, out, err_flag));
+                               target, (const int*)keep.pos, keep.meta, N, V, z_loss, reduce, keep.lse, values, out,
+                               err_flag));
     return check_launch(what);
 }
 
-extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int64_t ldh,
-                                  const uint16_t* weight, int64_t ldw, int dtype, const int64_t* target,
-                                  const int* src, const int* pos, int* meta, const float* lse, int64_t N,
-                                  int64_t V, int64_t D, int64_t hidden_cols, int reduce, float z_loss,
-                                  int64_t vocab_chunk, uint16_t* grad_hidden, uint16_t* grad_weight,
+extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int64_t rows_per_group,
+                                  int64_t group_stride, int64_t row_stride, const uint16_t* weight, int64_t ldw,
+                                  int dtype, const int64_t* target, int pack, int64_t N, int64_t V, int64_t D,
+                                  int reduce, float z_loss, int64_t vocab_chunk, void* state,
+                                  int64_t state_bytes, uint16_t* grad_hidden, uint16_t* grad_weight,
                                   void* workspace, int64_t workspace_bytes, fl_stream_t stream) {
     clear_error();
     const char* what = "fl_linear_loss_bwd";
-    if (int st = check_projection(hidden, ldh, weight, ldw, dtype, N, V, D, what)) return st;
-    FL_REQUIRE(reduce >= kLogp && reduce <= kMean, "%s: unknown reduction %d", what, reduce);
-    FL_REQUIRE((src == nullptr) == (pos == nullptr) && (src || reduce < kSum), "%s: bad packing", what);
+    Call c;
+    if (int st = check_call(&c, hidden, rows_per_group, group_stride, row_stride, weight, ldw, dtype, target, pack,
+                            N, V, D, reduce, state, state_bytes, what))
+        return st;
     FL_REQUIRE(vocab_chunk >= 0, "%s: vocab_chunk is negative", what);
-    FL_REQUIRE(hidden_cols >= 1 && hidden_cols <= D, "%s: bad hidden_cols", what);
     if (!grad_hidden && !grad_weight) return FL_OK;
-    FL_REQUIRE(grad_weight == nullptr || aligned_to(grad_weight, 16), "%s: misaligned buffer", what);
+    FL_REQUIRE(aligned_to(grad_weight, 16) && aligned_to(grad_hidden, 8), "%s: misaligned buffer", what);
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const int64_t Dp = c.Dp;
     if (N == 0) {
         if (!grad_weight) return FL_OK;
         if (int st = bind_device(stream, grad_weight)) return st;
-        FL_CUDA(cudaMemsetAsync(grad_weight, 0, (size_t)(V * D * 2), reinterpret_cast<cudaStream_t>(stream)));
+        FL_CUDA(cudaMemsetAsync(grad_weight, 0, (size_t)(V * Dp * 2), s));
         return FL_OK;
     }
-    FL_REQUIRE(grad && target && meta && lse && workspace, "%s: NULL buffer", what);
-    FL_REQUIRE(aligned_to(grad, 4) && aligned_to(target, 8) && aligned_to(lse, 4) &&
-                   aligned_to(grad_hidden, 8) && aligned_to(workspace, 256),
-               "%s: misaligned buffer", what);
+    FL_REQUIRE(grad && workspace && (hidden || pack != kPackNone), "%s: NULL buffer", what);
+    FL_REQUIRE(aligned_to(grad, 4) && aligned_to(workspace, 256), "%s: misaligned buffer", what);
     if (int st = bind_device(stream, workspace)) return st;
-    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int pairs = sm_count() / 2;
-    const BwdPlan plan = plan_bwd(N, V, D, vocab_chunk, grad_hidden != nullptr, pairs);
+    const BwdPlan plan = plan_bwd(N, V, Dp, vocab_chunk, grad_hidden != nullptr, pairs);
     FL_REQUIRE(workspace_bytes >= plan.bytes, "%s: workspace of %lld bytes, %lld needed", what,
                (long long)workspace_bytes, (long long)plan.bytes);
     FL_REQUIRE(plan.slab_rows * std::max(plan.splits, 1) <= kMaxExtent, "%s: shape too large", what);
+    const State keep = lay_state(state, N, Dp, pack);
+    const uint16_t* h = pack == kPackNone ? hidden : keep.packed;
+    const int64_t ldh = pack == kPackNone ? c.ldh : Dp;
     char* ws = static_cast<char*>(workspace);
     float* inv_scale = reinterpret_cast<float*>(ws);
     float* ca = reinterpret_cast<float*>(ws + plan.coef_off);
@@ -849,64 +904,64 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     const bool bf16 = dtype == 1;
     {
         LaunchCfg lc(dim3(1), dim3(1024), 0, s, false);
-        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, coefficients_kernel, grad, reduce, z_loss, lse, src,
-                                   (const int*)meta, N, ca, cb, inv_scale));
+        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, coefficients_kernel, grad, reduce, z_loss, (const float*)keep.lse,
+                                   (const int*)keep.src, (const int*)keep.meta, N, ca, cb, inv_scale));
         if (int st = check_launch(what)) return st;
     }
     // operand and output views: hidden and weight by rows and by columns, dz both ways
     CUtensorMap h_k, w_k, dz_out, dz_mn, h_mn, dw_out, dz_k, w_mn, slab_out;
-    if (int st = make_tensor_map(&h_k, kMap16[dtype], 2, hidden, D, N, ldh, kBlockK, kHalfTile)) return st;
-    if (int st = make_tensor_map(&w_k, kMap16[dtype], 2, weight, D, V, ldw, kBlockK, kHalfTile)) return st;
-    if (int st = make_tensor_map(&dz_out, kMap16[dtype], 2, dz, plan.chunk, N, plan.chunk, 64, 32)) return st;
+    const CUtensorMapDataType t16 = kMap16[dtype];
+    if (int st = make_tensor_map(&h_k, t16, 2, h, Dp, N, ldh, kBlockK, kHalfTile)) return st;
+    if (int st = make_tensor_map(&w_k, t16, 2, weight, Dp, V, ldw, kBlockK, kHalfTile)) return st;
+    if (int st = make_tensor_map(&dz_out, t16, 2, dz, plan.chunk, N, plan.chunk, 64, 32)) return st;
     if (grad_weight) {
-        if (int st = make_tensor_map(&dz_mn, kMap16[dtype], 2, dz, plan.chunk, N, plan.chunk, 64, kBlockK)) return st;
-        if (int st = make_tensor_map(&h_mn, kMap16[dtype], 2, hidden, D, N, ldh, 64, kBlockK)) return st;
-        if (int st = make_tensor_map(&dw_out, kMap16[dtype], 2, grad_weight, D, V, D, 64, 32)) return st;
+        if (int st = make_tensor_map(&dz_mn, t16, 2, dz, plan.chunk, N, plan.chunk, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&h_mn, t16, 2, h, Dp, N, ldh, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&dw_out, t16, 2, grad_weight, Dp, V, Dp, 64, 32)) return st;
     }
     if (grad_hidden) {
-        if (int st = make_tensor_map(&dz_k, kMap16[dtype], 2, dz, plan.chunk, N, plan.chunk, kBlockK, kHalfTile))
-            return st;
-        if (int st = make_tensor_map(&w_mn, kMap16[dtype], 2, weight, D, V, ldw, 64, kBlockK)) return st;
-        if (int st = make_tensor_map(&slab_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, slabs, D,
-                                     plan.slab_rows * plan.splits, D, 32, 32))
+        if (int st = make_tensor_map(&dz_k, t16, 2, dz, plan.chunk, N, plan.chunk, kBlockK, kHalfTile)) return st;
+        if (int st = make_tensor_map(&w_mn, t16, 2, weight, Dp, V, ldw, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&slab_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, slabs, Dp,
+                                     plan.slab_rows * plan.splits, Dp, 32, 32))
             return st;
     }
     GemmArgs base = {};
     base.rows = (int)N;
-    base.packed = src != nullptr;
+    base.packed = pack == kPackKept;
     base.splits = 1;
-    base.meta = meta;
-    const int64_t mt = (N + kTile - 1) / kTile, dt = (D + kTile - 1) / kTile;
+    base.meta = keep.meta;
+    const int64_t mt = (N + kTile - 1) / kTile, dt = (Dp + kTile - 1) / kTile;
     for (int64_t v0 = 0; v0 < V; v0 += plan.chunk) {
         const int64_t cv = std::min(plan.chunk, V - v0), ct = (cv + kTile - 1) / kTile;
         GemmArgs g = base;
         g.m_extent = -1;
         g.n_extent = (int)cv;
-        g.k_extent = (int)D;
+        g.k_extent = (int)Dp;
         g.b_offset = (int)v0;
         g.idesc = umma_idesc(bf16, false, false);
         g.target = target;
-        g.src = src;
-        g.lse = lse;
+        g.src = keep.src;
+        g.lse = keep.lse;
         g.a = ca;
         g.b = cb;
         if (int st = launch_product<kEpiGradZ>(h_k, w_k, dz_out, g, mt * ct, bf16, s, what)) return st;
         if (grad_weight) {
             g = base;
             g.m_extent = (int)cv;
-            g.n_extent = (int)D;
+            g.n_extent = (int)Dp;
             g.k_extent = -1;
             g.out_row = (int)v0;
             g.idesc = umma_idesc(bf16, true, true);
             g.inv_scale = inv_scale;
             g.out = grad_weight;
-            g.out_elems = V * D;
+            g.out_elems = V * Dp;
             if (int st = launch_product<kEpiOut16>(dz_mn, h_mn, dw_out, g, ct * dt, bf16, s, what)) return st;
         }
         if (grad_hidden) {
             g = base;
             g.m_extent = -1;
-            g.n_extent = (int)D;
+            g.n_extent = (int)Dp;
             g.k_extent = (int)cv;
             g.b_offset = (int)v0;
             g.splits = plan.splits;
@@ -919,11 +974,11 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     }
     if (grad_hidden) {
         auto kern = bf16 ? finish_hidden_kernel<true> : finish_hidden_kernel<false>;
-        const int64_t gy = std::min<int64_t>(8, (hidden_cols + 1023) / 1024);
+        const int64_t gy = std::min<int64_t>(8, (D + 1023) / 1024);
         LaunchCfg lc(dim3((unsigned)N, (unsigned)gy), dim3(256), 0, s, false);
-        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, (const float*)slabs, plan.splits, plan.slab_rows * D, pos,
-                                   (const int*)meta, (const float*)inv_scale, (int)hidden_cols, (int)D,
-                                   grad_hidden));
+        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, (const float*)slabs, plan.splits, plan.slab_rows * Dp,
+                                   (const int*)keep.pos, (const int*)keep.meta, (const float*)inv_scale, (int)D,
+                                   (int)Dp, grad_hidden));
         return check_launch(what);
     }
     return FL_OK;

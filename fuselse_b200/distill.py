@@ -21,19 +21,17 @@ class TopkDistillation(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_index, temperature, reduce, err_flag):
-        out, (lse, tlse, count) = ext.topk_distill_forward(logits, teacher_logits, teacher_index,
-                                                           temperature, reduce, err_flag)
-        ctx.save_for_backward(logits, teacher_logits, teacher_index, lse, tlse, count)
+        out, saved = ext.topk_distill_forward(logits, teacher_logits, teacher_index, temperature, reduce,
+                                              err_flag)
+        ctx.save_for_backward(*saved)
         ctx.config = temperature, reduce
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        temperature, reduce = ctx.config
-        grad = ext.topk_distill_backward(grad_output, *ctx.saved_tensors, temperature=temperature,
-                                         reduce=reduce)
-        return grad, None, None, None, None, None
+        return (ext.topk_distill_backward(grad_output, *ctx.saved_tensors, *ctx.config),
+                None, None, None, None, None)
 
 
 def topk_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
@@ -56,8 +54,11 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, t
     if ext.row_layout(logits) is None:
         logits = logits.contiguous()
     err = torch.zeros(1, dtype=torch.int32, device=logits.device) if check_index else None
-    out = TopkDistillation.apply(logits, teacher_logits.detach(), teacher_index, temperature,
-                                 _REDUCTIONS[reduction], err)
+    reduce = _REDUCTIONS[reduction]
+    if torch.is_grad_enabled() and logits.requires_grad:
+        out = TopkDistillation.apply(logits, teacher_logits.detach(), teacher_index, temperature, reduce, err)
+    else:
+        out, _ = ext.topk_distill_forward(logits, teacher_logits, teacher_index, temperature, reduce, err)
     if check_index and int(err.item()):
         raise RuntimeError(f"topk_distillation_loss: index out of range for {logits.shape[-1]} classes")
     return out

@@ -23,7 +23,9 @@ row_layout / *_strided (rows read in place) and logsumexp_dim* (dim != -1).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -178,148 +180,156 @@ def selective_logsoftmax_backward(grad_output: torch.Tensor, x: torch.Tensor, ls
 # Losses from hidden states and the output projection (no reference kernel)
 # --------------------------------------------------------------------------
 _DTYPE16 = {torch.float16: 0, torch.bfloat16: 1}
-_LOSS_LOGP = 0
+_INDEX = (torch.int64, torch.int32)
+
+
+def _on_device(dev: torch.device):
+    """The guard of a call on `dev`: workspace sizes and outputs follow the current device."""
+    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _addr(t):
+    """A tensor's address as an integer argument (None for no tensor)."""
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
 def check_linear_loss(what: str, hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor) -> None:
     """The argument checks of linear_cross_entropy and linear_selective_log_softmax."""
     for t, name in ((hidden, "hidden"), (weight, "weight"), (target, "target")):
-        _check(isinstance(t, torch.Tensor), f"{what}: {name} must be a tensor")
-    _check(hidden.dtype in _DTYPE16 and weight.dtype == hidden.dtype,
-           f"{what}: hidden and weight must both be fp16 or both bf16 "
-           f"(got {hidden.dtype} and {weight.dtype})")
-    _check(target.dtype in (torch.int64, torch.int32), f"{what}: the targets must be int64 or int32")
-    _check(hidden.dim() >= 1 and weight.dim() == 2, f"{what}: hidden (..., D) and weight (V, D) expected")
-    _check(hidden.shape[-1] == weight.shape[1],
-           f"{what}: hidden has {hidden.shape[-1]} columns, weight {weight.shape[1]}")
-    _check(weight.shape[0] >= 1 and weight.shape[1] >= 1, f"{what}: weight is empty")
-    _check(target.shape == hidden.shape[:-1],
-           f"{what}: targets of shape {tuple(hidden.shape[:-1])} expected, got {tuple(target.shape)}")
-    _check(hidden.is_cuda and weight.is_cuda and target.is_cuda, f"{what}: the tensors must be CUDA")
-    _check(weight.device == hidden.device and target.device == hidden.device,
-           f"{what}: the tensors must be on one device")
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"{what}: {name} must be a tensor")
+    hs, ws = hidden.shape, weight.shape
+    if hidden.dtype not in _DTYPE16 or weight.dtype != hidden.dtype:
+        raise RuntimeError(f"{what}: hidden and weight must both be fp16 or both bf16 "
+                           f"(got {hidden.dtype} and {weight.dtype})")
+    if target.dtype not in _INDEX:
+        raise RuntimeError(f"{what}: the targets must be int64 or int32")
+    if len(hs) < 1 or len(ws) != 2:
+        raise RuntimeError(f"{what}: hidden (..., D) and weight (V, D) expected")
+    if hs[-1] != ws[1]:
+        raise RuntimeError(f"{what}: hidden has {hs[-1]} columns, weight {ws[1]}")
+    if ws[0] < 1 or ws[1] < 1:
+        raise RuntimeError(f"{what}: weight is empty")
+    if target.shape != hs[:-1]:
+        raise RuntimeError(f"{what}: targets of shape {tuple(hs[:-1])} expected, got {tuple(target.shape)}")
+    if not (hidden.is_cuda and weight.is_cuda and target.is_cuda):
+        raise RuntimeError(f"{what}: the tensors must be CUDA")
+    if weight.device != hidden.device or target.device != hidden.device:
+        raise RuntimeError(f"{what}: the tensors must be on one device")
 
 
-def _u16(t):
-    return ptr(t, ctypes.c_uint16)
+def _weight_rows(weight: torch.Tensor):
+    """(weight, row stride), or a copy whose rows are zero-filled to 8 elements where
+    the rows of weight cannot be copied by a tensor map as they lie."""
+    V, D = weight.shape
+    ld, unit = weight.stride()
+    if V == 1:
+        ld = D
+    if D % 8 == 0 and unit == 1 and ld % 8 == 0 and ld >= D and weight.data_ptr() % 16 == 0:
+        return weight, ld
+    if unit != 1 and D > 1:
+        weight = weight.contiguous()
+        ld = D
+    out = torch.empty((V, (D + 7) // 8 * 8), dtype=weight.dtype, device=weight.device)
+    call("fl_copy_rows16", weight.data_ptr(), out.data_ptr(), V, D, out.shape[1], V, 0, ld,
+         _raw_stream(weight.device))
+    return out, out.shape[1]
 
 
-def _tma_rows(t: torch.Tensor) -> bool:
-    """Whether (R, D) rows can be copied by a tensor map as they lie."""
-    return (t.shape[1] % 8 == 0 and t.stride(1) == 1 and t.data_ptr() % 16 == 0
-            and (t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])))
+PACK_NONE, PACK_ALL, PACK_KEPT = 0, 1, 2
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+@functools.lru_cache(maxsize=256)
+def linear_loss_sizes(N: int, V: int, D: int, pack: int = PACK_KEPT, vocab_chunk: int = 0,
+                      want_hidden: bool = True) -> tuple[int, int, int]:
+    """Bytes of the state that linear_loss_forward keeps and of the scratch that it and
+    linear_loss_backward allocate."""
+    out = [ctypes.c_int64() for _ in range(3)]
+    call("fl_linear_loss_sizes", N, V, D, pack, vocab_chunk, int(want_hidden), *map(ctypes.byref, out))
+    return tuple(v.value for v in out)
 
 
-def _padded_rows(t: torch.Tensor) -> torch.Tensor:
-    """(R, D) rows as dense rows of D rounded up to 8 elements."""
-    if t.stride(1) != 1 and t.shape[1] > 1:
-        t = t.contiguous()
-    R, D = t.shape
-    out = torch.empty((R, (D + 7) // 8 * 8), dtype=t.dtype, device=t.device)
-    if R:
-        call("fl_copy_rows16", _u16(t), _u16(out), R, D, out.shape[1], R, 0, t.stride(0), _stream(t))
-    return out
-
-
-def linear_loss_workspace_bytes(N: int, V: int, D: int, vocab_chunk: int = 0,
-                                want_hidden: bool = True) -> tuple[int, int]:
-    """Bytes of scratch that linear_loss_forward and linear_loss_backward allocate."""
-    fwd, bwd = ctypes.c_int64(), ctypes.c_int64()
-    call("fl_linear_loss_workspace", N, V, D, vocab_chunk, int(want_hidden), ctypes.byref(fwd),
-         ctypes.byref(bwd))
-    return fwd.value, bwd.value
+def _hidden_rows(hidden: torch.Tensor):
+    """(hidden, rows_per_group, group_stride, row_stride, whether the products can read
+    it as it lies); a copy where the rows have no layout that row_layout names."""
+    lay = row_layout(hidden)
+    if lay is None:
+        hidden = hidden.contiguous()
+        lay = row_layout(hidden)
+    N, D, rpg, gs, rs = lay
+    plain = (D % 8 == 0 and rs % 8 == 0 and rs >= D and (rpg < 0 or rpg >= N)
+             and hidden.data_ptr() % 16 == 0)
+    return hidden, rpg, gs, rs, plain
 
 
 def linear_loss_forward(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduce: int,
                         ignore_index: int | None = None, z_loss: float = 0.0, err_flag=None):
-    """(out, state): reduce 0 log-probabilities, 1 losses (both like target), 2 their
+    """(out, saved): reduce 0 log-probabilities, 1 losses (both like target), 2 their
     sum, 3 their mean over the kept rows.  Rows whose target is `ignore_index` are
-    left out (None: all rows are kept; needed by 2 and 3).  state is
-    (packed, padded, src, pos, meta, lse) for linear_loss_backward: packed / padded
-    are None where hidden / weight are used as they lie."""
+    left out (None: all rows are kept; needed by 2 and 3).  saved is what
+    linear_loss_backward takes: (hidden or None, weight rows, target, state, pack)."""
     check_linear_loss("linear_loss_forward", hidden, weight, target)
     V, D = weight.shape
-    N, shape = target.numel(), target.shape
-    dev = hidden.device
-    with torch.cuda.device(dev):
-        stream = _stream(hidden)
-        target = target.reshape(-1).to(torch.int64).contiguous()
-        padded = None if _tma_rows(weight) else _padded_rows(weight)
-        w = weight if padded is None else padded
-        packed = src = pos = None
-        lay = row_layout(hidden)
-        if lay is None:  # neither packing nor the products can address these rows
-            hidden = packed = hidden.reshape(N, D).contiguous()
-            lay = row_layout(hidden)
-        meta = torch.empty(4, dtype=torch.int32, device=dev)
-        lse = torch.empty(N, dtype=torch.float32, device=dev)
-        one_level = lay[3] == 0  # the rows are one stride apart
-        rows = hidden.as_strided((N, D), (lay[4], 1)) if one_level and N else None
-        if ignore_index is not None:
-            packed = torch.empty((N, w.shape[1]), dtype=hidden.dtype, device=dev)
-            src, pos = torch.empty((2, N), dtype=torch.int32, device=dev).unbind(0)
-            call("fl_linear_loss_pack", _u16(hidden), ptr(target, ctypes.c_int64), ignore_index,
-                 _u16(packed), ptr(src, ctypes.c_int), ptr(pos, ctypes.c_int), ptr(meta, ctypes.c_int),
-                 N, D, lay[2], lay[3], lay[4], stream)
-            rows = packed
-        elif N and not (rows is not None and _tma_rows(rows)):
-            packed = torch.empty((N, w.shape[1]), dtype=hidden.dtype, device=dev)
-            call("fl_copy_rows16", _u16(hidden), _u16(packed), N, D, w.shape[1], lay[2], lay[3], lay[4],
-                 stream)
-            rows = packed
+    shape, dev = target.shape, hidden.device
+    with _on_device(dev):
+        stream = _raw_stream(dev)
+        N = target.numel()
+        if target.dtype != torch.int64 or not target.is_contiguous():
+            target = target.to(torch.int64).contiguous()
+        w, ldw = _weight_rows(weight)
+        rows, rpg, gs, rs, plain = _hidden_rows(hidden)
+        pack = PACK_KEPT if ignore_index is not None else PACK_NONE if plain and rows is hidden else PACK_ALL
         out = torch.empty(shape if reduce < 2 else (), dtype=torch.float32, device=dev)
         if N == 0:
             if reduce >= 2:
                 out.fill_(float("nan") if reduce == 3 else 0.0)
-        else:
-            need, _ = linear_loss_workspace_bytes(N, V, D)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            call("fl_linear_loss_fwd", _u16(rows), _row_stride(rows), _u16(w), _row_stride(w),
-                 _DTYPE16[hidden.dtype], ptr(target, ctypes.c_int64), ptr(src, ctypes.c_int),
-                 ptr(pos, ctypes.c_int), ptr(meta, ctypes.c_int), N, V, w.shape[1], reduce, z_loss,
-                 ptr(lse), ptr(out), ctypes.c_void_p(ws.data_ptr()), need,
-                 ptr(err_flag, ctypes.c_int), stream)
-    return out, (packed, padded, src, pos, meta, lse)
+            return out, (None, w, target, None, pack)
+        need_state, need, _ = linear_loss_sizes(N, V, D, pack)
+        state = torch.empty(need_state, dtype=torch.uint8, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        call("fl_linear_loss_fwd", rows.data_ptr(), rpg, gs, rs, w.data_ptr(), ldw, _DTYPE16[hidden.dtype],
+             target.data_ptr(), pack, 0 if ignore_index is None else ignore_index, N, V, D, reduce, z_loss,
+             state.data_ptr(), need_state, out.data_ptr(), ws.data_ptr(), need, _addr(err_flag), stream)
+    return out, (hidden if pack == PACK_NONE else None, w, target, state, pack)
 
 
-def linear_loss_backward(grad_output: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor,
-                         target: torch.Tensor, src, pos, meta: torch.Tensor, lse: torch.Tensor,
-                         hidden_cols: int, reduce: int, z_loss: float = 0.0, vocab_chunk: int = 0,
+def linear_loss_backward(grad_output: torch.Tensor, hidden, weight: torch.Tensor, target: torch.Tensor, state,
+                         pack: int, hidden_cols: int, reduce: int, z_loss: float = 0.0, vocab_chunk: int = 0,
                          want_hidden: bool = True, want_weight: bool = True):
     """(grad_hidden (N, hidden_cols), grad_weight (V, hidden_cols)) of linear_loss_forward,
-    None where not wanted; hidden and weight as its state gives them (the packed or padded
-    copies where it made any)."""
-    V, Dp = weight.shape
-    N, D = target.numel(), hidden_cols
-    dev = weight.device
+    None where not wanted; hidden to pack as its `saved` gives them."""
     if not (want_hidden or want_weight):
         return None, None
-    with torch.cuda.device(dev):
-        stream = _stream(weight)
-        g = grad_output.to(torch.float32).reshape(-1).contiguous()
+    V, Dp = weight.shape[0], (hidden_cols + 7) // 8 * 8
+    N, D, dev, dtype = target.numel(), hidden_cols, weight.device, weight.dtype
+    with _on_device(dev):
+        stream = _raw_stream(dev)
+        g = grad_output
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.to(torch.float32).contiguous()
         _check(g.numel() == (1 if reduce >= 2 else N), "grad_output does not match the forward's output")
-        target = target.reshape(-1).to(torch.int64).contiguous()
-        grad_hidden = torch.empty((N, D), dtype=weight.dtype, device=dev) if want_hidden else None
-        grad_weight = torch.empty((V, Dp), dtype=weight.dtype, device=dev) if want_weight else None
+        grad_hidden = torch.empty((N, D), dtype=dtype, device=dev) if want_hidden else None
+        grad_weight = torch.empty((V, Dp), dtype=dtype, device=dev) if want_weight else None
         if N:
-            lay = row_layout(hidden)
-            rows = hidden.as_strided((N, Dp), (lay[4], 1))
-            _, need = linear_loss_workspace_bytes(N, V, Dp, vocab_chunk, want_hidden)
+            rpg, gs, rs = row_layout(hidden)[2:] if hidden is not None else (-1, 0, 0)
+            need_state, _, need = linear_loss_sizes(N, V, D, pack, vocab_chunk, want_hidden)
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            call("fl_linear_loss_bwd", ptr(g), _u16(rows), _row_stride(rows), _u16(weight),
-                 _row_stride(weight), _DTYPE16[weight.dtype], ptr(target, ctypes.c_int64),
-                 ptr(src, ctypes.c_int), ptr(pos, ctypes.c_int), ptr(meta, ctypes.c_int), ptr(lse), N, V,
-                 Dp, D, reduce, z_loss, vocab_chunk, _u16(grad_hidden), _u16(grad_weight),
-                 ctypes.c_void_p(ws.data_ptr()), need, stream)
+            call("fl_linear_loss_bwd", g.data_ptr(), _addr(hidden), rpg, gs, rs, weight.data_ptr(),
+                 weight.stride(0) if V > 1 else Dp, _DTYPE16[dtype], target.data_ptr(), pack, N, V, D, reduce,
+                 z_loss, vocab_chunk, state.data_ptr(), need_state, _addr(grad_hidden), _addr(grad_weight),
+                 ws.data_ptr(), need, stream)
         elif want_weight:
             grad_weight.zero_()
         if want_weight and Dp != D:
-            cut = torch.empty((V, D), dtype=weight.dtype, device=dev)
-            call("fl_copy_rows16", _u16(grad_weight), _u16(cut), V, Dp, D, -1, 0, 0, stream)
+            cut = torch.empty((V, D), dtype=dtype, device=dev)
+            call("fl_copy_rows16", grad_weight.data_ptr(), cut.data_ptr(), V, Dp, D, -1, 0, 0, stream)
             grad_weight = cut
     return grad_hidden, grad_weight
 
@@ -336,69 +346,85 @@ def check_topk_distill(what: str, logits: torch.Tensor, teacher_logits: torch.Te
     """The argument checks of topk_distillation_loss."""
     for t, name in ((logits, "logits"), (teacher_logits, "teacher_logits"),
                     (teacher_index, "teacher_index")):
-        _check(isinstance(t, torch.Tensor), f"{what}: {name} must be a tensor")
-    _check(logits.dtype in _DTYPE and teacher_logits.dtype in _DTYPE,
-           f"{what}: logits must be fp32, fp16 or bf16 (got {logits.dtype} and {teacher_logits.dtype})")
-    _check(teacher_index.dtype in (torch.int64, torch.int32), f"{what}: teacher_index must be int64 or int32")
-    _check(logits.dim() >= 1 and logits.shape[-1] >= 1, f"{what}: logits (..., V) expected")
-    _check(teacher_logits.shape == teacher_index.shape,
-           f"{what}: teacher_logits and teacher_index must have one shape")
-    _check(teacher_logits.shape[:-1] == logits.shape[:-1] and teacher_logits.dim() == logits.dim(),
-           f"{what}: teacher entries of shape {tuple(logits.shape[:-1])} + (K,) expected, "
-           f"got {tuple(teacher_logits.shape)}")
-    _check(1 <= teacher_logits.shape[-1] <= MAX_TOP, f"{what}: 1 to {MAX_TOP} teacher entries per row")
-    # 1 / T and T^2 are formed in fp32
-    _check(2.0 ** -60 <= temperature <= 2.0 ** 60, f"{what}: temperature must be positive and finite")
-    _check(logits.is_cuda and teacher_logits.is_cuda and teacher_index.is_cuda,
-           f"{what}: the tensors must be CUDA")
-    _check(teacher_logits.device == logits.device and teacher_index.device == logits.device,
-           f"{what}: the tensors must be on one device")
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"{what}: {name} must be a tensor")
+    zs, ts = logits.shape, teacher_logits.shape
+    if logits.dtype not in _DTYPE or teacher_logits.dtype not in _DTYPE:
+        raise RuntimeError(f"{what}: logits must be fp32, fp16 or bf16 "
+                           f"(got {logits.dtype} and {teacher_logits.dtype})")
+    if teacher_index.dtype not in _INDEX:
+        raise RuntimeError(f"{what}: teacher_index must be int64 or int32")
+    if len(zs) < 1 or zs[-1] < 1:
+        raise RuntimeError(f"{what}: logits (..., V) expected")
+    if teacher_index.shape != ts:
+        raise RuntimeError(f"{what}: teacher_logits and teacher_index must have one shape")
+    if len(ts) != len(zs) or ts[:-1] != zs[:-1]:
+        raise RuntimeError(f"{what}: teacher entries of shape {tuple(zs[:-1])} + (K,) expected, "
+                           f"got {tuple(ts)}")
+    if not 1 <= ts[-1] <= MAX_TOP:
+        raise RuntimeError(f"{what}: 1 to {MAX_TOP} teacher entries per row")
+    if not 2.0 ** -60 <= temperature <= 2.0 ** 60:  # 1 / T and T^2 are formed in fp32
+        raise RuntimeError(f"{what}: temperature must be positive and finite")
+    if not (logits.is_cuda and teacher_logits.is_cuda and teacher_index.is_cuda):
+        raise RuntimeError(f"{what}: the tensors must be CUDA")
+    if teacher_logits.device != logits.device or teacher_index.device != logits.device:
+        raise RuntimeError(f"{what}: the tensors must be on one device")
+
+
+def _teacher(teacher_logits, teacher_index):
+    if not teacher_logits.is_contiguous():
+        teacher_logits = teacher_logits.contiguous()
+    if teacher_index.dtype != torch.int64 or not teacher_index.is_contiguous():
+        teacher_index = teacher_index.to(torch.int64).contiguous()
+    return teacher_logits, teacher_index
 
 
 def topk_distill_forward(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
                          temperature: float = 1.0, reduce: int = 1, err_flag=None):
-    """(out, state): reduce 1 per-row losses (logits.shape[:-1]), 2 their sum, 3 their
+    """(out, saved): reduce 1 per-row losses (logits.shape[:-1]), 2 their sum, 3 their
     mean over the rows that keep a teacher entry.  logits rows are read in place
-    (row_layout must address them); state is (lse, teacher_lse, count) for
-    topk_distill_backward."""
+    (row_layout must address them); saved is what topk_distill_backward takes:
+    (logits, teacher_logits, teacher_index, state)."""
     check_topk_distill("topk_distill_forward", logits, teacher_logits, teacher_index, temperature)
     lay = row_layout(logits)
     _check(lay is not None, "logits rows cannot be addressed in place (more than two leading stride levels)")
     N, V, rpg, gs, rs = lay
     K, dev = teacher_logits.shape[-1], logits.device
-    tl, ti = teacher_logits.contiguous(), teacher_index.to(torch.int64).contiguous()
-    with torch.cuda.device(dev):
-        # the results share no storage with what the backward keeps: a caller may change them in place
-        lse, tlse = torch.empty((2, N), dtype=torch.float32, device=dev).unbind(0)
-        values = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-        out = torch.empty((), dtype=torch.float32, device=dev) if reduce >= 2 else None
-        count = torch.empty((), dtype=torch.float32, device=dev) if reduce == 3 else None
-        if N == 0 and out is not None:
-            out.fill_(float("nan") if reduce == 3 else 0.0)
-        elif N:
-            call("fl_topk_distill_fwd", ctypes.c_void_p(logits.data_ptr()), _DTYPE[logits.dtype],
-                 ctypes.c_void_p(tl.data_ptr()), _DTYPE[tl.dtype], ptr(ti, ctypes.c_int64), N, V, K, rpg,
-                 gs, rs, temperature, reduce, ptr(lse), ptr(tlse), ptr(values), ptr(out),
-                 ptr(count), ptr(err_flag, ctypes.c_int), _stream(logits))
-    return values if out is None else out, (lse, tlse, count)
+    with _on_device(dev):
+        tl, ti = _teacher(teacher_logits, teacher_index)
+        # the result shares no storage with what the backward keeps: a caller may change it in place
+        out = torch.empty(logits.shape[:-1] if reduce == 1 else (), dtype=torch.float32, device=dev)
+        state = torch.empty(2 * N + 1 + (0 if reduce == 1 else N), dtype=torch.float32, device=dev)
+        if N == 0:
+            if reduce >= 2:
+                out.fill_(float("nan") if reduce == 3 else 0.0)
+        else:
+            at = state.data_ptr()  # lse, teacher_lse, count, values of a reduced loss
+            values = out.data_ptr() if reduce == 1 else at + 4 * (2 * N + 1)
+            call("fl_topk_distill_fwd", logits.data_ptr(), _DTYPE[logits.dtype], tl.data_ptr(),
+                 _DTYPE[tl.dtype], ti.data_ptr(), N, V, K, rpg, gs, rs, temperature, reduce, at, at + 4 * N,
+                 values, out.data_ptr(), at + 8 * N, _addr(err_flag), _raw_stream(dev))
+    return out, (logits, tl, ti, state)
 
 
 def topk_distill_backward(grad_output: torch.Tensor, logits: torch.Tensor, teacher_logits: torch.Tensor,
-                          teacher_index: torch.Tensor, lse: torch.Tensor, teacher_lse: torch.Tensor, count,
-                          temperature: float = 1.0, reduce: int = 1) -> torch.Tensor:
+                          teacher_index: torch.Tensor, state: torch.Tensor, temperature: float = 1.0,
+                          reduce: int = 1) -> torch.Tensor:
     """Dense gradient of logits, of their shape and dtype."""
     N, V, rpg, gs, rs = row_layout(logits)
     K, dev = teacher_logits.shape[-1], logits.device
-    tl, ti = teacher_logits.contiguous(), teacher_index.to(torch.int64).contiguous()
-    with torch.cuda.device(dev):
-        g = grad_output.to(torch.float32).reshape(-1).contiguous()
+    with _on_device(dev):
+        g = grad_output
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.to(torch.float32).contiguous()
         _check(g.numel() == (N if reduce == 1 else 1), "grad_output does not match the forward's output")
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         if N:
-            call("fl_topk_distill_bwd", ptr(g), ctypes.c_void_p(logits.data_ptr()), _DTYPE[logits.dtype],
-                 ctypes.c_void_p(tl.data_ptr()), _DTYPE[tl.dtype], ptr(ti, ctypes.c_int64), N, V, K, rpg,
-                 gs, rs, temperature, reduce, ptr(lse), ptr(teacher_lse), ptr(count),
-                 ctypes.c_void_p(grad.data_ptr()), _stream(logits))
+            at = state.data_ptr()
+            call("fl_topk_distill_bwd", g.data_ptr(), logits.data_ptr(), _DTYPE[logits.dtype],
+                 teacher_logits.data_ptr(), _DTYPE[teacher_logits.dtype], teacher_index.data_ptr(), N, V, K,
+                 rpg, gs, rs, temperature, reduce, at, at + 4 * N, at + 8 * N, grad.data_ptr(),
+                 _raw_stream(dev))
     return grad
 
 

@@ -29,27 +29,22 @@ class LinearLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err_flag):
-        out, state = ext.linear_loss_forward(hidden, weight, target, reduce=reduce,
-                                             ignore_index=ignore_index, z_loss=z_loss, err_flag=err_flag)
-        packed, padded, src, pos, meta, lse = state
-        # an operand used as it lies is saved as the input it is, a copy as what it is
-        ctx.save_for_backward(hidden if packed is None else packed, weight if padded is None else padded,
-                              target, src, pos, meta, lse)
-        ctx.shapes = hidden.shape, weight.shape
-        ctx.config = reduce, z_loss, vocab_chunk
+        out, saved = ext.linear_loss_forward(hidden, weight, target, reduce, ignore_index, z_loss, err_flag)
+        # an operand that is used as it lies is saved as the input it is
+        ctx.save_for_backward(*saved[:4])
+        ctx.config = hidden.shape, reduce, z_loss, vocab_chunk, saved[4]
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        hidden, weight, target, src, pos, meta, lse = ctx.saved_tensors
-        reduce, z_loss, vocab_chunk = ctx.config
+        shape, reduce, z_loss, vocab_chunk, pack = ctx.config
+        want_hidden, want_weight = ctx.needs_input_grad[:2]
         grad_hidden, grad_weight = ext.linear_loss_backward(
-            grad_output, hidden, weight, target, src, pos, meta, lse, hidden_cols=ctx.shapes[0][-1],
-            reduce=reduce, z_loss=z_loss, vocab_chunk=vocab_chunk,
-            want_hidden=ctx.needs_input_grad[0], want_weight=ctx.needs_input_grad[1])
+            grad_output, *ctx.saved_tensors, pack, shape[-1], reduce, z_loss, vocab_chunk, want_hidden,
+            want_weight)
         if grad_hidden is not None:
-            grad_hidden = grad_hidden.view(ctx.shapes[0])
+            grad_hidden = grad_hidden.view(shape)
         return grad_hidden, grad_weight, None, None, None, None, None, None
 
 
@@ -59,9 +54,11 @@ def _apply(what, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chu
         vocab_chunk = 0
     elif isinstance(vocab_chunk, bool) or not isinstance(vocab_chunk, int) or vocab_chunk < 1:
         raise RuntimeError(f"{what}: vocab_chunk must be a positive int or None")
-    target = target.to(torch.int64)
     err = torch.zeros(1, dtype=torch.int32, device=hidden.device) if check_index else None
-    out = LinearLoss.apply(hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        out = LinearLoss.apply(hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err)
+    else:
+        out, _ = ext.linear_loss_forward(hidden, weight, target, reduce, ignore_index, z_loss, err)
     if check_index and int(err.item()):
         raise RuntimeError(f"{what}: index out of range for {weight.shape[0]} classes")
     return out

@@ -354,50 +354,48 @@ int fl_sparse_f32_bwd_workspace(int64_t num_nodes, int64_t batch, int64_t num_un
  * fp16, 1: bf16 (uint16 bit patterns, both operands alike); products and sums
  * in fp32.  No reference counterpart (the reference starts from logits).
  *
- * fl_linear_loss_pack keeps the rows whose target differs from ignore_index,
- * in order, as rows of Dp = D rounded up to 8 elements (zero-filled):
- *   src[p] = row of packed row p, pos[row] = p or -1, meta[0] = rows kept.
- *   hidden rows may be strided (rows_per_group as fl_lse_f32_fwd_strided; < 0:
- *   dense).  packed (N, Dp) 16-byte aligned, src and pos int32 (N,), meta
- *   int32 (4,) handed on to the calls below.  N, D >= 1 up to 2^31 - 1024, 2^20.
- * fl_linear_loss_fwd:
- *   lse[p] of each (packed) row, and by `reduce`
+ * hidden rows lie as fl_lse_f32_fwd_strided's (rows_per_group < 0: dense);
+ * weight rows are ldw elements apart, 16-byte aligned, ldw a multiple of 8 and
+ * at least Dp = D rounded up to 8; columns past D must be zero.  Dp - D
+ * columns need not exist in hidden.  `pack`:
+ *   0: hidden is read as it lies: D a multiple of 8, one row stride, a multiple
+ *      of 8, 16-byte aligned;
+ *   1: hidden rows are copied first (any layout);
+ *   2: only the rows whose target differs from ignore_index are copied, in
+ *      order; the others take no part in any product.
+ * fl_linear_loss_fwd writes by `reduce`, with lse the row's log-sum-exp,
  *   0: out[row] = z[row, target] - lse                       (log-probabilities)
- *   1: out[row] = lse - z[row, target] + z_loss * lse^2, 0 for rows not kept
- *   2, 3: out[0] = the sum of those, its mean over the kept rows (0 / 0 if none)
- *   hidden rows ldh, weight rows ldw elements apart: 16-byte aligned, multiples
- *   of 8; D a multiple of 8.  src and pos NULL: hidden is not packed (reduce 0
- *   and 1; meta is cleared by the call).  target int64 (N,), by original row; a
- *   kept target outside [0, V) makes its value NaN and, when err_flag is not
- *   NULL, sets *err_flag |= 1.  workspace: the forward size of
- *   fl_linear_loss_workspace, 256-byte aligned, one call in flight.
+ *   1: out[row] = lse - z[row, target] + z_loss * lse^2, 0 for rows left out
+ *   2, 3 (pack 2): out[0] = the sum of those, its mean over the rows kept
+ *      (0 / 0 if none)
+ *   and leaves in `state` what its backward reads.  target is int64 (N,); one
+ *   outside [0, V) makes its value NaN and, when err_flag is not NULL, sets
+ *   *err_flag |= 1.
  * fl_linear_loss_bwd: with grad one float (reduce 2, 3) or (N,) by row,
  *   d z = grad * (softmax (1 + 2 z_loss lse) - onehot)   (reduce 0: grad * (onehot - softmax))
- *   of `vocab_chunk` vocabulary columns at a time (0: a size that bounds the
- *   workspace; rounded down to a multiple of 256) is held in 16 bits, and
- *   grad_hidden (N, hidden_cols) dense, by original row (0 for rows not kept),
- *   grad_weight (V, D) dense; either may be NULL.  hidden_cols <= D is the
- *   width before padding.  A target outside [0, V) contributes no one-hot term.
- *   Sums run in a fixed order: equal calls give equal bits.
+ *   is formed for `vocab_chunk` vocabulary columns at a time (0: a size that
+ *   bounds the workspace; rounded down to a multiple of 256), in 16 bits, and
+ *   taken to grad_hidden (N, D) dense, zero in rows left out, and grad_weight
+ *   (V, Dp) dense; either may be NULL.  A target outside [0, V) contributes no
+ *   one-hot term.  Sums run in a fixed order: equal calls give equal bits.
+ * fl_linear_loss_sizes: bytes of state and of the two workspaces (256-byte
+ *   aligned, contents undefined on entry, one call in flight each).
  * Waits between the kernels' own copies and products end after 4 s at most;
  * the call's outputs are NaN then.
  * ---------------------------------------------------------------------- */
-int fl_linear_loss_workspace(int64_t N, int64_t V, int64_t D, int64_t vocab_chunk,
-                             int want_hidden, int64_t* forward, int64_t* backward);
-int fl_linear_loss_pack(const uint16_t* hidden, const int64_t* target, int64_t ignore_index,
-                        uint16_t* packed, int* src, int* pos, int* meta, int64_t N, int64_t D,
-                        int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
-                        fl_stream_t stream);
-int fl_linear_loss_fwd(const uint16_t* hidden, int64_t ldh, const uint16_t* weight, int64_t ldw,
-                       int dtype, const int64_t* target, const int* src, const int* pos, int* meta,
-                       int64_t N, int64_t V, int64_t D, int reduce, float z_loss, float* lse,
+int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int pack, int64_t vocab_chunk,
+                         int want_hidden, int64_t* state, int64_t* forward, int64_t* backward);
+int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group, int64_t group_stride,
+                       int64_t row_stride, const uint16_t* weight, int64_t ldw, int dtype,
+                       const int64_t* target, int pack, int64_t ignore_index, int64_t N, int64_t V,
+                       int64_t D, int reduce, float z_loss, void* state, int64_t state_bytes,
                        float* out, void* workspace, int64_t workspace_bytes, int* err_flag,
                        fl_stream_t stream);
-int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int64_t ldh,
-                       const uint16_t* weight, int64_t ldw, int dtype, const int64_t* target,
-                       const int* src, const int* pos, int* meta, const float* lse, int64_t N,
-                       int64_t V, int64_t D, int64_t hidden_cols, int reduce, float z_loss,
-                       int64_t vocab_chunk, uint16_t* grad_hidden, uint16_t* grad_weight,
+int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int64_t rows_per_group,
+                       int64_t group_stride, int64_t row_stride, const uint16_t* weight, int64_t ldw,
+                       int dtype, const int64_t* target, int pack, int64_t N, int64_t V, int64_t D,
+                       int reduce, float z_loss, int64_t vocab_chunk, void* state,
+                       int64_t state_bytes, uint16_t* grad_hidden, uint16_t* grad_weight,
                        void* workspace, int64_t workspace_bytes, fl_stream_t stream);
 
 /* ------------------------------------------------------------------------
