@@ -34,7 +34,6 @@ constexpr int kGemmThreads = 384;     // 4 warps of roles, 8 epilogue warps
 constexpr int kEpiWarps = 8;
 constexpr uint32_t kOperandBytes = kHalfTile * kBlockK * 2;   // 16 KB
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
-constexpr uint32_t kStageTx = 2 * kStageBytes;                // both CTAs' copies
 constexpr uint32_t kStagingBuf = 4096;                        // 32 rows of 128 bytes
 constexpr uint32_t kTmemCols = 512;                           // two fp32 accumulators
 
@@ -68,6 +67,9 @@ struct GemmArgs {
     int slab_rows;
     int add;               // add to the slab instead of storing it
     uint32_t idesc;
+    int a_rows;            // rows of A staged by a CTA that has any
+    int one_half;          // A has no rows for the pair's second CTA
+    int first;             // no kernel of the call has set meta
     int* meta;
     const int64_t* target;
     const int* src;        // packed row -> row of target
@@ -150,7 +152,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         if (EPI != kEpiStats) tma_prefetch_map(&map_out);
     }
     if (warp == 2) tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
-    if (threadIdx.x == 0) stop_flag = args.meta[kMetaStop];  // an earlier kernel of the call gave up
+    pdl_wait();
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        // whether an earlier kernel of the call gave up; the first one clears the words
+        stop_flag = args.first ? 0 : args.meta[kMetaStop];
+        if (args.first && blockIdx.x == 0) args.meta[kMetaStop] = 0;
+    }
     const int rows = args.packed ? args.meta[kMetaRows] : args.rows;
     tc_fence_before();
     __syncthreads();
@@ -170,6 +178,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         // ---- copies ----
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
+            const uint32_t stage_tx = 2 * kOperandBytes + (args.one_half ? 1 : 2) * args.a_rows * (kBlockK * 2);
             for (int u = pair; u < units && !*stop; u += pairs) {
                 const Unit t = decode_unit(u, mt, nt, args.splits, kb_total);
                 const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * kTile + rank * kHalfTile;
@@ -177,12 +186,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, stop)) break;
                     const uint32_t bar = map_to_rank(full0 + 8 * stage, 0);
                     const uint32_t sa = smem + stage * kStageBytes, sb = sa + kOperandBytes;
-                    if (rank == 0) mbar_expect_tx(full0 + 8 * stage, kStageTx);
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * stage, stage_tx);
                     const int k = kb * kBlockK;
                     if (Shape::kAMn) {
                         tma_load_pair(sa, &map_a, bar, ma, k);
                         tma_load_pair(sa + kOperandBytes / 2, &map_a, bar, ma + 64, k);
-                    } else {
+                    } else if (rank == 0 || !args.one_half) {
                         tma_load_pair(sa, &map_a, bar, k, ma);
                     }
                     if (Shape::kBMn) {
@@ -418,7 +427,9 @@ __device__ __forceinline__ int block_sum(int v, int* sh) {
 __global__ void __launch_bounds__(kPackThreads) pack_rows_kernel(
     const uint16_t* __restrict__ hidden, const int64_t* __restrict__ target, int64_t ignore,
     uint16_t* __restrict__ packed, int* __restrict__ src, int* __restrict__ pos, int* __restrict__ meta,
-    int N, int D, int Dp, RowMap rm) {
+    int N, int D, int Dp, int ld, RowMap rm) {
+    pdl_wait();
+    pdl_launch_dependents();
     __shared__ int sh[kPackThreads / 32];
     __shared__ int list[kPackThreads];
     const int r0 = static_cast<int>((int64_t)blockIdx.x * N / gridDim.x);
@@ -446,14 +457,14 @@ __global__ void __launch_bounds__(kPackThreads) pack_rows_kernel(
         }
         __syncthreads();
         for (int i = warp; i < n; i += kPackThreads / 32)
-            copy_row16(hidden + rm(list[i]), packed + (int64_t)(base + i) * Dp, D, Dp, lane);
+            copy_row16(hidden + rm(list[i]), packed + (int64_t)(base + i) * ld, D, Dp, lane);
         base += n;
     }
     if (blockIdx.x == gridDim.x - 1) {
         // the weight gradient sums over whole blocks of 64 packed rows
         const int end = min(N, max(kBlockK, (base + kBlockK - 1) / kBlockK * kBlockK));
         for (int i = base + warp; i < end; i += kPackThreads / 32)
-            for (int j = lane; j < Dp; j += 32) packed[(int64_t)i * Dp + j] = 0;
+            for (int j = lane; j < Dp; j += 32) packed[(int64_t)i * ld + j] = 0;
         if (threadIdx.x == 0) {
             meta[kMetaRows] = base;
             meta[kMetaCount] = 0;
@@ -462,14 +473,15 @@ __global__ void __launch_bounds__(kPackThreads) pack_rows_kernel(
     }
 }
 
-// Rows of D 16-bit elements to rows of Dp >= D (zero-filled) at stride Dp or,
-// with Dp < D, their first Dp elements.
+// Rows of D 16-bit elements to rows of Dp >= D (zero-filled) or, with Dp < D,
+// their first Dp elements; ld elements apart.
 __global__ void __launch_bounds__(256) copy_rows16_kernel(const uint16_t* __restrict__ src,
                                                           uint16_t* __restrict__ dst, int64_t rows, int D,
-                                                          int Dp, RowMap rm) {
+                                                          int Dp, int ld, RowMap rm) {
+    pdl_wait();
+    pdl_launch_dependents();
     const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row < rows)
-        copy_row16(src + rm(row), dst + row * Dp, min(D, Dp), Dp, threadIdx.x & 31);
+    if (row < rows) copy_row16(src + rm(row), dst + row * ld, min(D, Dp), Dp, threadIdx.x & 31);
 }
 
 // ---------------------------------------------------------------------------
@@ -477,37 +489,67 @@ __global__ void __launch_bounds__(256) copy_rows16_kernel(const uint16_t* __rest
 // ---------------------------------------------------------------------------
 enum Reduce { kLogp = 0, kNone = 1, kSum = 2, kMean = 3 };
 
+// WARPS warps of a CTA share a row: one while rows are many, all eight where a few
+// rows of many pieces would leave the SMs idle.
+template <int WARPS>
 __global__ void __launch_bounds__(256) finish_forward_kernel(
     const float2* __restrict__ part, int pieces, const float* __restrict__ zt,
     const int64_t* __restrict__ target, const int* __restrict__ pos, int* meta, int64_t N, int64_t V,
     float z_loss, int reduce, float* __restrict__ lse_out, float* values, float* __restrict__ out,
     int* err) {
     __shared__ double sums[8];
+    __shared__ float2 states[8];
     __shared__ int last;
+    pdl_wait();
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kRows = 8 / WARPS;
     const float nan = __int_as_float(0x7fc00000);
-    for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < N; row += (int64_t)gridDim.x * 8) {
+    for (int64_t row = (int64_t)blockIdx.x * kRows + warp / WARPS; row < N; row += (int64_t)gridDim.x * kRows) {
         const int64_t p = pos ? pos[row] : row;
         float value = 0.0f;
         if (p >= 0) {
+            const int64_t t = __ldg(target + row);
+            const bool bad = t < 0 || t >= V;
+            const float z = bad ? nan : __ldg(zt + p);
             float m = -INFINITY, s = 0.0f;
-            for (int i = lane; i < pieces; i += 32) {
-                const float2 v = __ldg(part + p * pieces + i);
+            const float2* pp = part + p * pieces;
+            constexpr int kStep = 32 * WARPS, U = 4;
+            int i = (WARPS > 1 ? warp * 32 : 0) + lane;
+            for (; i + (U - 1) * kStep < pieces; i += U * kStep) {
+                float2 v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = __ldg(pp + i + u * kStep);
+                const float M = max_nan(max_nan(max_nan(v[0].x, v[1].x), max_nan(v[2].x, v[3].x)), m);
+                const float Ms = safe_max(M);
+                s *= exp_from(m, Ms);
+#pragma unroll
+                for (int u = 0; u < U; ++u) s += v[u].y * exp_from(v[u].x, Ms);
+                m = M;
+            }
+            for (; i < pieces; i += kStep) {
+                const float2 v = __ldg(pp + i);
                 ms_merge(m, s, v.x, v.y);
             }
             ms_warp_allreduce(m, s);
+            if (WARPS > 1) {
+                if (lane == 0) states[warp] = make_float2(m, s);
+                __syncthreads();
+                m = states[0].x, s = states[0].y;
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) ms_merge(m, s, states[w].x, states[w].y);
+                __syncthreads();
+            }
             const float lse = ms_finalize(m, s, -INFINITY);
-            const int64_t t = __ldg(target + row);
-            const bool bad = t < 0 || t >= V;
-            if (lane == 0) {
+            if (lane == 0 && warp % WARPS == 0) {
                 lse_out[p] = lse;
                 if (bad && err) atomicOr(err, 1);
             }
-            const float nll = bad || meta[kMetaStop] ? nan : lse - __ldg(zt + p);
+            const float nll = meta[kMetaStop] ? nan : lse - z;
             value = reduce == kLogp ? -nll : nll;
             if (z_loss != 0.0f) value += z_loss * lse * lse;
         }
-        if (lane == 0) values[row] = value;
+        if (lane == 0 && warp % WARPS == 0) values[row] = value;
     }
     if (reduce == kLogp || reduce == kNone) return;  // values is the result
     __threadfence();
@@ -542,6 +584,8 @@ __global__ void __launch_bounds__(1024) coefficients_kernel(
     const float* __restrict__ g, int reduce, float z_loss, const float* __restrict__ lse,
     const int* __restrict__ src, const int* __restrict__ meta, int64_t N, float* __restrict__ a,
     float* __restrict__ b, float* __restrict__ inv_scale) {
+    pdl_wait();
+    pdl_launch_dependents();
     __shared__ float top[32];
     const int64_t rows = src ? meta[kMetaRows] : N;
     float g0 = 0.0f;
@@ -582,12 +626,14 @@ __global__ void __launch_bounds__(256) finish_hidden_kernel(const float* __restr
                                                             int64_t slab_elems, const int* __restrict__ pos,
                                                             const int* __restrict__ meta,
                                                             const float* __restrict__ inv_scale, int D,
-                                                            int Dp, uint16_t* __restrict__ out) {
+                                                            int ld, uint16_t* __restrict__ out) {
+    pdl_wait();
+    pdl_launch_dependents();
     const int64_t row = blockIdx.x;
     const int64_t p = pos ? pos[row] : row;
     const float scale = meta[kMetaStop] ? __int_as_float(0x7fc00000) : *inv_scale;
     uint16_t* o = out + row * D;
-    const float* s = slabs + p * Dp;
+    const float* s = slabs + p * ld;
     const bool wide = D % 4 == 0;
     for (int j = 4 * (blockIdx.y * 256 + threadIdx.x); j < D; j += 4 * 256 * gridDim.y) {
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -614,6 +660,10 @@ __global__ void __launch_bounds__(256) finish_hidden_kernel(const float* __restr
 constexpr int64_t kMaxExtent = INT32_MAX - 4 * kTile;
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Packed rows start on 128-byte lines: a copy of a row piece that straddles two
+// lines takes two requests (products of 1000-element rows measured 1.8x as long).
+int64_t packed_ld(int64_t D) { return round_up(D, 64); }
 
 // K pieces of the hidden gradient: as many as fill the CTA pairs best, at least
 // 8 blocks deep each and slabs of at most 64 MB in all (one slab is needed anyway).
@@ -643,7 +693,7 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidd
     if (chunk <= 0) chunk = (256ll << 20) / std::max<int64_t>(N, 1);
     p.chunk = std::min(all, std::max<int64_t>(kTile, chunk / kTile * kTile));
     p.slab_rows = round_up(N, kTile);
-    const int64_t slab = p.slab_rows * Dp * 4;
+    const int64_t slab = p.slab_rows * packed_ld(Dp) * 4;
     p.splits = want_hidden ? choose_splits((p.slab_rows / kTile) * ((Dp + kTile - 1) / kTile),
                                            p.chunk / kBlockK, slab, pairs)
                            : 0;
@@ -654,6 +704,11 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidd
     return p;
 }
 
+// Rows of A that a CTA stages: all 128, or with fewer rows than that in all, only
+// those (a whole number of 8-row groups).  Rows of the accumulator past them hold
+// whatever was staged there before and are never read.
+int staged_rows(int64_t rows) { return rows >= kHalfTile ? kHalfTile : (int)round_up(rows, 8); }
+
 template <int EPI>
 int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GemmArgs& args,
                    int64_t units, bool bf16, cudaStream_t stream, const char* what) {
@@ -661,7 +716,7 @@ int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
     constexpr uint32_t smem = GemmShape<EPI>::kSmem;
     FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const int64_t pairs = std::max<int64_t>(1, std::min<int64_t>(units, sm_count() / 2));
-    LaunchCfg lc(dim3((unsigned)(2 * pairs)), dim3(kGemmThreads), smem, stream, /*pdl=*/false);
+    LaunchCfg lc(dim3((unsigned)(2 * pairs)), dim3(kGemmThreads), smem, stream);
     FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, a, b, out, args));
     return check_launch(what);
 }
@@ -670,6 +725,15 @@ constexpr CUtensorMapDataType kMap16[2] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_T
 
 int64_t fwd_bytes(int64_t N, int64_t V) {
     return round_up(N * 2 * ((V + kTile - 1) / kTile) * 8, 256) + 2 * round_up(N * 4, 256);
+}
+
+int launch_copy_rows(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t D, int64_t Dp, int64_t ld,
+                     RowMap rm, cudaStream_t stream, const char* what) {
+    const int64_t grid = (rows + 7) / 8;
+    FL_REQUIRE(grid <= INT32_MAX, "%s: too many rows", what);
+    LaunchCfg lc(dim3((unsigned)grid), dim3(256), 0, stream);
+    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, copy_rows16_kernel, src, dst, rows, (int)D, (int)Dp, (int)ld, rm));
+    return check_launch(what);
 }
 
 // What a forward leaves for its backward: meta, the rows' lse, the packing's
@@ -684,7 +748,7 @@ struct State {
     int64_t bytes;
 };
 
-State lay_state(void* base, int64_t N, int64_t Dp, int pack) {
+State lay_state(void* base, int64_t N, int64_t D, int pack) {
     State s = {};
     char* p = static_cast<char*>(base);
     int64_t at = 256;
@@ -699,7 +763,7 @@ State lay_state(void* base, int64_t N, int64_t Dp, int pack) {
         s.src = reinterpret_cast<int*>(take(N * 4));
         s.pos = reinterpret_cast<int*>(take(N * 4));
     }
-    if (pack != kPackNone) s.packed = reinterpret_cast<uint16_t*>(take(N * Dp * 2));
+    if (pack != kPackNone) s.packed = reinterpret_cast<uint16_t*>(take(N * packed_ld(D) * 2));
     s.bytes = at;
     return s;
 }
@@ -742,9 +806,9 @@ int check_call(Call* c, const uint16_t* hidden, int64_t rows_per_group, int64_t 
     FL_REQUIRE(N == 0 || (weight && target && state), "%s: NULL buffer", what);
     FL_REQUIRE(aligned_to(hidden, 2) && aligned_to(target, 8) && aligned_to(state, 256), "%s: misaligned buffer",
                what);
-    FL_REQUIRE(N == 0 || state_bytes >= lay_state(nullptr, N, c->Dp, pack).bytes,
+    FL_REQUIRE(N == 0 || state_bytes >= lay_state(nullptr, N, D, pack).bytes,
                "%s: state of %lld bytes, %lld needed", what, (long long)state_bytes,
-               (long long)lay_state(nullptr, N, c->Dp, pack).bytes);
+               (long long)lay_state(nullptr, N, D, pack).bytes);
     c->hidden = hidden;
     return FL_OK;
 }
@@ -764,7 +828,7 @@ extern "C" int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int pack, i
         return st;
     FL_REQUIRE(N >= 0 && N <= kMaxExtent && vocab_chunk >= 0 && state && forward && backward,
                "%s: bad arguments", what);
-    *state = lay_state(nullptr, N, c.Dp, pack).bytes;
+    *state = lay_state(nullptr, N, D, pack).bytes;
     *forward = fwd_bytes(N, V);
     *backward = plan_bwd(N, V, c.Dp, vocab_chunk, want_hidden != 0, sm_count() / 2).bytes;
     return FL_OK;
@@ -784,11 +848,7 @@ extern "C" int fl_copy_rows16(const uint16_t* src, uint16_t* dst, int64_t rows, 
         rm = RowMap{rows_per_group, group_stride, row_stride};
     }
     if (int st = bind_device(stream, dst)) return st;
-    const int64_t grid = (rows + 7) / 8;
-    FL_REQUIRE(grid <= INT32_MAX, "%s: too many rows", what);
-    LaunchCfg lc(dim3((unsigned)grid), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), false);
-    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, copy_rows16_kernel, src, dst, rows, (int)D, (int)Dp, rm));
-    return check_launch(what);
+    return launch_copy_rows(src, dst, rows, D, Dp, Dp, rm, reinterpret_cast<cudaStream_t>(stream), what);
 }
 
 extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group, int64_t group_stride,
@@ -811,40 +871,38 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group
                (long long)workspace_bytes, (long long)fwd_bytes(N, V));
     if (int st = bind_device(stream, state)) return st;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const State keep = lay_state(state, N, c.Dp, pack);
+    const State keep = lay_state(state, N, D, pack);
     const uint16_t* h = hidden;
     int64_t ldh = c.ldh;
     if (pack == kPackKept) {
-        LaunchCfg lc(dim3((unsigned)std::min<int64_t>(N, 2 * sm_count())), dim3(kPackThreads), 0, s, false);
+        LaunchCfg lc(dim3((unsigned)std::min<int64_t>(N, 2 * sm_count())), dim3(kPackThreads), 0, s);
         FL_CUDA(cudaLaunchKernelEx(&lc.cfg, pack_rows_kernel, hidden, target, ignore_index, keep.packed, keep.src,
-                                   keep.pos, keep.meta, (int)N, (int)D, (int)c.Dp, c.rows));
+                                   keep.pos, keep.meta, (int)N, (int)D, (int)c.Dp, (int)packed_ld(D), c.rows));
         if (int st = check_launch(what)) return st;
-    } else {
-        FL_CUDA(cudaMemsetAsync(keep.meta, 0, 16, s));
-        if (pack == kPackAll) {
-            LaunchCfg lc(dim3((unsigned)((N + 7) / 8)), dim3(256), 0, s, false);
-            FL_CUDA(cudaLaunchKernelEx(&lc.cfg, copy_rows16_kernel, hidden, keep.packed, N, (int)D, (int)c.Dp,
-                                       c.rows));
-            if (int st = check_launch(what)) return st;
-        }
+    } else if (pack == kPackAll) {
+        if (int st = launch_copy_rows(hidden, keep.packed, N, D, c.Dp, packed_ld(D), c.rows, s, what)) return st;
     }
-    if (pack != kPackNone) h = keep.packed, ldh = c.Dp;
+    if (pack != kPackNone) h = keep.packed, ldh = packed_ld(D);
     const int64_t tiles_n = (V + kTile - 1) / kTile;
     float2* part = static_cast<float2*>(workspace);
     float* zt = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(N * 2 * tiles_n * 8, 256));
     float* values = reduce < kSum ? out
                                   : reinterpret_cast<float*>(reinterpret_cast<char*>(zt) + round_up(N * 4, 256));
     CUtensorMap a, b;
-    if (int st = make_tensor_map(&a, kMap16[dtype], 2, h, c.Dp, N, ldh, kBlockK, kHalfTile)) return st;
+    const int a_rows = staged_rows(N);
+    if (int st = make_tensor_map(&a, kMap16[dtype], 2, h, c.Dp, N, ldh, kBlockK, a_rows)) return st;
     if (int st = make_tensor_map(&b, kMap16[dtype], 2, weight, c.Dp, V, ldw, kBlockK, kHalfTile)) return st;
     GemmArgs g = {};
     g.rows = (int)N;
     g.packed = pack == kPackKept;
+    g.first = pack != kPackKept;
     g.m_extent = -1;
     g.n_extent = (int)V;
     g.k_extent = (int)c.Dp;
     g.splits = 1;
     g.idesc = umma_idesc(dtype == 1, false, false);
+    g.a_rows = a_rows;
+    g.one_half = N <= kHalfTile;
     g.meta = keep.meta;
     g.target = target;
     g.src = keep.src;
@@ -853,10 +911,11 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group
     g.zt = zt;
     if (int st = launch_product<kEpiStats>(a, b, a, g, ((N + kTile - 1) / kTile) * tiles_n, dtype == 1, s, what))
         return st;
-    const int64_t grid = std::min<int64_t>((N + 7) / 8, 8ll * sm_count());
-    LaunchCfg lc(dim3((unsigned)grid), dim3(256), 0, s, false);
-    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, finish_forward_kernel, (const float2*)part, g.pieces, (const float*)zt,
-                               target, (const int*)keep.pos, keep.meta, N, V, z_loss, reduce, keep.lse, values, out,
+    const bool few = N <= 2 * sm_count();
+    auto finish = few ? finish_forward_kernel<8> : finish_forward_kernel<1>;
+    LaunchCfg lc(dim3((unsigned)(few ? N : std::min<int64_t>((N + 7) / 8, 8ll * sm_count()))), dim3(256), 0, s);
+    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, finish, (const float2*)part, g.pieces, (const float*)zt, target,
+                               (const int*)keep.pos, keep.meta, N, V, z_loss, reduce, keep.lse, values, out,
                                err_flag));
     return check_launch(what);
 }
@@ -892,9 +951,9 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     FL_REQUIRE(workspace_bytes >= plan.bytes, "%s: workspace of %lld bytes, %lld needed", what,
                (long long)workspace_bytes, (long long)plan.bytes);
     FL_REQUIRE(plan.slab_rows * std::max(plan.splits, 1) <= kMaxExtent, "%s: shape too large", what);
-    const State keep = lay_state(state, N, Dp, pack);
+    const State keep = lay_state(state, N, D, pack);
     const uint16_t* h = pack == kPackNone ? hidden : keep.packed;
-    const int64_t ldh = pack == kPackNone ? c.ldh : Dp;
+    const int64_t ldh = pack == kPackNone ? c.ldh : packed_ld(D);
     char* ws = static_cast<char*>(workspace);
     float* inv_scale = reinterpret_cast<float*>(ws);
     float* ca = reinterpret_cast<float*>(ws + plan.coef_off);
@@ -903,7 +962,7 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     uint16_t* dz = reinterpret_cast<uint16_t*>(ws + plan.dz_off);
     const bool bf16 = dtype == 1;
     {
-        LaunchCfg lc(dim3(1), dim3(1024), 0, s, false);
+        LaunchCfg lc(dim3(1), dim3(1024), 0, s);
         FL_CUDA(cudaLaunchKernelEx(&lc.cfg, coefficients_kernel, grad, reduce, z_loss, (const float*)keep.lse,
                                    (const int*)keep.src, (const int*)keep.meta, N, ca, cb, inv_scale));
         if (int st = check_launch(what)) return st;
@@ -911,7 +970,8 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     // operand and output views: hidden and weight by rows and by columns, dz both ways
     CUtensorMap h_k, w_k, dz_out, dz_mn, h_mn, dw_out, dz_k, w_mn, slab_out;
     const CUtensorMapDataType t16 = kMap16[dtype];
-    if (int st = make_tensor_map(&h_k, t16, 2, h, Dp, N, ldh, kBlockK, kHalfTile)) return st;
+    const int a_rows = staged_rows(N);
+    if (int st = make_tensor_map(&h_k, t16, 2, h, Dp, N, ldh, kBlockK, a_rows)) return st;
     if (int st = make_tensor_map(&w_k, t16, 2, weight, Dp, V, ldw, kBlockK, kHalfTile)) return st;
     if (int st = make_tensor_map(&dz_out, t16, 2, dz, plan.chunk, N, plan.chunk, 64, 32)) return st;
     if (grad_weight) {
@@ -920,16 +980,18 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
         if (int st = make_tensor_map(&dw_out, t16, 2, grad_weight, Dp, V, Dp, 64, 32)) return st;
     }
     if (grad_hidden) {
-        if (int st = make_tensor_map(&dz_k, t16, 2, dz, plan.chunk, N, plan.chunk, kBlockK, kHalfTile)) return st;
+        if (int st = make_tensor_map(&dz_k, t16, 2, dz, plan.chunk, N, plan.chunk, kBlockK, a_rows)) return st;
         if (int st = make_tensor_map(&w_mn, t16, 2, weight, Dp, V, ldw, 64, kBlockK)) return st;
         if (int st = make_tensor_map(&slab_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, slabs, Dp,
-                                     plan.slab_rows * plan.splits, Dp, 32, 32))
+                                     plan.slab_rows * plan.splits, packed_ld(D), 32, 32))
             return st;
     }
     GemmArgs base = {};
     base.rows = (int)N;
     base.packed = pack == kPackKept;
     base.splits = 1;
+    base.a_rows = a_rows;
+    base.one_half = N <= kHalfTile;
     base.meta = keep.meta;
     const int64_t mt = (N + kTile - 1) / kTile, dt = (Dp + kTile - 1) / kTile;
     for (int64_t v0 = 0; v0 < V; v0 += plan.chunk) {
@@ -953,6 +1015,8 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
             g.k_extent = -1;
             g.out_row = (int)v0;
             g.idesc = umma_idesc(bf16, true, true);
+            g.a_rows = kHalfTile;
+            g.one_half = 0;
             g.inv_scale = inv_scale;
             g.out = grad_weight;
             g.out_elems = V * Dp;
@@ -975,10 +1039,10 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     if (grad_hidden) {
         auto kern = bf16 ? finish_hidden_kernel<true> : finish_hidden_kernel<false>;
         const int64_t gy = std::min<int64_t>(8, (D + 1023) / 1024);
-        LaunchCfg lc(dim3((unsigned)N, (unsigned)gy), dim3(256), 0, s, false);
-        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, (const float*)slabs, plan.splits, plan.slab_rows * Dp,
-                                   (const int*)keep.pos, (const int*)keep.meta, (const float*)inv_scale, (int)D,
-                                   (int)Dp, grad_hidden));
+        LaunchCfg lc(dim3((unsigned)N, (unsigned)gy), dim3(256), 0, s);
+        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, (const float*)slabs, plan.splits,
+                                   plan.slab_rows * packed_ld(D), (const int*)keep.pos, (const int*)keep.meta,
+                                   (const float*)inv_scale, (int)D, (int)packed_ld(D), grad_hidden));
         return check_launch(what);
     }
     return FL_OK;

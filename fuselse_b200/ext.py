@@ -266,6 +266,10 @@ def _hidden_rows(hidden: torch.Tensor):
     N, D, rpg, gs, rs = lay
     plain = (D % 8 == 0 and rs % 8 == 0 and rs >= D and (rpg < 0 or rpg >= N)
              and hidden.data_ptr() % 16 == 0)
+    # rows off the 128-byte lines are read at half the rate by every vocabulary tile: many of
+    # them are worth one copy
+    if plain and N > 128 and rs % 64:
+        plain = False
     return hidden, rpg, gs, rs, plain
 
 
