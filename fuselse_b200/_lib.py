@@ -79,7 +79,8 @@ SIGNATURES = {
     "fl_copy_rows16": [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _stream],
     "fl_topk_distill_fwd": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64,
                             c_int64, c_int64, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-                            c_void_p, c_void_p, _stream],
+                            c_void_p, c_void_p, c_int64, c_void_p, _stream],
+    "fl_topk_distill_workspace": [c_int64, c_int64, c_int, POINTER(c_int64)],
     "fl_topk_distill_bwd": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64,
                             c_int64, c_int64, c_int64, c_float, c_int, c_void_p, c_void_p, c_void_p,
                             c_void_p, _stream],

@@ -2,16 +2,19 @@
 // (V entries) and K teacher logits t_j at columns i_j,
 //   p = softmax(t / T) over the kept entries, q = softmax(z / T),
 //   loss = T^2 sum_j p_j (log p_j - log q_{i_j}),  d loss / d z = T (q - p).
-// Forward: one pass over z folds (max, sum-exp) of z / T; the K entries are
-// gathered while it streams.  Backward: one read and one write of each element,
-// then the K entries of the row are put right by the CTA that wrote them.
+// Forward: one pass over z folds pieces of rows to (max, sum-exp), a second small
+// kernel merges a row's pieces with its K entries.  Backward: one read and one
+// write of each element, then the K entries of the row are put right by the CTA
+// that wrote them.
 // Both are bound by memory: V elements per row read, and read and written.
 #include "common.cuh"
+#include "pairs.cuh"
 #include "rows.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <type_traits>
 
 namespace fl {
 
@@ -34,7 +37,9 @@ struct Elem<__nv_bfloat16> {
 namespace {
 
 constexpr int kMaxTop = 1024;
-constexpr int kDThreads = 256;
+// Backward: 128 threads with 8 vectors each, one pass (16 KB of x per CTA): 174 us at
+// (2048, 128256) bf16 against 203 for 256 x 8, 197 for 128 x 4, 186 for 128 x 16.
+constexpr int kDThreads = 128, kBVec = 8;
 
 template <typename T>
 __device__ __forceinline__ T narrow(float v);
@@ -89,26 +94,68 @@ struct Teacher {
 // Padding entries (index -1) and entries of -inf carry no probability.
 __device__ __forceinline__ bool kept(float t, int64_t column) { return column != -1 && t != -INFINITY; }
 
-template <int K>
-__device__ __forceinline__ void scale_by(float* v, float inv_t) {
-#pragma unroll
-    for (int i = 0; i < K; ++i) v[i] *= inv_t;
+// The temperature enters as the scale of the base-2 exponents, log2(e) / T, and
+// every maximum and log-sum-exp is kept in the logits' own units, T * LSE(z / T):
+// no element is multiplied by 1 / T.
+__device__ __forceinline__ float finalize_scaled(float m, float s, float temp) {
+    if (m != m || m == INFINITY || m == -INFINITY) return m;
+    return m + temp * logf(s);
 }
 
-// One warp forms the row's value from lse = LSE(z / T) and its own pass over the
-// K entries; every lane ends with it, and with the teacher's lse (-inf: nothing kept).
+__device__ __forceinline__ void warp_merge_scaled(float& m, float& s, float scale) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, off);
+        const float s2 = __shfl_xor_sync(0xffffffffu, s, off);
+        ms_merge_scaled(m, s, m2, s2, scale);
+    }
+}
+
+// Largest of U 16-byte vectors: 16-bit elements are compared two at a time as they come.
+template <typename T, int U>
+__device__ __forceinline__ float max_vectors(const uint4* r, const float* v, float m) {
+    if constexpr (sizeof(T) == 4) {
+        return max_of<U * 4>(m, v);
+    } else {
+        auto max2 = [](uint32_t a, uint32_t b) {
+            uint32_t o;
+            if constexpr (std::is_same<T, __half>::value)
+                asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(o) : "r"(a), "r"(b));
+            else
+                asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o) : "r"(a), "r"(b));
+            return o;
+        };
+        uint32_t t = max2(max2(r[0].x, r[0].y), max2(r[0].z, r[0].w));
+#pragma unroll
+        for (int u = 1; u < U; ++u) t = max2(t, max2(max2(r[u].x, r[u].y), max2(r[u].z, r[u].w)));
+        const uint4 one = make_uint4(t, t, t, t);
+        float w[8];
+        Elem<T>::unpack(one, w);
+        return max3_nan(m, w[0], w[1]);
+    }
+}
+
+// A warp's pass over a row's K entries, all that does not need the student's lse:
+// the teacher's lse (in logit units; -inf: nothing kept), sum p_j and
+// sum p_j (t_j - z_j).  0 log 0 = 0: an entry without probability adds nothing.
+struct TeacherSums {
+    float lse, p, pd;
+    bool bad;
+};
+
 template <typename T>
-__device__ __forceinline__ float row_loss(const T* rowp, int64_t V, int64_t row, const Teacher& te,
-                                          float lse, float inv_t, float t2, float& teacher_lse, bool& bad) {
+__device__ __forceinline__ TeacherSums teacher_sums(const T* rowp, int64_t V, int64_t row, const Teacher& te,
+                                                    float temp, float scale) {
     const int lane = threadIdx.x & 31;
     float m = -INFINITY, s = 0.0f;
     for (int j = lane; j < te.K; j += 32) {
         const float t = te.logit(row, j);
-        if (kept(t, te.column(row, j))) ms_fold1(m, s, t * inv_t);
+        if (kept(t, te.column(row, j))) ms_merge_scaled(m, s, t, 1.0f, scale);
     }
-    ms_warp_allreduce(m, s);
-    teacher_lse = ms_finalize(m, s, -INFINITY);
-    float sum = 0.0f;
+    warp_merge_scaled(m, s, scale);
+    TeacherSums r;
+    r.lse = finalize_scaled(m, s, temp);
+    r.p = r.pd = 0.0f;
     bool off = false;
     for (int j = lane; j < te.K; j += 32) {
         const float t = te.logit(row, j);
@@ -118,116 +165,143 @@ __device__ __forceinline__ float row_loss(const T* rowp, int64_t V, int64_t row,
             off = true;
             continue;
         }
-        const float lp = t * inv_t - teacher_lse;
-        const float p = ex2(lp * kLog2e);
-        // log p - log q, taken as (t - z) / T - (teacher lse - lse): near a matched
-        // student both differences are small and exact
-        const float gap = (t * inv_t - Elem<T>::load1(rowp + c) * inv_t) - (teacher_lse - lse);
-        if (p != 0.0f) sum += p * gap;  // 0 log 0 = 0, a NaN stays
+        const float p = ex2((t - r.lse) * scale);
+        if (p != 0.0f) {  // a NaN stays
+            r.p += p;
+            r.pd += p * (t - Elem<T>::load1(rowp + c));
+        }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    bad = __any_sync(0xffffffffu, off);
-    if (teacher_lse == -INFINITY) return 0.0f;
-    return bad ? __int_as_float(0x7fc00000) : t2 * sum;
+    for (int o = 16; o > 0; o >>= 1) {
+        r.p += __shfl_xor_sync(0xffffffffu, r.p, o);
+        r.pd += __shfl_xor_sync(0xffffffffu, r.pd, o);
+    }
+    r.bad = __any_sync(0xffffffffu, off);
+    return r;
 }
 
-// A CTA per row segment, the nseg CTAs of a row in one cluster (as lse_segment_kernel).
-template <typename T, bool SCALED>
-__global__ void __launch_bounds__(kDThreads) distill_fwd_kernel(
-    const T* __restrict__ x, int64_t V, RowMap rm, Teacher te, float inv_t, float t2, int nseg,
-    float* __restrict__ lse_out, float* __restrict__ teacher_lse_out, float* __restrict__ values,
-    int* __restrict__ err) {
-    constexpr int E = Elem<T>::kPerVec, U = 4;
-    __shared__ float2 seg[kMaxSeg];
-    const int64_t row = blockIdx.x / nseg;
-    const int rank = blockIdx.x % nseg;
+// Fold of one piece of a row by a CTA of its own, so that a grid of many short CTAs
+// stays balanced to its end: `rounds` rounds of 128 threads with 4 vectors each.
+// 4 rounds (32 KB pieces) measured 96 us at (2048, 128256) bf16 with the rows' kernel
+// (108 for 2 rounds, 99 for 8; one CTA or cluster per row 104); 1 round while that
+// still leaves SMs without a CTA (4 rows: 10.2 us against 12.3).
+constexpr int kFThreads = 128, kFVec = 4;
+constexpr int kRoundVec = kFThreads * kFVec;
+
+template <typename T>
+__global__ void __launch_bounds__(kFThreads) distill_pieces_kernel(const T* __restrict__ x, int64_t V,
+                                                                   RowMap rm, float scale, int pieces,
+                                                                   int rounds, float2* __restrict__ part,
+                                                                   int* __restrict__ arrived) {
+    constexpr int E = Elem<T>::kPerVec, U = kFVec;
+    const int64_t row = blockIdx.x / pieces;
+    const int piece = blockIdx.x % pieces;
     const T* rowp = x + rm(row);
     const int64_t head = head_elems(rowp, V), nv = (V - head) / E, tail0 = head + nv * E;
-    const int64_t per = (nv + nseg - 1) / nseg;
-    const int64_t v0 = min(nv, per * rank), v1 = min(nv, v0 + per);
-    const uint4* vp = reinterpret_cast<const uint4*>(rowp + head);
-    if (nseg > 1) cluster_arrive_relaxed();
+    const int64_t v0 = min(nv, (int64_t)piece * rounds * kRoundVec);
+    const int nvec = static_cast<int>(min(nv, v0 + rounds * kRoundVec) - v0);
+    const uint4* vp = reinterpret_cast<const uint4*>(rowp + head) + v0;
+    pdl_wait();
+    pdl_launch_dependents();
     float m = -INFINITY, s = 0.0f;
-    int64_t i = v0 + threadIdx.x;
-    for (; i + (U - 1) * kDThreads < v1; i += U * kDThreads) {
+    int i = threadIdx.x;
+    for (; i + (U - 1) * kFThreads < nvec; i += U * kFThreads) {
         uint4 r[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) r[u] = ld_stream_u4(vp + i + u * kDThreads);
+        for (int u = 0; u < U; ++u) r[u] = ld_stream_u4(vp + i + u * kFThreads);
         float v[U * E];
 #pragma unroll
         for (int u = 0; u < U; ++u) Elem<T>::unpack(r[u], v + u * E);
-        if (SCALED) scale_by<U * E>(v, inv_t);
-        ms_fold<U * E>(m, s, v);
+        fold_pairs<U * E>(m, s, v, max_vectors<T, U>(r, v, m), scale);
     }
-    for (; i < v1; i += kDThreads) {
+    for (; i < nvec; i += kFThreads) {
+        const uint4 r = ld_stream_u4(vp + i);
         float v[E];
-        Elem<T>::unpack(ld_stream_u4(vp + i), v);
-        if (SCALED) scale_by<E>(v, inv_t);
-        ms_fold<E>(m, s, v);
+        Elem<T>::unpack(r, v);
+        fold_pairs<E>(m, s, v, max_vectors<T, 1>(&r, v, m), scale);
     }
-    if (rank == 0) {
-        if (threadIdx.x < head) ms_fold1(m, s, Elem<T>::load1(rowp + threadIdx.x) * inv_t);
-        if (tail0 + threadIdx.x < V) ms_fold1(m, s, Elem<T>::load1(rowp + tail0 + threadIdx.x) * inv_t);
-    }
-    ms_block_reduce<kDThreads>(m, s);
-    if (nseg > 1) {
-        cluster_wait();
-        if (threadIdx.x == 0) {
-            const uint32_t own = static_cast<uint32_t>(__cvta_generic_to_shared(&seg[rank]));
-            uint32_t dst;
-            asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(dst) : "r"(own));
-            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(m), "f"(s) : "memory");
-        }
-        asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        if (rank != 0) return;
-    }
-    if (threadIdx.x >= 32) return;
-    if (nseg > 1) {
-        m = seg[0].x, s = seg[0].y;
-        for (int r = 1; r < nseg; ++r) ms_merge(m, s, seg[r].x, seg[r].y);
-    } else {
-        m = __shfl_sync(0xffffffffu, m, 0);
-        s = __shfl_sync(0xffffffffu, s, 0);
-    }
-    const float lse = ms_finalize(m, s, -INFINITY);
-    float tl;
-    bool bad;
-    const float value = row_loss(rowp, V, row, te, lse, inv_t, t2, tl, bad);
+    auto one = [&](int64_t e) {
+        const float z = Elem<T>::load1(rowp + e);
+        ms_merge_scaled(m, s, z, z == -INFINITY ? 0.0f : 1.0f, scale);
+    };
+    if (piece == 0 && threadIdx.x < head) one(threadIdx.x);
+    if (piece == pieces - 1 && tail0 + threadIdx.x < V) one(tail0 + threadIdx.x);
+    warp_merge_scaled(m, s, scale);
+    __shared__ float2 states[kFThreads / 32];
+    if ((threadIdx.x & 31) == 0) states[threadIdx.x >> 5] = make_float2(m, s);
+    __syncthreads();
     if (threadIdx.x == 0) {
-        lse_out[row] = lse;
-        teacher_lse_out[row] = tl;
-        values[row] = value;
-        if (bad && err) atomicOr(err, 1);
+#pragma unroll
+        for (int w = 1; w < kFThreads / 32; ++w) ms_merge_scaled(m, s, states[w].x, states[w].y, scale);
+        part[blockIdx.x] = make_float2(m, s);
+        if (blockIdx.x == 0) *arrived = 0;
     }
 }
 
-// Sum or mean (over the rows that keep an entry) in a fixed order, in 64 bits.
-__global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __restrict__ values,
-                                                              const float* __restrict__ teacher_lse,
-                                                              int64_t N, int mean, float* __restrict__ out,
-                                                              float* __restrict__ count_out) {
-    __shared__ double sums[32];
-    __shared__ int counts[32];
+// One warp merges a row's pieces and forms its value; the last CTA to finish sums
+// the rows (in a fixed order, in 64 bits) for a reduced loss.
+template <typename T>
+__global__ void __launch_bounds__(256) distill_rows_kernel(
+    const T* __restrict__ x, int64_t N, int64_t V, RowMap rm, Teacher te, float temp, float scale, int pieces,
+    const float2* part, int* arrived, int reduce, float* __restrict__ lse_out,
+    float* teacher_lse, float* values, float* __restrict__ out, float* __restrict__ count_out,
+    int* __restrict__ err) {
+    __shared__ double sums[8];
+    __shared__ int counts[8];
+    __shared__ int last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // Only the pieces come from the kernel before this one, which itself waited for all
+    // earlier ones: the first row's entries are read while its last CTAs still run.
+    bool waited = false;
+    for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < N; row += (int64_t)gridDim.x * 8) {
+        const TeacherSums t = teacher_sums(x + rm(row), V, row, te, temp, scale);
+        if (!waited) pdl_wait();
+        waited = true;
+        float m = -INFINITY, s = 0.0f;
+        for (int i = lane; i < pieces; i += 32) {
+            const float2 v = __ldcg(part + row * pieces + i);
+            ms_merge_scaled(m, s, v.x, v.y, scale);
+        }
+        warp_merge_scaled(m, s, scale);
+        const float lse = finalize_scaled(m, s, temp);
+        // T^2 sum p (log p - log q) = T (sum p (t - z) - (teacher lse - lse) sum p)
+        float value = temp * (t.pd - (t.lse - lse) * t.p);
+        if (t.lse == -INFINITY) value = 0.0f;
+        else if (t.bad) value = __int_as_float(0x7fc00000);
+        if (lane == 0) {
+            lse_out[row] = lse;
+            teacher_lse[row] = t.lse;
+            values[row] = value;
+            if (t.bad && err) atomicOr(err, 1);
+        }
+    }
+    if (!waited) pdl_wait();
+    pdl_launch_dependents();
+    if (reduce == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(arrived, 1) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
     double sum = 0.0;
     int count = 0;
-    for (int64_t i = threadIdx.x; i < N; i += 1024) {
-        sum += values[i];
-        count += teacher_lse[i] != -INFINITY;
+    for (int64_t i = threadIdx.x; i < N; i += 256) {
+        sum += __ldcg(values + i);
+        count += __ldcg(teacher_lse + i) != -INFINITY;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
         count += __shfl_xor_sync(0xffffffffu, count, o);
     }
-    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum, counts[threadIdx.x >> 5] = count;
+    if (lane == 0) sums[warp] = sum, counts[warp] = count;
     __syncthreads();
     if (threadIdx.x == 0) {
         sum = 0.0, count = 0;
-        for (int w = 0; w < 32; ++w) sum += sums[w], count += counts[w];
-        *out = static_cast<float>(mean ? sum / count : sum);
-        if (mean) *count_out = static_cast<float>(count);
+        for (int w = 0; w < 8; ++w) sum += sums[w], count += counts[w];
+        *out = static_cast<float>(reduce == 3 ? sum / count : sum);
+        if (reduce == 3) *count_out = static_cast<float>(count);
     }
 }
 
@@ -236,10 +310,10 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __res
 template <typename T>
 __global__ void __launch_bounds__(kDThreads) distill_bwd_kernel(
     const float* __restrict__ g, int scalar_g, const float* __restrict__ count, float temp,
-    const T* __restrict__ x, int64_t V, RowMap rm, Teacher te, float inv_t,
+    const T* __restrict__ x, int64_t V, RowMap rm, Teacher te, float scale,
     const float* __restrict__ lse_in, const float* __restrict__ teacher_lse_in, T* __restrict__ gx,
-    int nchunk, int64_t chunk_vec) {
-    constexpr int E = Elem<T>::kPerVec, U = 4;
+    int nchunk) {
+    constexpr int E = Elem<T>::kPerVec, U = kBVec;
     __shared__ int fix_col[kMaxTop];
     __shared__ float fix_p[kMaxTop];
     __shared__ int fix_n;
@@ -247,18 +321,31 @@ __global__ void __launch_bounds__(kDThreads) distill_bwd_kernel(
     const int64_t row = blockIdx.x / nchunk;
     const T* rowp = x + rm(row);
     T* outp = gx + row * V;
+    const int64_t head = head_elems(rowp, V), nv = (V - head) / E, tail0 = head + nv * E;
+    const int64_t v0 = min(nv, chunk * (int64_t)(U * kDThreads)), v1 = min(nv, v0 + U * kDThreads);
+    const uint4* vp = reinterpret_cast<const uint4*>(rowp + head) + v0;
+    uint4* op = reinterpret_cast<uint4*>(outp + head) + v0;
+    const int nvec = static_cast<int>(v1 - v0);
+    const bool vector = ((reinterpret_cast<uintptr_t>(rowp) ^ reinterpret_cast<uintptr_t>(outp)) & 15u) == 0;
+    if (threadIdx.x == 0) fix_n = 0;
+    pdl_wait();
+    pdl_launch_dependents();
+    // the chunk's elements are on their way while the row's figures and entries are looked up
+    uint4 r[U];
+    if (vector) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (threadIdx.x + u * kDThreads < nvec) r[u] = ld_stream_u4(vp + threadIdx.x + u * kDThreads);
+    }
     const float lse = __ldg(lse_in + row), tl = __ldg(teacher_lse_in + row);
     const bool live = tl != -INFINITY;
     float c = scalar_g ? __ldg(g) : __ldg(g + row);
     if (count) c /= __ldg(count);
     c *= temp;
-    const int64_t head = head_elems(rowp, V), nv = (V - head) / E, tail0 = head + nv * E;
-    const int64_t v0 = min(nv, chunk * chunk_vec), v1 = min(nv, v0 + chunk_vec);
-    auto q = [&](float z) { return live ? c * exp_from(z * inv_t, lse) : 0.0f; };
+    auto q = [&](float z) { return live ? c * ex2((z - lse) * scale) : 0.0f; };
     // this chunk's columns (the first chunk has the head, the last the tail)
     const int64_t c0 = chunk == 0 ? 0 : head + v0 * E;
     const int64_t c1 = chunk == nchunk - 1 ? V : head + v1 * E;
-    if (threadIdx.x == 0) fix_n = 0;
     __syncthreads();
     if (live) {
         for (int j = threadIdx.x; j < te.K; j += kDThreads) {
@@ -268,7 +355,7 @@ __global__ void __launch_bounds__(kDThreads) distill_bwd_kernel(
                 if (t != -INFINITY) {
                     const int at = atomicAdd(&fix_n, 1);
                     fix_col[at] = static_cast<int>(col - c0);
-                    fix_p[at] = ex2((t * inv_t - tl) * kLog2e);
+                    fix_p[at] = ex2((t - tl) * scale);
                 }
             }
         }
@@ -277,25 +364,23 @@ __global__ void __launch_bounds__(kDThreads) distill_bwd_kernel(
         outp[threadIdx.x] = narrow<T>(q(Elem<T>::load1(rowp + threadIdx.x)));
     if (chunk == nchunk - 1 && tail0 + threadIdx.x < V)
         outp[tail0 + threadIdx.x] = narrow<T>(q(Elem<T>::load1(rowp + tail0 + threadIdx.x)));
-    const uint4* vp = reinterpret_cast<const uint4*>(rowp + head);
-    if (((reinterpret_cast<uintptr_t>(rowp) ^ reinterpret_cast<uintptr_t>(outp)) & 15u) == 0) {
-        uint4* op = reinterpret_cast<uint4*>(outp + head);
-        auto vec = [&](uint4 r) {
-            float v[E];
-            Elem<T>::unpack(r, v);
+    const f32x2 neg_lse = pair(-lse, -lse), scale2 = pair(scale, scale), c2 = pair(c, c);
+    if (vector) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = q(v[e]);
-            return pack_vec<T>(v);
-        };
-        int64_t i = v0 + threadIdx.x;
-        for (; i + (U - 1) * kDThreads < v1; i += U * kDThreads) {
-            uint4 r[U];
+        for (int u = 0; u < U; ++u) {
+            if (threadIdx.x + u * kDThreads < nvec) {
+                float v[E];
+                Elem<T>::unpack(r[u], v);
 #pragma unroll
-            for (int u = 0; u < U; ++u) r[u] = ld_stream_u4(vp + i + u * kDThreads);
-#pragma unroll
-            for (int u = 0; u < U; ++u) __stcs(op + i + u * kDThreads, vec(r[u]));
+                for (int e = 0; e < E; e += 2) {
+                    const float2 t = exp_pair(pair(v[e], v[e + 1]), neg_lse, scale2);
+                    const float2 o = unpair(mul2(pair(t.x, t.y), c2));
+                    v[e] = live ? o.x : 0.0f;
+                    v[e + 1] = live ? o.y : 0.0f;
+                }
+                __stcs(op + threadIdx.x + u * kDThreads, pack_vec<T>(v));
+            }
         }
-        for (; i < v1; i += kDThreads) __stcs(op + i, vec(ld_stream_u4(vp + i)));
     } else {
         // x and gx rows start at different phases of 16 bytes: element by element
         for (int64_t e = head + v0 * E + threadIdx.x; e < head + v1 * E; e += kDThreads)
@@ -334,7 +419,7 @@ __global__ void __launch_bounds__(kDThreads) distill_bwd_kernel(
             }
         }
         const int64_t e = c0 + col;
-        outp[e] = narrow<T>(c * (exp_from(Elem<T>::load1(rowp + e) * inv_t, lse) - sum));
+        outp[e] = narrow<T>(c * (ex2((Elem<T>::load1(rowp + e) - lse) * scale) - sum));
     }
 }
 
@@ -346,7 +431,7 @@ int check_distill(const void* x, int dtype, const void* tlogits, int tdtype, con
     FL_REQUIRE(N >= 0 && V >= 1 && K >= 1, "%s: bad shape (%lld, %lld), %lld teacher entries", what,
                (long long)N, (long long)V, (long long)K);
     FL_REQUIRE(K <= kMaxTop, "%s: at most %d teacher entries", what, kMaxTop);
-    FL_REQUIRE(V <= INT32_MAX, "%s: V too large", what);
+    FL_REQUIRE(V <= INT32_MAX && N <= INT32_MAX, "%s: shape too large", what);
     FL_REQUIRE(dtype >= 0 && dtype <= 2 && tdtype >= 0 && tdtype <= 2, "%s: unknown dtype", what);
     FL_REQUIRE(temperature > 0.0f && temperature <= 3.0e38f, "%s: temperature must be positive", what);
     FL_REQUIRE(N == 0 || (x && tlogits && index), "%s: NULL buffer", what);
@@ -365,19 +450,43 @@ int distill_rows(int64_t N, int64_t V, int64_t rows_per_group, int64_t group_str
     return FL_OK;
 }
 
+constexpr int kElemBytes[3] = {4, 2, 2};
+
+struct Pieces {
+    int rounds;
+    int64_t count;  // per row
+};
+
+// At most 7 elements of a row's head and 7 of its tail lie outside whole vectors.
+Pieces row_pieces(int64_t N, int64_t V, int dtype) {
+    const int64_t vectors = V * kElemBytes[dtype] / 16;
+    auto count = [&](int rounds) {
+        return std::max<int64_t>(1, (vectors + rounds * kRoundVec - 1) / (rounds * kRoundVec));
+    };
+    const int rounds = N * count(4) >= 2ll * kNumSMs ? 4 : 1;
+    return Pieces{rounds, count(rounds)};
+}
+
+int64_t distill_bytes(int64_t N, int64_t V, int dtype) { return 256 + N * row_pieces(N, V, dtype).count * 8; }
+
 template <typename T>
-int launch_fwd(const void* x, int64_t N, int64_t V, RowMap rm, Teacher te, float temp, float* lse,
-               float* tlse, float* values, int* err, cudaStream_t s, const char* what) {
-    // rows that cannot fill the SMs are split over a cluster, at least 32 KB to a CTA
-    const int64_t target = 2ll * sm_count(), bytes = V * (int64_t)sizeof(T);
-    int64_t nseg = N >= target ? 1 : (target + N - 1) / N;
-    nseg = std::max<int64_t>(1, std::min<int64_t>({nseg, bytes / 32768, (int64_t)kMaxSeg}));
-    FL_REQUIRE(N * nseg <= INT32_MAX, "%s: too many rows", what);
-    LaunchCfg lc(dim3((unsigned)(N * nseg)), dim3(kDThreads), 0, s, false);
-    lc.cluster((int)nseg);
-    auto kern = temp == 1.0f ? distill_fwd_kernel<T, false> : distill_fwd_kernel<T, true>;
-    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, static_cast<const T*>(x), V, rm, te, 1.0f / temp, temp * temp,
-                               (int)nseg, lse, tlse, values, err));
+int launch_fwd(const void* x, int64_t N, int64_t V, RowMap rm, Teacher te, float temp, Pieces pieces,
+               int reduce, float* lse, float* tlse, float* values, float* out, float* count, void* workspace,
+               int* err, cudaStream_t s, const char* what) {
+    FL_REQUIRE(N <= INT32_MAX / pieces.count, "%s: too many rows", what);
+    int* arrived = static_cast<int*>(workspace);
+    float2* part = reinterpret_cast<float2*>(static_cast<char*>(workspace) + 256);
+    const T* xt = static_cast<const T*>(x);
+    {
+        LaunchCfg lc(dim3((unsigned)(N * pieces.count)), dim3(kFThreads), 0, s);
+        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, distill_pieces_kernel<T>, xt, V, rm, kLog2e / temp, (int)pieces.count,
+                                   pieces.rounds, part, arrived));
+        if (int st = check_launch(what)) return st;
+    }
+    LaunchCfg lc(dim3((unsigned)std::min<int64_t>((N + 7) / 8, 8ll * sm_count())), dim3(256), 0, s);
+    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, distill_rows_kernel<T>, xt, N, V, rm, te, temp, kLog2e / temp,
+                               (int)pieces.count, (const float2*)part, arrived, reduce, lse, tlse, values, out, count,
+                               err));
     return check_launch(what);
 }
 
@@ -385,13 +494,13 @@ template <typename T>
 int launch_bwd(const float* g, int scalar_g, const float* count, const void* x, int64_t N, int64_t V,
                RowMap rm, Teacher te, float temp, const float* lse, const float* tlse, void* gx,
                cudaStream_t s, const char* what) {
-    const int64_t nv = V * (int64_t)sizeof(T) / 16 + 1, chunk = 1024;
+    const int64_t nv = V * (int64_t)sizeof(T) / 16 + 1, chunk = kBVec * kDThreads;
     const int64_t nchunk = (nv + chunk - 1) / chunk;
     FL_REQUIRE(N <= INT32_MAX / nchunk, "%s: too many rows", what);
-    LaunchCfg lc(dim3((unsigned)(N * nchunk)), dim3(kDThreads), 0, s, false);
+    LaunchCfg lc(dim3((unsigned)(N * nchunk)), dim3(kDThreads), 0, s);
     FL_CUDA(cudaLaunchKernelEx(&lc.cfg, distill_bwd_kernel<T>, g, scalar_g, count, temp,
-                               static_cast<const T*>(x), V, rm, te, 1.0f / temp, lse, tlse,
-                               static_cast<T*>(gx), (int)nchunk, chunk));
+                               static_cast<const T*>(x), V, rm, te, kLog2e / temp, lse, tlse,
+                               static_cast<T*>(gx), (int)nchunk));
     return check_launch(what);
 }
 
@@ -400,12 +509,20 @@ int launch_bwd(const float* g, int scalar_g, const float* count, const void* x, 
 
 using namespace fl;
 
+extern "C" int fl_topk_distill_workspace(int64_t N, int64_t V, int dtype, int64_t* bytes) {
+    clear_error();
+    FL_REQUIRE(N >= 0 && V >= 1 && N <= INT32_MAX && V <= INT32_MAX && dtype >= 0 && dtype <= 2 && bytes,
+               "fl_topk_distill_workspace: bad arguments");
+    *bytes = distill_bytes(N, V, dtype);
+    return FL_OK;
+}
+
 extern "C" int fl_topk_distill_fwd(const void* x, int dtype, const void* teacher_logits, int teacher_dtype,
                                    const int64_t* teacher_index, int64_t N, int64_t V, int64_t K,
                                    int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
                                    float temperature, int reduce, float* lse, float* teacher_lse,
-                                   float* values, float* out, float* count, int* err_flag,
-                                   fl_stream_t stream) {
+                                   float* values, float* out, float* count, void* workspace,
+                                   int64_t workspace_bytes, int* err_flag, fl_stream_t stream) {
     clear_error();
     const char* what = "fl_topk_distill_fwd";
     if (int st = check_distill(x, dtype, teacher_logits, teacher_dtype, teacher_index, N, V, K, temperature, what))
@@ -414,25 +531,21 @@ extern "C" int fl_topk_distill_fwd(const void* x, int dtype, const void* teacher
     if (int st = distill_rows(N, V, rows_per_group, group_stride, row_stride, &rm, what)) return st;
     FL_REQUIRE(reduce >= 1 && reduce <= 3, "%s: unknown reduction %d", what, reduce);
     if (N == 0) return FL_OK;
-    FL_REQUIRE(lse && teacher_lse && values && (reduce == 1 || out) && (reduce != 3 || count), "%s: NULL buffer", what);
+    FL_REQUIRE(lse && teacher_lse && values && workspace && (reduce == 1 || out) && (reduce != 3 || count),
+               "%s: NULL buffer", what);
     FL_REQUIRE(aligned_to(lse, 4) && aligned_to(teacher_lse, 4) && aligned_to(values, 4) &&
-                   aligned_to(out, 4) && aligned_to(count, 4) && aligned_to(err_flag, 4),
+                   aligned_to(out, 4) && aligned_to(count, 4) && aligned_to(err_flag, 4) &&
+                   aligned_to(workspace, 256),
                "%s: misaligned buffer", what);
+    FL_REQUIRE(workspace_bytes >= distill_bytes(N, V, dtype), "%s: workspace of %lld bytes, %lld needed", what,
+               (long long)workspace_bytes, (long long)distill_bytes(N, V, dtype));
     if (int st = bind_device(stream, lse)) return st;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const Teacher te{teacher_logits, teacher_index, (int)K, teacher_dtype};
-    int st;
-    if (dtype == 0)
-        st = launch_fwd<float>(x, N, V, rm, te, temperature, lse, teacher_lse, values, err_flag, s, what);
-    else if (dtype == 1)
-        st = launch_fwd<__half>(x, N, V, rm, te, temperature, lse, teacher_lse, values, err_flag, s, what);
-    else
-        st = launch_fwd<__nv_bfloat16>(x, N, V, rm, te, temperature, lse, teacher_lse, values, err_flag, s, what);
-    if (st || reduce == 1) return st;
-    LaunchCfg lc(dim3(1), dim3(1024), 0, s, false);
-    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, distill_reduce_kernel, (const float*)values, (const float*)teacher_lse,
-                               N, reduce == 3, out, count));
-    return check_launch(what);
+    const Pieces pieces = row_pieces(N, V, dtype);
+    auto run = dtype == 0 ? launch_fwd<float> : dtype == 1 ? launch_fwd<__half> : launch_fwd<__nv_bfloat16>;
+    return run(x, N, V, rm, te, temperature, pieces, reduce, lse, teacher_lse, values, out, count, workspace,
+               err_flag, s, what);
 }
 
 extern "C" int fl_topk_distill_bwd(const float* grad, const void* x, int dtype, const void* teacher_logits,

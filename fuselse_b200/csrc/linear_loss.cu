@@ -85,23 +85,37 @@ struct Unit {
     int m, n, k0, k1, slab;
 };
 
-// Work unit u: K piece by K piece, tiles of a piece in groups of 8 tile rows,
+// Work unit u: K piece by K piece, tiles of a piece in groups of kGroupM tile rows,
 // so that the tiles in flight share operand rows through L2.
 constexpr int kGroupM = 8;
-__device__ __forceinline__ Unit decode_unit(int u, int mt, int nt, int splits, int kb) {
-    Unit t;
-    const int tiles = mt * nt;
-    t.slab = u / tiles;
-    const int r = u - t.slab * tiles;
-    const int group = r / (kGroupM * nt);
-    const int gm = min(kGroupM, mt - group * kGroupM);
-    const int q = r - group * kGroupM * nt;
-    t.m = group * kGroupM + q % gm;
-    t.n = q / gm;
-    t.k0 = static_cast<int>((int64_t)kb * t.slab / splits);
-    t.k1 = static_cast<int>((int64_t)kb * (t.slab + 1) / splits);
-    return t;
-}
+struct Schedule {
+    int mt, nt, splits, kb, tiles;
+    __device__ __forceinline__ Unit operator()(int u) const {
+        Unit t;
+        t.slab = 0;
+        t.k0 = 0;
+        t.k1 = kb;
+        if (splits > 1) {
+            t.slab = u / tiles;
+            u -= t.slab * tiles;
+            // kb <= 2^25 blocks and splits <= 64: the products fit 32 bits
+            t.k0 = static_cast<int>(static_cast<uint32_t>(kb) * static_cast<uint32_t>(t.slab) /
+                                    static_cast<uint32_t>(splits));
+            t.k1 = static_cast<int>(static_cast<uint32_t>(kb) * static_cast<uint32_t>(t.slab + 1) /
+                                    static_cast<uint32_t>(splits));
+        }
+        int m0 = 0, gm = mt;
+        if (mt > kGroupM) {
+            const int group = u / (kGroupM * nt);
+            m0 = group * kGroupM;
+            u -= m0 * nt;
+            gm = min(kGroupM, mt - m0);
+        }
+        t.n = u / gm;
+        t.m = m0 + u - t.n * gm;
+        return t;
+    }
+};
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -172,6 +186,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     const int nt = (args.n_extent + kTile - 1) / kTile;
     const int kb_total = max(1, (k_ext + kBlockK - 1) / kBlockK);
     const int units = mt * nt * args.splits;
+    const Schedule unit{mt, nt, args.splits, kb_total, mt * nt};
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (warp == 0) {
@@ -180,7 +195,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             uint32_t stage = 0, phase = 0;
             const uint32_t stage_tx = 2 * kOperandBytes + (args.one_half ? 1 : 2) * args.a_rows * (kBlockK * 2);
             for (int u = pair; u < units && !*stop; u += pairs) {
-                const Unit t = decode_unit(u, mt, nt, args.splits, kb_total);
+                const Unit t = unit(u);
                 const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * kTile + rank * kHalfTile;
                 for (int kb = t.k0; kb < t.k1; ++kb) {
                     if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, stop)) break;
@@ -215,7 +230,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             constexpr uint32_t step_b = Shape::kBMn ? 2048 >> 4 : 32 >> 4;
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
             for (int u = pair; u < units && !*stop; u += pairs) {
-                const Unit t = decode_unit(u, mt, nt, args.splits, kb_total);
+                const Unit t = unit(u);
                 if (t.k0 == t.k1) continue;
                 if (!mbar_wait(acc_empty0 + 8 * acc, acc_phase ^ 1, stop)) break;
                 tc_fence_after();
@@ -249,7 +264,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         if (EPI == kEpiOut16) scale = __ldg(args.inv_scale);
         uint32_t acc = 0, acc_phase = 0;
         for (int u = pair; u < units; u += pairs) {
-            const Unit t = decode_unit(u, mt, nt, args.splits, kb_total);
+            const Unit t = unit(u);
             if (t.k0 == t.k1) continue;
             const int row0 = t.m * kTile + rank * kHalfTile + q * 32, row = row0 + lane;
             const int col0 = t.n * kTile + h * kHalfTile;
@@ -272,7 +287,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             if (busy) {
                 const uint32_t base = tmem + acc * kTile + h * kHalfTile + (static_cast<uint32_t>(q * 32) << 16);
                 float m = -INFINITY, s = 0.0f;
-#pragma unroll
+                // not unrolled: the epilogue's code is fetched once per tile by every warp, and
+                // four copies of it measured X us against Y us
+#pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t r[32];
                     tmem_ld32(base + 32 * c, r);

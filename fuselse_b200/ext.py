@@ -383,6 +383,14 @@ def _teacher(teacher_logits, teacher_index):
     return teacher_logits, teacher_index
 
 
+@functools.lru_cache(maxsize=256)
+def topk_distill_workspace_bytes(N: int, V: int, dtype: torch.dtype) -> int:
+    """Bytes of the scratch that topk_distill_forward allocates."""
+    out = ctypes.c_int64()
+    call("fl_topk_distill_workspace", N, V, _DTYPE[dtype], ctypes.byref(out))
+    return out.value
+
+
 def topk_distill_forward(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
                          temperature: float = 1.0, reduce: int = 1, err_flag=None):
     """(out, saved): reduce 1 per-row losses (logits.shape[:-1]), 2 their sum, 3 their
@@ -403,11 +411,13 @@ def topk_distill_forward(logits: torch.Tensor, teacher_logits: torch.Tensor, tea
             if reduce >= 2:
                 out.fill_(float("nan") if reduce == 3 else 0.0)
         else:
+            need = topk_distill_workspace_bytes(N, V, logits.dtype)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
             at = state.data_ptr()  # lse, teacher_lse, count, values of a reduced loss
             values = out.data_ptr() if reduce == 1 else at + 4 * (2 * N + 1)
             call("fl_topk_distill_fwd", logits.data_ptr(), _DTYPE[logits.dtype], tl.data_ptr(),
                  _DTYPE[tl.dtype], ti.data_ptr(), N, V, K, rpg, gs, rs, temperature, reduce, at, at + 4 * N,
-                 values, out.data_ptr(), at + 8 * N, _addr(err_flag), _raw_stream(dev))
+                 values, out.data_ptr(), at + 8 * N, ws.data_ptr(), need, _addr(err_flag), _raw_stream(dev))
     return out, (logits, tl, ti, state)
 
 

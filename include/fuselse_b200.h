@@ -409,7 +409,9 @@ int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int64_t rows_p
  *   reduce 1: values is the result; 2, 3: out[0] = their sum, their mean over
  *   the rows that keep an entry (0 / 0 if none), *count (3) the number of those.
  * An index outside [0, V) other than -1 makes its row NaN and, when err_flag
- * is not NULL, sets *err_flag |= 1.  lse and teacher_lse (N,) are kept for
+ * is not NULL, sets *err_flag |= 1.  workspace: fl_topk_distill_workspace
+ * bytes, 256-byte aligned, contents undefined on entry, one call in flight.
+ * lse and teacher_lse (N,) are kept for
  * the backward:  gx = grad * T * (q - p), grad one float for reduce 2 and 3
  * (divided by *count for 3), (N,) for 1; gx (N, V) dense, of x's
  * dtype; zero in rows that keep nothing.  Columns named twice count twice.
@@ -419,7 +421,9 @@ int fl_topk_distill_fwd(const void* x, int dtype, const void* teacher_logits, in
                         const int64_t* teacher_index, int64_t N, int64_t V, int64_t K,
                         int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
                         float temperature, int reduce, float* lse, float* teacher_lse, float* values,
-                        float* out, float* count, int* err_flag, fl_stream_t stream);
+                        float* out, float* count, void* workspace, int64_t workspace_bytes,
+                        int* err_flag, fl_stream_t stream);
+int fl_topk_distill_workspace(int64_t N, int64_t V, int dtype, int64_t* bytes);
 int fl_topk_distill_bwd(const float* grad, const void* x, int dtype, const void* teacher_logits,
                         int teacher_dtype, const int64_t* teacher_index, int64_t N, int64_t V,
                         int64_t K, int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
