@@ -17,6 +17,7 @@
 // by tensor-map copies 64 deep in K; warp 0 copies, warp 1 issues the products,
 // warps 4-11 are the epilogue.
 #include "common.cuh"
+#include "pairs.cuh"
 #include "rows.cuh"
 #include "umma.cuh"
 
@@ -28,14 +29,12 @@ namespace fl {
 namespace {
 
 constexpr int kTile = 256;            // rows and columns of a CTA pair's tile
-constexpr int kHalfTile = 128;        // rows of A and of B staged by one CTA
+constexpr int kHalfTile = 128;        // rows of A (and of a 256-column B) staged by one CTA
 constexpr int kBlockK = 64;           // 128 bytes of a 16-bit operand
 constexpr int kGemmThreads = 384;     // 4 warps of roles, 8 epilogue warps
 constexpr int kEpiWarps = 8;
 constexpr uint32_t kOperandBytes = kHalfTile * kBlockK * 2;   // 16 KB
-constexpr uint32_t kStageBytes = 2 * kOperandBytes;
 constexpr uint32_t kStagingBuf = 4096;                        // 32 rows of 128 bytes
-constexpr uint32_t kTmemCols = 512;                           // two fp32 accumulators
 
 // What a product's epilogue does with a tile.
 enum Epi {
@@ -43,15 +42,21 @@ enum Epi {
     kEpiGradZ = 1,   // dz of the tile in 16 bits
     kEpiOut16 = 2,   // scaled, in 16 bits
     kEpiSlab = 3,    // fp32 partial sums (stored, or added to what is there)
+    kEpiFew = 4,     // as kEpiStats with the operands exchanged: few rows, vocabulary in M
 };
 
-template <int EPI>
+// NT: columns of a tile (256; fewer for kEpiFew).
+template <int EPI, int NT>
 struct GemmShape {
     static constexpr bool kAMn = EPI == kEpiOut16;                    // A given as [k][m]
     static constexpr bool kBMn = EPI == kEpiOut16 || EPI == kEpiSlab;  // B given as [k][n]
-    static constexpr int kStages = EPI == kEpiStats ? 7 : 5;
-    static constexpr uint32_t kStaging = EPI == kEpiStats ? 0 : kEpiWarps * 2 * kStagingBuf;
-    static constexpr uint32_t kSmem = kStages * kStageBytes + kStaging + 1024 + 256;
+    static constexpr bool kStores = EPI != kEpiStats && EPI != kEpiFew;
+    static constexpr uint32_t kBBytes = NT / 2 * kBlockK * 2;
+    static constexpr uint32_t kStageBytes = kOperandBytes + kBBytes;
+    static constexpr uint32_t kStaging = kStores ? kEpiWarps * 2 * kStagingBuf : 0;
+    static constexpr int kStages = (227 * 1024 - 1280 - kStaging) / kStageBytes;
+    static constexpr uint32_t kSmem = kStages * kStageBytes + kStaging + 1024;
+    static constexpr uint32_t kTmemCols = 2 * NT;  // two accumulators
 };
 
 // meta words shared by the kernels of a call
@@ -133,11 +138,60 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
                  : "memory");
 }
 
-template <int EPI, bool BF16>
+__device__ __forceinline__ float warp_max_nan(float v) {
+    float r;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// kEpiFew: 16 rows (columns of the accumulator) over the 32 vocabulary entries
+// v0.. of this warp's lanes: each row's (max, sum-exp) over the lanes.
+__device__ __forceinline__ void few_rows_piece(uint32_t addr, int row0, int v0, int rows, int vocab,
+                                               const GemmArgs& args, int piece) {
+    const int lane = threadIdx.x & 31;
+    // lane j < 16 looks up row row0 + j's target, as a lane of this piece (or none)
+    int want = -1;
+    if (lane < 16 && row0 + lane < rows) {
+        const int64_t t = __ldg(args.target + (args.src ? __ldg(args.src + row0 + lane) : row0 + lane));
+        if (t >= v0 && t < v0 + 32 && t < vocab) want = static_cast<int>(t) - v0;
+    }
+    uint32_t r[16];
+    tmem_ld16(addr, r);
+    tmem_wait_ld(r);
+    const bool here = v0 + lane < vocab;
+    const uint32_t wanted = __ballot_sync(0xffffffffu, want >= 0);
+    float e[16], top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const float z = here ? __uint_as_float(r[j]) : -INFINITY;
+        if (wanted >> j & 1) {
+            if (__shfl_sync(0xffffffffu, want, j) == lane) args.zt[row0 + j] = z;
+        }
+        const float m = warp_max_nan(z);
+        e[j] = exp_from(z, safe_max(m));
+        if ((lane >> 1) == j) top = m;
+    }
+    // sums over the lanes: each exchange halves the rows a lane carries, so lanes 2j and
+    // 2j + 1 end with row j
+#pragma unroll
+    for (int w = 8; w >= 1; w /= 2) {
+        const bool upper = lane & (2 * w);
+#pragma unroll
+        for (int j = 0; j < w; ++j) {
+            const float give = upper ? e[j] : e[j + w], keep = upper ? e[j + w] : e[j];
+            e[j] = keep + __shfl_xor_sync(0xffffffffu, give, 2 * w);
+        }
+    }
+    const float sum = e[0] + __shfl_xor_sync(0xffffffffu, e[0], 1);
+    const int row = row0 + (lane >> 1);
+    if ((lane & 1) == 0 && row < rows) args.part[(int64_t)row * args.pieces + piece] = make_float2(top, sum);
+}
+
+template <int EPI, bool BF16, int NT = kTile>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ CUtensorMap map_out, const GemmArgs args) {
-    using Shape = GemmShape<EPI>;
+    using Shape = GemmShape<EPI, NT>;
     constexpr int kStages = Shape::kStages;
     extern __shared__ uint8_t smem_raw[];
     __shared__ alignas(8) uint64_t bars[2 * kStages + 4];
@@ -163,9 +217,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         mbar_init_fence();
         tma_prefetch_map(&map_a);
         tma_prefetch_map(&map_b);
-        if (EPI != kEpiStats) tma_prefetch_map(&map_out);
+        if (Shape::kStores) tma_prefetch_map(&map_out);
     }
-    if (warp == 2) tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
+    if (warp == 2) tmem_alloc_pair(smem_u32(&tmem_slot), Shape::kTmemCols);
     pdl_wait();
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
@@ -183,24 +237,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     const int m_ext = args.m_extent < 0 ? rows : args.m_extent;
     const int k_ext = args.k_extent < 0 ? rows : args.k_extent;
     const int mt = max(1, (m_ext + kTile - 1) / kTile);
-    const int nt = (args.n_extent + kTile - 1) / kTile;
+    const int n_ext = args.n_extent < 0 ? rows : args.n_extent;
+    const int nt = EPI == kEpiFew ? 1 : (n_ext + NT - 1) / NT;
     const int kb_total = max(1, (k_ext + kBlockK - 1) / kBlockK);
     const int units = mt * nt * args.splits;
     const Schedule unit{mt, nt, args.splits, kb_total, mt * nt};
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int pair_id = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (warp == 0) {
         // ---- copies ----
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
-            const uint32_t stage_tx = 2 * kOperandBytes + (args.one_half ? 1 : 2) * args.a_rows * (kBlockK * 2);
-            for (int u = pair; u < units && !*stop; u += pairs) {
+            const uint32_t stage_tx =
+                2 * Shape::kBBytes + (args.one_half ? 1 : 2) * args.a_rows * (kBlockK * 2);
+            for (int u = pair_id; u < units && !*stop; u += pairs) {
                 const Unit t = unit(u);
-                const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * kTile + rank * kHalfTile;
+                const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * NT + rank * (NT / 2);
                 for (int kb = t.k0; kb < t.k1; ++kb) {
                     if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, stop)) break;
                     const uint32_t bar = map_to_rank(full0 + 8 * stage, 0);
-                    const uint32_t sa = smem + stage * kStageBytes, sb = sa + kOperandBytes;
+                    const uint32_t sa = smem + stage * Shape::kStageBytes, sb = sa + kOperandBytes;
                     if (rank == 0) mbar_expect_tx(full0 + 8 * stage, stage_tx);
                     const int k = kb * kBlockK;
                     if (Shape::kAMn) {
@@ -229,7 +285,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             constexpr uint32_t step_a = Shape::kAMn ? 2048 >> 4 : 32 >> 4;
             constexpr uint32_t step_b = Shape::kBMn ? 2048 >> 4 : 32 >> 4;
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-            for (int u = pair; u < units && !*stop; u += pairs) {
+            for (int u = pair_id; u < units && !*stop; u += pairs) {
                 const Unit t = unit(u);
                 if (t.k0 == t.k1) continue;
                 if (!mbar_wait(acc_empty0 + 8 * acc, acc_phase ^ 1, stop)) break;
@@ -239,11 +295,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     ok = mbar_wait(full0 + 8 * stage, phase, stop);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sa = smem + stage * kStageBytes;
+                    const uint32_t sa = smem + stage * Shape::kStageBytes;
                     const uint64_t da = umma_desc(sa, lead_a), db = umma_desc(sa + kOperandBytes, lead_b);
 #pragma unroll
                     for (int k = 0; k < kBlockK / 16; ++k)
-                        umma_pair(tmem + acc * kTile, da + k * step_a, db + k * step_b, args.idesc,
+                        umma_pair(tmem + acc * NT, da + k * step_a, db + k * step_b, args.idesc,
                                   kb != t.k0 || k != 0);
                     umma_commit_pair(empty0 + 8 * stage);
                     if (++stage == kStages) stage = 0, phase ^= 1;
@@ -257,15 +313,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     } else if (warp >= 4) {
         // ---- epilogue: warp quarter q reads lanes (rows) 32q.., half h columns 128h.. ----
         const int q = warp & 3, h = (warp - 4) >> 2;
-        const uint32_t staging = smem + kStages * kStageBytes + (warp - 4) * 2 * kStagingBuf;
+        const uint32_t staging = smem + kStages * Shape::kStageBytes + (warp - 4) * 2 * kStagingBuf;
         const uint32_t srow = lane * 128, sxor = lane & 7;
         const uint32_t empty_leader = map_to_rank(acc_empty0, 0);
         float scale = 1.0f;
         if (EPI == kEpiOut16) scale = __ldg(args.inv_scale);
         uint32_t acc = 0, acc_phase = 0;
-        for (int u = pair; u < units; u += pairs) {
+        for (int u = pair_id; u < units; u += pairs) {
             const Unit t = unit(u);
             if (t.k0 == t.k1) continue;
+            if constexpr (EPI == kEpiFew) {
+                if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * acc, acc_phase, stop))) break;
+                tc_fence_after();
+                const int v0 = t.m * kTile + rank * kHalfTile + q * 32;
+#pragma unroll 1
+                for (int c = h * (NT / 2); c < min(rows, (h + 1) * (NT / 2)); c += 16)
+                    few_rows_piece(tmem + acc * NT + c + (static_cast<uint32_t>(q * 32) << 16), c, v0, rows,
+                                   args.m_extent, args, 8 * t.m + 4 * rank + q);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(empty_leader + 8 * acc);
+                if ((acc ^= 1) == 0) acc_phase ^= 1;
+                continue;
+            }
             const int row0 = t.m * kTile + rank * kHalfTile + q * 32, row = row0 + lane;
             const int col0 = t.n * kTile + h * kHalfTile;
             // a warp whose rows are all past the end has nothing to write, except that dz is
@@ -300,7 +370,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                         float v[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-                        if (cc + 32 > args.n_extent) {
+                        if (cc + 32 > n_ext) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
                                 if (cc + j >= args.n_extent) v[j] = -INFINITY;
@@ -312,19 +382,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                                 if (tcol == 32 * c + j) z = v[j];
                             if (col0 + tcol < args.n_extent) args.zt[row] = z;
                         }
-                        ms_fold<32>(m, s, v);
+                        fold_pairs<32>(m, s, v, max_of<32>(m, v), kLog2e);
                     } else if (EPI == kEpiGradZ || EPI == kEpiOut16) {
                         float v[32];
                         if (EPI == kEpiGradZ) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = a * exp_from(__uint_as_float(r[j]), lse);
+                            for (int j = 0; j < 32; j += 2) {
+                                const float2 e = exp_pair(pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+                                                          pair(-lse, -lse), pair(kLog2e, kLog2e));
+                                const float2 o = unpair(mul2(pair(e.x, e.y), pair(a, a)));
+                                v[j] = o.x;
+                                v[j + 1] = o.y;
+                            }
                             if (here) {
 #pragma unroll
                                 for (int j = 0; j < 32; ++j)
                                     if (tcol == 32 * c + j) v[j] -= b;
                             }
                             // rows and columns past the end are zero whatever was staged there
-                            if (row >= rows || cc + 32 > args.n_extent) {
+                            if (row >= rows || cc + 32 > n_ext) {
 #pragma unroll
                                 for (int j = 0; j < 32; ++j)
                                     if (row >= rows || cc + j >= args.n_extent) v[j] = 0.0f;
@@ -405,7 +481,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         }
     }
     cluster_sync_all();  // no arrival or operand read of the other CTA is left
-    if (warp == 2) tmem_free_pair(tmem, kTmemCols);
+    if (warp == 2) tmem_free_pair(tmem, Shape::kTmemCols);
 }
 
 // ---------------------------------------------------------------------------
@@ -726,11 +802,11 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidd
 // whatever was staged there before and are never read.
 int staged_rows(int64_t rows) { return rows >= kHalfTile ? kHalfTile : (int)round_up(rows, 8); }
 
-template <int EPI>
+template <int EPI, int NT = kTile>
 int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GemmArgs& args,
                    int64_t units, bool bf16, cudaStream_t stream, const char* what) {
-    auto kern = bf16 ? product_kernel<EPI, true> : product_kernel<EPI, false>;
-    constexpr uint32_t smem = GemmShape<EPI>::kSmem;
+    auto kern = bf16 ? product_kernel<EPI, true, NT> : product_kernel<EPI, false, NT>;
+    constexpr uint32_t smem = GemmShape<EPI, NT>::kSmem;
     FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const int64_t pairs = std::max<int64_t>(1, std::min<int64_t>(units, sm_count() / 2));
     LaunchCfg lc(dim3((unsigned)(2 * pairs)), dim3(kGemmThreads), smem, stream);
@@ -740,8 +816,15 @@ int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
 
 constexpr CUtensorMapDataType kMap16[2] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16};
 
+// Up to this many rows take the exchanged product: its tiles are as narrow as the
+// rows need, so that a pass over the weights is all there is to pay.
+constexpr int64_t kFewRows = 128;
+
+// Partial states of a row: of 128 columns, or of 32 lanes of vocabulary (kEpiFew).
+int64_t row_pieces(int64_t N, int64_t V) { return (N <= kFewRows ? 8 : 2) * ((V + kTile - 1) / kTile); }
+
 int64_t fwd_bytes(int64_t N, int64_t V) {
-    return round_up(N * 2 * ((V + kTile - 1) / kTile) * 8, 256) + 2 * round_up(N * 4, 256);
+    return round_up(N * row_pieces(N, V) * 8, 256) + 2 * round_up(N * 4, 256);
 }
 
 int launch_copy_rows(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t D, int64_t Dp, int64_t ld,
@@ -900,34 +983,44 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group
         if (int st = launch_copy_rows(hidden, keep.packed, N, D, c.Dp, packed_ld(D), c.rows, s, what)) return st;
     }
     if (pack != kPackNone) h = keep.packed, ldh = packed_ld(D);
-    const int64_t tiles_n = (V + kTile - 1) / kTile;
+    const int64_t tiles_v = (V + kTile - 1) / kTile, pieces = row_pieces(N, V);
     float2* part = static_cast<float2*>(workspace);
-    float* zt = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(N * 2 * tiles_n * 8, 256));
+    float* zt = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(N * pieces * 8, 256));
     float* values = reduce < kSum ? out
                                   : reinterpret_cast<float*>(reinterpret_cast<char*>(zt) + round_up(N * 4, 256));
-    CUtensorMap a, b;
-    const int a_rows = staged_rows(N);
-    if (int st = make_tensor_map(&a, kMap16[dtype], 2, h, c.Dp, N, ldh, kBlockK, a_rows)) return st;
-    if (int st = make_tensor_map(&b, kMap16[dtype], 2, weight, c.Dp, V, ldw, kBlockK, kHalfTile)) return st;
+    const bool bf16 = dtype == 1, exchanged = N <= kFewRows;
+    const int64_t few_cols = N <= 32 ? 32 : N <= 64 ? 64 : 128;
+    CUtensorMap h_map, w_map;
+    if (int st = make_tensor_map(&h_map, kMap16[dtype], 2, h, c.Dp, N, ldh, kBlockK,
+                                 exchanged ? (int)few_cols / 2 : kHalfTile))
+        return st;
+    if (int st = make_tensor_map(&w_map, kMap16[dtype], 2, weight, c.Dp, V, ldw, kBlockK, kHalfTile)) return st;
     GemmArgs g = {};
     g.rows = (int)N;
     g.packed = pack == kPackKept;
     g.first = pack != kPackKept;
-    g.m_extent = -1;
-    g.n_extent = (int)V;
+    g.m_extent = exchanged ? (int)V : -1;
+    g.n_extent = exchanged ? -1 : (int)V;
     g.k_extent = (int)c.Dp;
     g.splits = 1;
-    g.idesc = umma_idesc(dtype == 1, false, false);
-    g.a_rows = a_rows;
-    g.one_half = N <= kHalfTile;
+    g.idesc = umma_idesc(bf16, false, false, exchanged ? (uint32_t)few_cols : kTile);
+    g.a_rows = kHalfTile;
     g.meta = keep.meta;
     g.target = target;
     g.src = keep.src;
     g.part = part;
-    g.pieces = (int)(2 * tiles_n);
+    g.pieces = (int)pieces;
     g.zt = zt;
-    if (int st = launch_product<kEpiStats>(a, b, a, g, ((N + kTile - 1) / kTile) * tiles_n, dtype == 1, s, what))
-        return st;
+    int st;
+    if (!exchanged)
+        st = launch_product<kEpiStats>(h_map, w_map, h_map, g, ((N + kTile - 1) / kTile) * tiles_v, bf16, s, what);
+    else if (few_cols == 32)
+        st = launch_product<kEpiFew, 32>(w_map, h_map, h_map, g, tiles_v, bf16, s, what);
+    else if (few_cols == 64)
+        st = launch_product<kEpiFew, 64>(w_map, h_map, h_map, g, tiles_v, bf16, s, what);
+    else
+        st = launch_product<kEpiFew, 128>(w_map, h_map, h_map, g, tiles_v, bf16, s, what);
+    if (st) return st;
     const bool few = N <= 2 * sm_count();
     auto finish = few ? finish_forward_kernel<8> : finish_forward_kernel<1>;
     LaunchCfg lc(dim3((unsigned)(few ? N : std::min<int64_t>((N + 7) / 8, 8ll * sm_count()))), dim3(256), 0, s);
