@@ -21,8 +21,8 @@ class TopkDistillation(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_index, temperature, reduce, err_flag):
-        out, saved = ext.topk_distill_forward(logits, teacher_logits, teacher_index, temperature, reduce,
-                                              err_flag)
+        out, saved = ext.topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature,
+                                                      reduce, err_flag)
         ctx.save_for_backward(*saved)
         ctx.config = temperature, reduce
         return out
@@ -58,7 +58,7 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, t
     if torch.is_grad_enabled() and logits.requires_grad:
         out = TopkDistillation.apply(logits, teacher_logits.detach(), teacher_index, temperature, reduce, err)
     else:
-        out, _ = ext.topk_distill_forward(logits, teacher_logits, teacher_index, temperature, reduce, err)
+        out, _ = ext.topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err)
     if check_index and int(err.item()):
         raise RuntimeError(f"topk_distillation_loss: index out of range for {logits.shape[-1]} classes")
     return out

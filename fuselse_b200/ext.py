@@ -197,7 +197,8 @@ def _addr(t):
 
 
 def _raw_stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    """The current stream's handle, without the Stream object around it (2 us of a call)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def check_linear_loss(what: str, hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor) -> None:
@@ -274,12 +275,19 @@ def _hidden_rows(hidden: torch.Tensor):
 
 
 def linear_loss_forward(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduce: int,
-                        ignore_index: int | None = None, z_loss: float = 0.0, err_flag=None):
+                        ignore_index: int | None = None, z_loss: float = 0.0, err_flag=None,
+                        keep: bool = True):
     """(out, saved): reduce 0 log-probabilities, 1 losses (both like target), 2 their
     sum, 3 their mean over the kept rows.  Rows whose target is `ignore_index` are
     left out (None: all rows are kept; needed by 2 and 3).  saved is what
-    linear_loss_backward takes: (hidden or None, weight rows, target, state, pack)."""
+    linear_loss_backward takes: (hidden or None, weight rows, target, state, pack); without
+    `keep` there is none (None)."""
     check_linear_loss("linear_loss_forward", hidden, weight, target)
+    return linear_loss_forward_checked(hidden, weight, target, reduce, ignore_index, z_loss, err_flag, keep)
+
+
+def linear_loss_forward_checked(hidden, weight, target, reduce, ignore_index, z_loss, err_flag, keep):
+    """linear_loss_forward of arguments that check_linear_loss has passed."""
     V, D = weight.shape
     shape, dev = target.shape, hidden.device
     with _on_device(dev):
@@ -296,12 +304,18 @@ def linear_loss_forward(hidden: torch.Tensor, weight: torch.Tensor, target: torc
                 out.fill_(float("nan") if reduce == 3 else 0.0)
             return out, (None, w, target, None, pack)
         need_state, need, _ = linear_loss_sizes(N, V, D, pack)
-        state = torch.empty(need_state, dtype=torch.uint8, device=dev)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        if keep:
+            state = torch.empty(need_state, dtype=torch.uint8, device=dev)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            at_state, at_ws = state.data_ptr(), ws.data_ptr()
+        else:  # one scratch buffer holds both (sizes are multiples of 256 bytes)
+            ws = torch.empty(need_state + need, dtype=torch.uint8, device=dev)
+            at_state = ws.data_ptr()
+            at_ws = at_state + need_state
         call("fl_linear_loss_fwd", rows.data_ptr(), rpg, gs, rs, w.data_ptr(), ldw, _DTYPE16[hidden.dtype],
              target.data_ptr(), pack, 0 if ignore_index is None else ignore_index, N, V, D, reduce, z_loss,
-             state.data_ptr(), need_state, out.data_ptr(), ws.data_ptr(), need, _addr(err_flag), stream)
-    return out, (hidden if pack == PACK_NONE else None, w, target, state, pack)
+             at_state, need_state, out.data_ptr(), at_ws, need, _addr(err_flag), stream)
+    return out, None if not keep else (hidden if pack == PACK_NONE else None, w, target, state, pack)
 
 
 def linear_loss_backward(grad_output: torch.Tensor, hidden, weight: torch.Tensor, target: torch.Tensor, state,
@@ -398,6 +412,11 @@ def topk_distill_forward(logits: torch.Tensor, teacher_logits: torch.Tensor, tea
     (row_layout must address them); saved is what topk_distill_backward takes:
     (logits, teacher_logits, teacher_index, state)."""
     check_topk_distill("topk_distill_forward", logits, teacher_logits, teacher_index, temperature)
+    return topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err_flag)
+
+
+def topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err_flag):
+    """topk_distill_forward of arguments that check_topk_distill has passed."""
     lay = row_layout(logits)
     _check(lay is not None, "logits rows cannot be addressed in place (more than two leading stride levels)")
     N, V, rpg, gs, rs = lay

@@ -29,7 +29,8 @@ class LinearLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err_flag):
-        out, saved = ext.linear_loss_forward(hidden, weight, target, reduce, ignore_index, z_loss, err_flag)
+        out, saved = ext.linear_loss_forward_checked(hidden, weight, target, reduce, ignore_index, z_loss,
+                                                     err_flag, True)
         # an operand that is used as it lies is saved as the input it is
         ctx.save_for_backward(*saved[:4])
         ctx.config = hidden.shape, reduce, z_loss, vocab_chunk, saved[4]
@@ -58,7 +59,7 @@ def _apply(what, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chu
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         out = LinearLoss.apply(hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err)
     else:
-        out, _ = ext.linear_loss_forward(hidden, weight, target, reduce, ignore_index, z_loss, err)
+        out, _ = ext.linear_loss_forward_checked(hidden, weight, target, reduce, ignore_index, z_loss, err, False)
     if check_index and int(err.item()):
         raise RuntimeError(f"{what}: index out of range for {weight.shape[0]} classes")
     return out
