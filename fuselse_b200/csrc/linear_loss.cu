@@ -95,15 +95,34 @@ struct Unit {
 // Work unit u: K piece by K piece, tiles of a piece in groups of kGroupM tile rows,
 // so that the tiles in flight share operand rows through L2.
 constexpr int kGroupM = 8;
+
+// Division by a number known for the whole kernel: the quotient from the high half of a
+// product is at most one too small.  (The divide instruction sequence took the two
+// threads that feed the tensor cores 0.4 us at every tile.)
+struct Divisor {
+    uint32_t d, inv;
+    __device__ __forceinline__ explicit Divisor(int n) : d(n), inv(0xffffffffu / static_cast<uint32_t>(n)) {}
+    __device__ __forceinline__ int operator()(int u) const {
+        uint32_t q = __umulhi(static_cast<uint32_t>(u), inv);
+        if (static_cast<uint32_t>(u) - q * d >= d) ++q;
+        return static_cast<int>(q);
+    }
+};
+
 struct Schedule {
     int mt, nt, splits, kb, tiles;
+    Divisor by_tiles, by_group, by_full, by_last;
+    __device__ __forceinline__ Schedule(int mt_, int nt_, int splits_, int kb_)
+        : mt(mt_), nt(nt_), splits(splits_), kb(kb_), tiles(mt_ * nt_), by_tiles(mt_ * nt_),
+          by_group(kGroupM * nt_), by_full(min(mt_, kGroupM)),
+          by_last(mt_ % kGroupM ? mt_ % kGroupM : kGroupM) {}
     __device__ __forceinline__ Unit operator()(int u) const {
         Unit t;
         t.slab = 0;
         t.k0 = 0;
         t.k1 = kb;
         if (splits > 1) {
-            t.slab = u / tiles;
+            t.slab = by_tiles(u);
             u -= t.slab * tiles;
             // kb <= 2^25 blocks and splits <= 64: the products fit 32 bits
             t.k0 = static_cast<int>(static_cast<uint32_t>(kb) * static_cast<uint32_t>(t.slab) /
@@ -111,15 +130,11 @@ struct Schedule {
             t.k1 = static_cast<int>(static_cast<uint32_t>(kb) * static_cast<uint32_t>(t.slab + 1) /
                                     static_cast<uint32_t>(splits));
         }
-        int m0 = 0, gm = mt;
-        if (mt > kGroupM) {
-            const int group = u / (kGroupM * nt);
-            m0 = group * kGroupM;
-            u -= m0 * nt;
-            gm = min(kGroupM, mt - m0);
-        }
-        t.n = u / gm;
-        t.m = m0 + u - t.n * gm;
+        const int m0 = by_group(u) * kGroupM;
+        u -= m0 * nt;
+        const bool last = m0 + kGroupM > mt;
+        t.n = last ? by_last(u) : by_full(u);
+        t.m = m0 + u - t.n * (last ? mt - m0 : min(mt, kGroupM));
         return t;
     }
 };
@@ -243,28 +258,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     const int nt = EPI == kEpiFew ? 1 : (n_ext + NT - 1) / NT;
     const int kb_total = max(1, (k_ext + kBlockK - 1) / kBlockK);
     const int units = mt * nt * args.splits;
-    const Schedule unit{mt, nt, args.splits, kb_total, mt * nt};
+    const Schedule unit(mt, nt, args.splits, kb_total);
     const int pair_id = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (warp == 0) {
         // ---- copies ----
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            const uint32_t stage_tx =
-                2 * Shape::kBBytes + (args.one_half ? 1 : 2) * args.a_rows * (kBlockK * 2);
-            for (int u = pair_id; u < units && !*stop; u += pairs) {
-                const Unit t = unit(u);
-                const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * NT + rank * (NT / 2);
-                for (int kb = t.k0; kb < t.k1; ++kb) {
-                    if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, stop)) break;
-                    const uint32_t bar = map_to_rank(full0 + 8 * stage, 0);
+        const bool leader = elect_one();
+        const uint32_t stage_tx = 2 * Shape::kBBytes + (args.one_half ? 1 : 2) * args.a_rows * (kBlockK * 2);
+        const uint32_t full_leader = map_to_rank(full0, 0);  // the pair counts on one barrier
+        const bool has_a = rank == 0 || !args.one_half;
+        uint32_t stage = 0, phase = 0;
+        for (int u = pair_id; u < units && !*stop; u += pairs) {
+            const Unit t = unit(u);
+            const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * NT + rank * (NT / 2);
+            for (int kb = t.k0; kb < t.k1; ++kb) {
+                if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, stop)) break;
+                if (leader) {
+                    const uint32_t bar = full_leader + 8 * stage;
                     const uint32_t sa = smem + stage * Shape::kStageBytes, sb = sa + kOperandBytes;
                     if (rank == 0) mbar_expect_tx(full0 + 8 * stage, stage_tx);
                     const int k = kb * kBlockK;
                     if (Shape::kAMn) {
                         tma_load_pair(sa, &map_a, bar, ma, k);
                         tma_load_pair(sa + kOperandBytes / 2, &map_a, bar, ma + 64, k);
-                    } else if (rank == 0 || !args.one_half) {
+                    } else if (has_a) {
                         tma_load_pair(sa, &map_a, bar, k, ma);
                     }
                     if (Shape::kBMn) {
@@ -273,19 +290,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     } else {
                         tma_load_pair(sb, &map_b, bar, k, args.b_offset + nb);
                     }
-                    if (++stage == kStages) stage = 0, phase ^= 1;
                 }
+                __syncwarp();
+                if (++stage == kStages) stage = 0, phase ^= 1;
             }
         }
-        __syncwarp();
     } else if (warp == 1) {
         // ---- products, issued by the pair's first CTA for both ----
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            const bool leader = elect_one();
             constexpr uint32_t lead_a = Shape::kAMn ? kOperandBytes / 2 : 16;
             constexpr uint32_t lead_b = Shape::kBMn ? kOperandBytes / 2 : 16;
             // 16 deep in K: 32 bytes along a K-major row, two 8-row groups of an MN-major tile
             constexpr uint32_t step_a = Shape::kAMn ? 2048 >> 4 : 32 >> 4;
             constexpr uint32_t step_b = Shape::kBMn ? 2048 >> 4 : 32 >> 4;
+            const uint64_t desc_a = umma_desc(smem, lead_a), desc_b = umma_desc(smem + kOperandBytes, lead_b);
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
             for (int u = pair_id; u < units && !*stop; u += pairs) {
                 const Unit t = unit(u);
@@ -297,21 +316,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     ok = mbar_wait(full0 + 8 * stage, phase, stop);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sa = smem + stage * Shape::kStageBytes;
-                    const uint64_t da = umma_desc(sa, lead_a), db = umma_desc(sa + kOperandBytes, lead_b);
+                    if (leader) {
+                        const uint64_t da = desc_a + stage * (Shape::kStageBytes >> 4);
+                        const uint64_t db = desc_b + stage * (Shape::kStageBytes >> 4);
+                        umma_pair(tmem + acc * NT, da, db, args.idesc, kb != t.k0);
 #pragma unroll
-                    for (int k = 0; k < kBlockK / 16; ++k)
-                        umma_pair(tmem + acc * NT, da + k * step_a, db + k * step_b, args.idesc,
-                                  kb != t.k0 || k != 0);
-                    umma_commit_pair(empty0 + 8 * stage);
+                        for (int k = 1; k < kBlockK / 16; ++k)
+                            umma_pair(tmem + acc * NT, da + k * step_a, db + k * step_b, args.idesc, true);
+                        umma_commit_pair(empty0 + 8 * stage);
+                    }
+                    __syncwarp();
                     if (++stage == kStages) stage = 0, phase ^= 1;
                 }
                 if (!ok) break;
-                umma_commit_pair(acc_full0 + 8 * acc);
+                if (leader) umma_commit_pair(acc_full0 + 8 * acc);
+                __syncwarp();
                 if ((acc ^= 1) == 0) acc_phase ^= 1;
             }
         }
-        __syncwarp();
     } else if (warp >= 4) {
         // ---- epilogue: warp quarter q reads lanes (rows) 32q.., half h columns 128h.. ----
         const int q = warp & 3, h = (warp - 4) >> 2;
@@ -325,7 +347,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             const Unit t = unit(u);
             if (t.k0 == t.k1) continue;
             if constexpr (EPI == kEpiFew) {
-                if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * acc, acc_phase, stop))) break;
+                if (!mbar_wait(acc_full0 + 8 * acc, acc_phase, stop)) break;
                 tc_fence_after();
                 const int v0 = t.m * kTile + rank * kHalfTile + q * 32;
 #pragma unroll 1
@@ -354,7 +376,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     b = __ldg(args.b + row);
                 }
             }
-            if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * acc, acc_phase, stop))) break;
+            if (!mbar_wait(acc_full0 + 8 * acc, acc_phase, stop)) break;
             tc_fence_after();
             if (busy) {
                 const uint32_t base = tmem + acc * kTile + h * kHalfTile + (static_cast<uint32_t>(q * 32) << 16);
