@@ -604,8 +604,7 @@ __global__ void __launch_bounds__(256) copy_rows16_kernel(const uint16_t* __rest
 // ---------------------------------------------------------------------------
 enum Reduce { kLogp = 0, kNone = 1, kSum = 2, kMean = 3 };
 
-// WARPS warps of a CTA share a row: one while rows are many, all eight where a few
-// rows of many pieces would leave the SMs idle.
+// WARPS warps of a CTA share a row: all eight of them above 64 pieces.
 template <int WARPS>
 __global__ void __launch_bounds__(256) finish_forward_kernel(
     const float2* __restrict__ part, int pieces, const float* __restrict__ zt,
@@ -1043,9 +1042,9 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group
     else
         st = launch_product<kEpiFew, 128>(w_map, h_map, h_map, g, tiles_v, bf16, s, what);
     if (st) return st;
-    const bool few = N <= 2 * sm_count();
-    auto finish = few ? finish_forward_kernel<8> : finish_forward_kernel<1>;
-    LaunchCfg lc(dim3((unsigned)(few ? N : std::min<int64_t>((N + 7) / 8, 8ll * sm_count()))), dim3(256), 0, s);
+    const bool wide = pieces > 64;
+    auto finish = wide ? finish_forward_kernel<8> : finish_forward_kernel<1>;
+    LaunchCfg lc(dim3((unsigned)std::min<int64_t>(wide ? N : (N + 7) / 8, 32ll * sm_count())), dim3(256), 0, s);
     FL_CUDA(cudaLaunchKernelEx(&lc.cfg, finish, (const float2*)part, g.pieces, (const float*)zt, target,
                                (const int*)keep.pos, keep.meta, N, V, z_loss, reduce, keep.lse, values, out,
                                err_flag));
