@@ -307,6 +307,7 @@ __global__ void __launch_bounds__(256) distill_rows_kernel(
 
 // dz = c (q - p), c = g T: a CTA takes one chunk of one row, writes c q, then
 // rewrites the chunk's teacher columns with every entry of theirs taken off in fp32.
+constexpr unsigned long long kNotANumber = 1ull << 63;
 template <typename T>
 __global__ void __launch_bounds__(kDThreads) distill_bwd_kernel(
     const float* __restrict__ g, int scalar_g, const float* __restrict__ count, float temp,
@@ -316,6 +317,7 @@ __global__ void __launch_bounds__(kDThreads) distill_bwd_kernel(
     constexpr int E = Elem<T>::kPerVec, U = kBVec;
     __shared__ int fix_col[kMaxTop];
     __shared__ float fix_p[kMaxTop];
+    __shared__ unsigned long long fix_sum[kMaxTop];
     __shared__ int fix_n;
     const int chunk = blockIdx.x % nchunk;
     const int64_t row = blockIdx.x / nchunk;
@@ -356,6 +358,7 @@ __global__ void __launch_bounds__(kDThreads) distill_bwd_kernel(
                     const int at = atomicAdd(&fix_n, 1);
                     fix_col[at] = static_cast<int>(col - c0);
                     fix_p[at] = ex2((t - tl) * scale);
+                    fix_sum[at] = 0;
                 }
             }
         }
@@ -388,38 +391,24 @@ __global__ void __launch_bounds__(kDThreads) distill_bwd_kernel(
     }
     __syncthreads();
     const int n = fix_n;
+    if (n == 0) return;
+    // Entries of one column are summed in integers (units of 2^-62; they sum to at most 1),
+    // so that neither their order nor the list's has a part in the result.
     for (int j = threadIdx.x; j < n; j += kDThreads) {
-        // entries of one column: the largest probability leads (ties: any, they are
-        // equal), and sums them from the largest down, an order their list has no part in
-        const int col = fix_col[j];
-        bool lead = true;
-        float sum = fix_p[j];
-        int same = 0;
-        for (int k = 0; k < n; ++k)
-            if (fix_col[k] == col && k != j) {
-                ++same;
-                if (fix_p[k] > fix_p[j] || (fix_p[k] == fix_p[j] && k < j)) lead = false;
-            }
-        if (!lead) continue;
-        if (same) {
-            float last = fix_p[j];
-            int used_at = j;
-            for (int r = 0; r < same; ++r) {
-                float best = -1.0f;
-                int at = -1;
-                for (int k = 0; k < n; ++k) {
-                    if (fix_col[k] != col || k == j) continue;
-                    const bool after = fix_p[k] < last || (fix_p[k] == last && k > used_at);
-                    if (after && (fix_p[k] > best || (fix_p[k] == best && k < at))) best = fix_p[k], at = k;
-                }
-                if (at < 0) break;  // NaN probabilities: the sum is NaN already
-                sum += best;
-                last = best;
-                used_at = at;
-            }
-        }
-        const int64_t e = c0 + col;
-        outp[e] = narrow<T>(c * (ex2((Elem<T>::load1(rowp + e) - lse) * scale) - sum));
+        int lead = 0;
+        while (fix_col[lead] != fix_col[j]) ++lead;
+        const float p = fix_p[j];
+        atomicAdd(&fix_sum[lead], p == p ? __float2ull_rn(p * 0x1p62f) : kNotANumber);
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += kDThreads) {
+        const unsigned long long sum = fix_sum[j];
+        int lead = 0;
+        while (fix_col[lead] != fix_col[j]) ++lead;
+        if (lead != j) continue;
+        const int64_t e = c0 + fix_col[j];
+        const float p = sum >= kNotANumber ? __int_as_float(0x7fc00000) : __ull2float_rn(sum) * 0x1p-62f;
+        outp[e] = narrow<T>(c * (ex2((Elem<T>::load1(rowp + e) - lse) * scale) - p));
     }
 }
 

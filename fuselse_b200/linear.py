@@ -50,11 +50,11 @@ class LinearLoss(torch.autograd.Function):
 
 
 def _apply(what, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, check_index):
-    ext.check_linear_loss(what, hidden, weight, target)
     if vocab_chunk is None:
         vocab_chunk = 0
-    elif isinstance(vocab_chunk, bool) or not isinstance(vocab_chunk, int) or vocab_chunk < 1:
+    elif isinstance(vocab_chunk, bool) or not isinstance(vocab_chunk, int) or not 1 <= vocab_chunk < 1 << 62:
         raise RuntimeError(f"{what}: vocab_chunk must be a positive int or None")
+    ext.check_linear_loss(what, hidden, weight, target)
     err = torch.zeros(1, dtype=torch.int32, device=hidden.device) if check_index else None
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         out = LinearLoss.apply(hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err)
@@ -81,8 +81,13 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     vocabulary entries at a time (None: at most 512 MB)."""
     if reduction not in _REDUCTIONS:
         raise RuntimeError(f"linear_cross_entropy: unknown reduction {reduction!r}")
+    ignore_index, z_loss = int(ignore_index), float(z_loss)
+    if not -1 << 63 <= ignore_index < 1 << 63:
+        raise RuntimeError("linear_cross_entropy: ignore_index must fit 64 bits")
+    if not abs(z_loss) <= 1e30:
+        raise RuntimeError("linear_cross_entropy: z_loss must be finite")
     return _apply("linear_cross_entropy", hidden, weight, target, _REDUCTIONS[reduction],
-                  int(ignore_index), float(z_loss), vocab_chunk, check_index)
+                  ignore_index, z_loss, vocab_chunk, check_index)
 
 
 def linear_selective_log_softmax(hidden: torch.Tensor, weight: torch.Tensor, index: torch.Tensor, *,

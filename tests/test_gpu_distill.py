@@ -135,6 +135,31 @@ def test_columns_named_twice(dtype):
     assert torch.equal(a[1], b[1])
 
 
+def test_all_entries_in_one_column():
+    """The most entries there are, all naming one column, beside rows that spread them."""
+    z, t, index = make(5, 3000, 1024, torch.float32, pad=0.0)
+    index[0] = 1234
+    index[1] = torch.arange(1024, device="cuda") % 3
+    coef = torch.ones(5, dtype=F64, device="cuda")
+    value, verr, grad, gerr, _ = reference(z, t, index, 1.3, coef, torch.float32)
+    loss, got = run(z, t, index, 1.3, "none", torch.ones(5, device="cuda"))
+    close(loss, value, verr, "loss")
+    close(got, grad, gerr, "gradient")
+    assert torch.equal(got, run(z, t, index, 1.3, "none", torch.ones(5, device="cuda"))[1])
+
+
+def test_nan_and_inf_teachers():
+    z, t, index = make(4, 300, 6, torch.float32, pad=0.0)
+    t[1, 2] = float("nan")  # this row is padding only (make): what its logits hold is not read
+    t[2, 3] = float("inf")
+    t[3, 1] = float("nan")
+    loss, g = run(z, t, index, 1.0, "none", torch.ones(4, device="cuda"))
+    assert loss[1] == 0 and (g[1] == 0).all()
+    assert loss[2].isnan() and loss[3].isnan()
+    assert g[2, index[2, 3]].isnan() and g[3, index[3, 1]].isnan()
+    assert torch.isfinite(loss[0]) and torch.isfinite(g[0]).all()
+
+
 def test_rows_that_keep_nothing():
     z, t, index = make(6, 500, 8, torch.float32, pad=0.0)
     z[1] = float("nan")

@@ -1,0 +1,205 @@
+"""Argument checks of the vocabulary losses, without a GPU: what is refused, with
+RuntimeError, before anything runs; and the C entry points' own checks."""
+
+import pytest
+import torch
+
+import fuselse_b200
+from fuselse_b200 import _lib, ext, linear_cross_entropy, linear_selective_log_softmax, topk_distillation_loss
+
+BF16 = torch.bfloat16
+
+
+def operands(n=4, d=8, v=10, dtype=BF16):
+    return torch.zeros(n, d, dtype=dtype), torch.zeros(v, d, dtype=dtype), torch.zeros(n, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("fn", [linear_cross_entropy, linear_selective_log_softmax])
+@pytest.mark.parametrize("change,message", [
+    (lambda h, w, t: (h.float(), w.float(), t), "fp16 or both bf16"),
+    (lambda h, w, t: (h, w.half(), t), "fp16 or both bf16"),
+    (lambda h, w, t: (h, w.float(), t), "fp16 or both bf16"),
+    (lambda h, w, t: (h, w, t.float()), "int64 or int32"),
+    (lambda h, w, t: (h, w, t.bool()), "int64 or int32"),
+    (lambda h, w, t: (h, w[0], t), "weight (V, D) expected"),
+    (lambda h, w, t: (h, w[:, :4], t), "8 columns, weight 4"),
+    (lambda h, w, t: (h, w[:0], t), "weight is empty"),
+    (lambda h, w, t: (h[:, :0], w[:, :0], t), "weight is empty"),
+    (lambda h, w, t: (h, w, t[:3]), r"targets of shape \(4,\)"),
+    (lambda h, w, t: (h, w, t[:, None]), r"targets of shape \(4,\)"),
+    (lambda h, w, t: (h.tolist(), w, t), "must be a tensor"),
+    (lambda h, w, t: (h, w, t), "must be CUDA"),
+])
+def test_linear_losses_refuse(fn, change, message):
+    message = message.replace("(V, D)", r"\(V, D\)")
+    with pytest.raises(RuntimeError, match=message):
+        fn(*change(*operands()))
+
+
+def test_options_refused():
+    h, w, t = operands()
+    with pytest.raises(RuntimeError, match="unknown reduction"):
+        linear_cross_entropy(h, w, t, reduction="batchmean")
+    with pytest.raises(RuntimeError, match="unknown reduction"):
+        topk_distillation_loss(torch.zeros(3, 5), torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int64),
+                               reduction="batchmean")
+    with pytest.raises(RuntimeError, match="ignore_index"):
+        linear_cross_entropy(h, w, t, ignore_index=1 << 63)
+    with pytest.raises(RuntimeError, match="z_loss"):
+        linear_cross_entropy(h, w, t, z_loss=float("inf"))
+
+
+@pytest.mark.parametrize("chunk", [0, -256, 1.5, True])
+def test_vocab_chunk_refused(chunk):
+    h, w, t = operands()
+    with pytest.raises(RuntimeError, match="vocab_chunk"):
+        linear_cross_entropy(h, w, t, vocab_chunk=chunk)
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(logits=torch.zeros(3, 5, dtype=torch.float64)), "fp32, fp16 or bf16"),
+    (dict(teacher_logits=torch.zeros(3, 2, dtype=torch.int64)), "fp32, fp16 or bf16"),
+    (dict(teacher_index=torch.zeros(3, 2)), "int64 or int32"),
+    (dict(logits=torch.zeros(3, 0)), r"logits \(..., V\) expected"),
+    (dict(teacher_index=torch.zeros(3, 1, dtype=torch.int64)), "one shape"),
+    (dict(logits=torch.zeros(4, 5)), r"\(4,\) \+ \(K,\) expected"),
+    (dict(logits=torch.zeros(3, 1, 5)), r"expected"),
+    (dict(teacher_logits=torch.zeros(3, 0), teacher_index=torch.zeros(3, 0, dtype=torch.int64)), "1 to 1024"),
+    (dict(teacher_logits=torch.zeros(3, 1025), teacher_index=torch.zeros(3, 1025, dtype=torch.int64)), "1 to 1024"),
+    (dict(temperature=0.0), "temperature"),
+    (dict(temperature=-1.0), "temperature"),
+    (dict(temperature=float("nan")), "temperature"),
+    (dict(temperature=float("inf")), "temperature"),
+    (dict(teacher_logits=[1.0]), "must be a tensor"),
+    (dict(), "must be CUDA"),
+])
+def test_distillation_refuses(kw, message):
+    args = dict(logits=torch.zeros(3, 5), teacher_logits=torch.zeros(3, 2),
+                teacher_index=torch.zeros(3, 2, dtype=torch.int64))
+    args.update(kw)
+    temperature = args.pop("temperature", 1.0)
+    with pytest.raises(RuntimeError, match=message):
+        topk_distillation_loss(args["logits"], args["teacher_logits"], args["teacher_index"],
+                               temperature=temperature)
+
+
+def _status(name, *args):
+    L = _lib.lib()
+    return getattr(L, name)(*args), L.fl_last_error().decode()
+
+
+def _fwd(**kw):
+    a = dict(hidden=4096, rpg=-1, gs=0, rs=0, weight=8192, ldw=64, dtype=1, target=16384, pack=0, ignore=-100,
+             N=4, V=100, D=64, reduce=0, z=0.0, state=32768, state_bytes=1 << 20, out=65536, ws=131072,
+             ws_bytes=1 << 24, err=None, stream=None)
+    a.update(kw)
+    return _status("fl_linear_loss_fwd", *a.values())
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(N=-1), "bad shape"), (dict(V=0), "bad shape"), (dict(D=0), "bad shape"),
+    (dict(dtype=2), "dtype"), (dict(pack=3), "packing"), (dict(reduce=4), "reduction"),
+    (dict(reduce=3), "needs packing 2"), (dict(N=1 << 31), "too large"), (dict(D=1 << 21, ldw=1 << 21), "too large"),
+    (dict(N=1 << 30, V=1 << 30), "too large"),
+    (dict(ldw=60), "weight rows"), (dict(ldw=68), "weight rows"), (dict(weight=8200), "weight rows"),
+    (dict(D=60), "unpacked hidden"), (dict(rpg=4, rs=60), "unpacked hidden"), (dict(rpg=2, rs=64), "unpacked hidden"),
+    (dict(hidden=4104), "unpacked hidden"), (dict(rpg=0), "row layout"), (dict(rpg=4, rs=-64), "row layout"),
+    (dict(target=None), "NULL"), (dict(weight=None), "NULL"), (dict(hidden=None), "NULL"), (dict(out=None), "NULL"),
+    (dict(state=None), "NULL"), (dict(ws=None), "NULL"), (dict(target=16388), "misaligned"),
+    (dict(state=32776), "misaligned"), (dict(ws=131080), "misaligned"), (dict(err=65537), "misaligned"),
+    (dict(state_bytes=256), "state of 256 bytes"), (dict(ws_bytes=0), "workspace of 0 bytes"),
+])
+def test_forward_entry_checks(kw, message):
+    status, text = _fwd(**kw)
+    assert status == _lib.FL_ERR_INVALID_ARGUMENT and message in text, text
+
+
+def test_empty_calls_are_no_ops():
+    assert _fwd(N=0)[0] == _lib.FL_OK
+    assert _fwd(N=0, hidden=None, weight=None, target=None, state=None, out=None, ws=None)[0] == _lib.FL_OK
+
+
+def _bwd(**kw):
+    a = dict(grad=2048, hidden=4096, rpg=-1, gs=0, rs=0, weight=8192, ldw=64, dtype=1, target=16384, pack=0,
+             N=4, V=100, D=64, reduce=0, z=0.0, chunk=0, state=32768, state_bytes=1 << 20, gh=65536, gw=131072,
+             ws=262144, ws_bytes=1 << 30, stream=None)
+    a.update(kw)
+    return _status("fl_linear_loss_bwd", *a.values())
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(N=-1), "bad shape"), (dict(dtype=-1), "dtype"), (dict(reduce=2), "needs packing 2"),
+    (dict(chunk=-1), "vocab_chunk"), (dict(grad=None), "NULL"), (dict(ws=None), "NULL"), (dict(hidden=None), "NULL"),
+    (dict(gw=131080), "misaligned"), (dict(gh=65540), "misaligned"), (dict(grad=2050), "misaligned"),
+    (dict(ws=262152), "misaligned"),
+])
+def test_backward_entry_checks(kw, message):
+    status, text = _bwd(**kw)
+    assert status == _lib.FL_ERR_INVALID_ARGUMENT and message in text, text
+    assert _bwd(gh=None, gw=None)[0] == _lib.FL_OK  # nothing wanted
+
+
+def test_sizes():
+    state, fwd, bwd = ext.linear_loss_sizes(1000, 5000, 100, ext.PACK_KEPT, 0, True)
+    # meta; lse, src and pos; packed rows of 128 elements
+    r = lambda v: (v + 255) // 256 * 256
+    assert state == 256 + 3 * r(4000) + r(1000 * 128 * 2)
+    assert ext.linear_loss_sizes(1000, 5000, 100, ext.PACK_NONE, 0, True)[0] == 256 + r(4000)
+    assert fwd >= 1000 * 2 * 20 * 8 and bwd >= 1000 * 5120 * 2
+    # a piece bounds the backward's scratch, whatever the vocabulary
+    small = ext.linear_loss_sizes(1000, 1 << 20, 100, ext.PACK_KEPT, 512, False)[2]
+    assert small <= 1000 * 512 * 2 + 3 * r(8000)
+    for bad in ((-1, 10, 10), (10, 0, 10), (10, 10, 0)):
+        with pytest.raises(_lib.FuseLSEError):
+            ext.linear_loss_sizes(*bad)
+    with pytest.raises(_lib.FuseLSEError, match="bad arguments"):
+        ext.linear_loss_sizes(10, 10, 10, ext.PACK_KEPT, -1)
+
+
+def _dfwd(**kw):
+    a = dict(x=4096, dtype=0, tl=8192, td=0, ti=16384, N=2, V=100, K=4, rpg=-1, gs=0, rs=0, T=1.0, reduce=3,
+             lse=32768, tlse=33792, values=34816, out=35840, count=36864, ws=65536, ws_bytes=1 << 20, err=None,
+             stream=None)
+    a.update(kw)
+    return _status("fl_topk_distill_fwd", *a.values())
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(N=-1), "bad shape"), (dict(V=0), "bad shape"), (dict(K=0), "bad shape"), (dict(K=1025), "at most 1024"),
+    (dict(V=1 << 31), "too large"), (dict(dtype=3), "dtype"), (dict(td=-1), "dtype"), (dict(T=0.0), "temperature"),
+    (dict(T=float("nan")), "temperature"), (dict(reduce=0), "reduction"), (dict(x=None), "NULL"),
+    (dict(ti=None), "NULL"), (dict(out=None), "NULL"), (dict(count=None), "NULL"), (dict(ws=None), "NULL"),
+    (dict(x=4098), "misaligned"), (dict(ti=16388), "misaligned"), (dict(ws=65544), "misaligned"),
+    (dict(rpg=0), "row layout"), (dict(ws_bytes=256), "workspace of 256 bytes"),
+])
+def test_distill_entry_checks(kw, message):
+    status, text = _dfwd(**kw)
+    assert status == _lib.FL_ERR_INVALID_ARGUMENT and message in text, text
+
+
+def test_distill_backward_entry_checks():
+    def bwd(**kw):
+        a = dict(grad=2048, x=4096, dtype=0, tl=8192, td=0, ti=16384, N=2, V=100, K=4, rpg=-1, gs=0, rs=0, T=1.0,
+                 reduce=3, lse=32768, tlse=33792, count=36864, gx=65536, stream=None)
+        a.update(kw)
+        return _status("fl_topk_distill_bwd", *a.values())
+
+    for kw, message in ((dict(K=2000), "at most"), (dict(grad=None), "NULL"), (dict(count=None), "NULL"),
+                        (dict(gx=65538), "misaligned"), (dict(T=-1.0), "temperature")):
+        status, text = bwd(**kw)
+        assert status == _lib.FL_ERR_INVALID_ARGUMENT and message in text, text
+    assert bwd(N=0)[0] == _lib.FL_OK
+
+
+def test_copy_rows_entry_checks():
+    ok = (4096, 8192, 0, 8, 8, -1, 0, 0, None)
+    assert _status("fl_copy_rows16", *ok)[0] == _lib.FL_OK
+    for args in ((4096, 8192, -1, 8, 8, -1, 0, 0, None), (4096, 8192, 2, 0, 8, -1, 0, 0, None),
+                 (None, 8192, 2, 8, 8, -1, 0, 0, None), (4097, 8192, 2, 8, 8, -1, 0, 0, None),
+                 (4096, 8192, 2, 8, 8, 0, 0, 0, None)):
+        assert _status("fl_copy_rows16", *args)[0] == _lib.FL_ERR_INVALID_ARGUMENT
+
+
+def test_exported_names():
+    for name in ("linear_cross_entropy", "linear_selective_log_softmax", "topk_distillation_loss"):
+        assert name in fuselse_b200.__all__ and callable(getattr(fuselse_b200, name))
