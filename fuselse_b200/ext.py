@@ -319,21 +319,22 @@ def linear_loss_forward_checked(hidden, weight, target, reduce, ignore_index, z_
 
 
 def linear_loss_backward(grad_output: torch.Tensor, hidden, weight: torch.Tensor, target: torch.Tensor, state,
-                         pack: int, hidden_cols: int, reduce: int, z_loss: float = 0.0, vocab_chunk: int = 0,
+                         pack: int, shape, reduce: int, z_loss: float = 0.0, vocab_chunk: int = 0,
                          want_hidden: bool = True, want_weight: bool = True):
-    """(grad_hidden (N, hidden_cols), grad_weight (V, hidden_cols)) of linear_loss_forward,
-    None where not wanted; hidden to pack as its `saved` gives them."""
+    """(grad_hidden, grad_weight) of linear_loss_forward, None where not wanted; hidden to
+    pack as its `saved` gives them, shape that of its hidden states."""
     if not (want_hidden or want_weight):
         return None, None
-    V, Dp = weight.shape[0], (hidden_cols + 7) // 8 * 8
-    N, D, dev, dtype = target.numel(), hidden_cols, weight.device, weight.dtype
+    D = shape[-1]
+    V, Dp = weight.shape[0], (D + 7) // 8 * 8
+    N, dev, dtype = target.numel(), weight.device, weight.dtype
     with _on_device(dev):
         stream = _raw_stream(dev)
         g = grad_output
         if g.dtype != torch.float32 or not g.is_contiguous():
             g = g.to(torch.float32).contiguous()
         _check(g.numel() == (1 if reduce >= 2 else N), "grad_output does not match the forward's output")
-        grad_hidden = torch.empty((N, D), dtype=dtype, device=dev) if want_hidden else None
+        grad_hidden = torch.empty(shape, dtype=dtype, device=dev) if want_hidden else None
         grad_weight = torch.empty((V, Dp), dtype=dtype, device=dev) if want_weight else None
         if N:
             rpg, gs, rs = row_layout(hidden)[2:] if hidden is not None else (-1, 0, 0)

@@ -42,10 +42,8 @@ class LinearLoss(torch.autograd.Function):
         shape, reduce, z_loss, vocab_chunk, pack = ctx.config
         want_hidden, want_weight = ctx.needs_input_grad[:2]
         grad_hidden, grad_weight = ext.linear_loss_backward(
-            grad_output, *ctx.saved_tensors, pack, shape[-1], reduce, z_loss, vocab_chunk, want_hidden,
+            grad_output, *ctx.saved_tensors, pack, shape, reduce, z_loss, vocab_chunk, want_hidden,
             want_weight)
-        if grad_hidden is not None:
-            grad_hidden = grad_hidden.view(shape)
         return grad_hidden, grad_weight, None, None, None, None, None, None
 
 
