@@ -36,9 +36,19 @@ int make_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, 
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * elem_bytes};
     const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
     const cuuint32_t one[2] = {1, 1};
-    const CUresult r = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, one,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto attempt = [&] {
+        return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, one,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = attempt();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+        // a host thread that has made no runtime call yet has a device but no context
+        int dev = 0;
+        FL_CUDA(cudaGetDevice(&dev));
+        FL_CUDA(cudaSetDevice(dev));
+        r = attempt();
+    }
     if (r != CUDA_SUCCESS) {
         set_error("tensor map of (%lld, %lld), row stride %lld, refused (driver error %d)",
                   (long long)outer, (long long)inner, (long long)ld, (int)r);

@@ -328,6 +328,28 @@ def test_two_streams_at_once():
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_fresh_host_threads():
+    """Host threads whose first CUDA call is one of these, forward and backward."""
+    import threading
+    from fuselse_b200 import ext
+    h, w, t, up = make(130, 64, 500, BF16)
+    want = _logp_case(h, w, t, up)
+    got = {}
+
+    def forward():
+        got["out"], got["saved"] = ext.linear_loss_forward(h, w, t, 0)
+
+    def backward():
+        got["grads"] = ext.linear_loss_backward(up, *got["saved"], h.shape, 0)
+
+    for f in (forward, backward):
+        worker = threading.Thread(target=f)
+        worker.start()
+        worker.join()
+    assert torch.equal(got["out"], want[0])
+    assert torch.equal(got["grads"][0], want[1]) and torch.equal(got["grads"][1], want[2])
+
+
 def test_captured_step_replays_on_new_data():
     h, w, t, _ = make(300, 128, 1500, BF16, seed=1)
     h2, w2, t2, _ = make(300, 128, 1500, BF16, seed=2)
