@@ -36,6 +36,9 @@ constexpr int kEpiWarps = 8;
 constexpr uint32_t kOperandBytes = kHalfTile * kBlockK * 2;   // 16 KB
 constexpr uint32_t kStagingBuf = 4096;                        // 32 rows of 128 bytes
 
+// What a row's values become (fl_linear_loss_fwd's `reduce`).
+enum Reduce { kLogp = 0, kNone = 1, kSum = 2, kMean = 3 };
+
 // What a product's epilogue does with a tile.
 enum Epi {
     kEpiStats = 0,   // (max, sum-exp) of each row's 128-column pieces, target logits
@@ -83,7 +86,11 @@ struct GemmArgs {
     float2* part;          // [row][pieces] partial states
     int pieces;
     float* zt;
-    const float *lse, *a, *b, *inv_scale;
+    const float *lse, *a, *b;  // kEpiGradZ; without a and b (bf16) they are formed from
+    const float* grad;         // the upstream gradient
+    int reduce;
+    float z_loss;
+    const float* inv_scale;    // kEpiOut16 (none: 1)
     void* out;             // kEpiOut16: filled with NaN when a wait ran out
     int64_t out_elems;
 };
@@ -153,6 +160,15 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
                                              uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
+}
+
+// d value / d z = a softmax - b onehot of packed row `row`.
+__device__ __forceinline__ void row_coefficients(const float* grad, int reduce, float z_loss, float lse,
+                                                 const int* src, int64_t row, int64_t rows, float& a, float& b) {
+    b = reduce >= kSum ? __ldg(grad) : __ldg(grad + (src ? __ldg(src + row) : row));
+    if (reduce == kMean) b /= static_cast<float>(rows);
+    if (reduce == kLogp) b = -b;
+    a = z_loss != 0.0f ? b * (1.0f + 2.0f * z_loss * lse) : b;
 }
 
 __device__ __forceinline__ float warp_max_nan(float v) {
@@ -341,7 +357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         const uint32_t srow = lane * 128, sxor = lane & 7;
         const uint32_t empty_leader = map_to_rank(acc_empty0, 0);
         float scale = 1.0f;
-        if (EPI == kEpiOut16) scale = __ldg(args.inv_scale);
+        if (EPI == kEpiOut16 && args.inv_scale) scale = __ldg(args.inv_scale);
         uint32_t acc = 0, acc_phase = 0;
         for (int u = pair_id; u < units; u += pairs) {
             const Unit t = unit(u);
@@ -372,8 +388,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 tcol = tcol < 0 ? -1 : tcol - (EPI == kEpiGradZ ? args.b_offset : 0) - col0;
                 if (EPI == kEpiGradZ) {
                     lse = __ldg(args.lse + row);
-                    a = __ldg(args.a + row);
-                    b = __ldg(args.b + row);
+                    if (args.a) {
+                        a = __ldg(args.a + row);
+                        b = __ldg(args.b + row);
+                    } else {
+                        row_coefficients(args.grad, args.reduce, args.z_loss, lse, args.src, row, rows, a, b);
+                    }
                 }
             }
             if (!mbar_wait(acc_full0 + 8 * acc, acc_phase, stop)) break;
@@ -602,8 +622,6 @@ __global__ void __launch_bounds__(256) copy_rows16_kernel(const uint16_t* __rest
 // ---------------------------------------------------------------------------
 // Forward: merge a row's pieces, form its value, reduce
 // ---------------------------------------------------------------------------
-enum Reduce { kLogp = 0, kNone = 1, kSum = 2, kMean = 3 };
-
 // WARPS warps of a CTA share a row: all eight of them above 64 pieces.
 template <int WARPS>
 __global__ void __launch_bounds__(256) finish_forward_kernel(
@@ -691,9 +709,10 @@ __global__ void __launch_bounds__(256) finish_forward_kernel(
 // ---------------------------------------------------------------------------
 // Backward: row coefficients of dz, and the hidden gradient from its slabs
 // ---------------------------------------------------------------------------
-// dz = a softmax - b onehot, scaled by a power of two that brings the largest
-// coefficient to [2^13, 2^14): fp16 keeps its relative accuracy down to
-// probabilities of 1e-9 of it instead of flushing them.
+// fp16 only: the coefficients of dz = a softmax - b onehot, scaled by a power of two
+// that brings the largest to [2^13, 2^14): fp16 keeps its relative accuracy down to
+// probabilities of 1e-9 of it instead of flushing them.  bf16 has fp32's range and
+// forms its coefficients where it uses them.
 __global__ void __launch_bounds__(1024) coefficients_kernel(
     const float* __restrict__ g, int reduce, float z_loss, const float* __restrict__ lse,
     const int* __restrict__ src, const int* __restrict__ meta, int64_t N, float* __restrict__ a,
@@ -702,13 +721,8 @@ __global__ void __launch_bounds__(1024) coefficients_kernel(
     pdl_launch_dependents();
     __shared__ float top[32];
     const int64_t rows = src ? meta[kMetaRows] : N;
-    float g0 = 0.0f;
-    if (reduce == kSum) g0 = *g;
-    if (reduce == kMean) g0 = *g / static_cast<float>(rows);
     auto coef = [&](int64_t r, float& ca, float& cb) {
-        cb = reduce >= kSum ? g0 : __ldg(g + (src ? src[r] : r));
-        if (reduce == kLogp) cb = -cb;
-        ca = z_loss != 0.0f ? cb * (1.0f + 2.0f * z_loss * lse[r]) : cb;
+        row_coefficients(g, reduce, z_loss, lse[r], src, r, rows, ca, cb);
     };
     float big = 0.0f;
     for (int64_t r = threadIdx.x; r < rows; r += 1024) {
@@ -745,7 +759,7 @@ __global__ void __launch_bounds__(256) finish_hidden_kernel(const float* __restr
     pdl_launch_dependents();
     const int64_t row = blockIdx.x;
     const int64_t p = pos ? pos[row] : row;
-    const float scale = meta[kMetaStop] ? __int_as_float(0x7fc00000) : *inv_scale;
+    const float scale = meta[kMetaStop] ? __int_as_float(0x7fc00000) : inv_scale ? *inv_scale : 1.0f;
     uint16_t* o = out + row * D;
     const float* s = slabs + p * ld;
     const bool wide = D % 4 == 0;
@@ -1092,11 +1106,13 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     float* slabs = reinterpret_cast<float*>(ws + plan.slab_off);
     uint16_t* dz = reinterpret_cast<uint16_t*>(ws + plan.dz_off);
     const bool bf16 = dtype == 1;
-    {
+    if (!bf16) {
         LaunchCfg lc(dim3(1), dim3(1024), 0, s);
         FL_CUDA(cudaLaunchKernelEx(&lc.cfg, coefficients_kernel, grad, reduce, z_loss, (const float*)keep.lse,
                                    (const int*)keep.src, (const int*)keep.meta, N, ca, cb, inv_scale));
         if (int st = check_launch(what)) return st;
+    } else {
+        inv_scale = ca = cb = nullptr;
     }
     // operand and output views: hidden and weight by rows and by columns, dz both ways
     CUtensorMap h_k, w_k, dz_out, dz_mn, h_mn, dw_out, dz_k, w_mn, slab_out;
@@ -1138,6 +1154,9 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
         g.lse = keep.lse;
         g.a = ca;
         g.b = cb;
+        g.grad = grad;
+        g.reduce = reduce;
+        g.z_loss = z_loss;
         if (int st = launch_product<kEpiGradZ>(h_k, w_k, dz_out, g, mt * ct, bf16, s, what)) return st;
         if (grad_weight) {
             g = base;
