@@ -359,6 +359,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         float scale = 1.0f;
         if (EPI == kEpiOut16 && args.inv_scale) scale = __ldg(args.inv_scale);
         uint32_t acc = 0, acc_phase = 0;
+        // This warp has read its part of the accumulator.
+        auto release = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty_leader + 8 * acc);
+            if ((acc ^= 1) == 0) acc_phase ^= 1;
+        };
         for (int u = pair_id; u < units; u += pairs) {
             const Unit t = unit(u);
             if (t.k0 == t.k1) continue;
@@ -370,10 +377,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 for (int c = h * (NT / 2); c < min(rows, (h + 1) * (NT / 2)); c += 16)
                     few_rows_piece(tmem + acc * NT + c + (static_cast<uint32_t>(q * 32) << 16), c, v0, rows,
                                    args.m_extent, args, 8 * t.m + 4 * rank + q);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(empty_leader + 8 * acc);
-                if ((acc ^= 1) == 0) acc_phase ^= 1;
+                release();
                 continue;
             }
             const int row0 = t.m * kTile + rank * kHalfTile + q * 32, row = row0 + lane;
@@ -408,6 +412,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     uint32_t r[32];
                     tmem_ld32(base + 32 * c, r);
                     tmem_wait_ld(r);
+                    if (c == 3) release();  // all is read: the next tile may have the accumulator
                     const int cc = col0 + 32 * c;
                     const bool here = tcol >= 32 * c && tcol < 32 * c + 32;  // the target's column
                     if (EPI == kEpiStats) {
@@ -499,10 +504,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 if (EPI == kEpiStats && row < rows)
                     args.part[(int64_t)row * args.pieces + 2 * t.n + h] = make_float2(m, s);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(empty_leader + 8 * acc);
-            if ((acc ^= 1) == 0) acc_phase ^= 1;
+            if (!busy) release();
         }
         if (EPI != kEpiStats && lane == 0) tma_store_wait_all();
         __syncwarp();

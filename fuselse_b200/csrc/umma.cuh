@@ -47,10 +47,11 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
                  : "memory");
 }
 
-// Arrival on a barrier of any CTA of the cluster (address from map_to_rank).
+// Arrival on a barrier of any CTA of the cluster (address from map_to_rank).  It orders
+// this CTA's accesses only (the default scope): a release at cluster scope waits for every
+// global store of the warp, 2000 cycles at each tile.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
-                 : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
