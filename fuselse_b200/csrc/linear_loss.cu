@@ -275,6 +275,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     const int kb_total = max(1, (k_ext + kBlockK - 1) / kBlockK);
     const int units = mt * nt * args.splits;
     const Schedule unit(mt, nt, args.splits, kb_total);
+    // a last column of tiles with at most 128 columns left is done 128 wide (MN-major B:
+    // 64 columns staged by each CTA)
+    auto narrow = [&](const Unit& t) { return Shape::kBMn && n_ext - t.n * NT <= NT / 2; };
     const int pair_id = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (warp == 0) {
@@ -286,13 +289,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         uint32_t stage = 0, phase = 0;
         for (int u = pair_id; u < units && !*stop; u += pairs) {
             const Unit t = unit(u);
-            const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * NT + rank * (NT / 2);
+            const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * NT + rank * (narrow(t) ? NT / 4 : NT / 2);
             for (int kb = t.k0; kb < t.k1; ++kb) {
                 if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, stop)) break;
                 if (leader) {
                     const uint32_t bar = full_leader + 8 * stage;
                     const uint32_t sa = smem + stage * Shape::kStageBytes, sb = sa + kOperandBytes;
-                    if (rank == 0) mbar_expect_tx(full0 + 8 * stage, stage_tx);
+                    if (rank == 0)
+                        mbar_expect_tx(full0 + 8 * stage, narrow(t) ? stage_tx - Shape::kBBytes : stage_tx);
                     const int k = kb * kBlockK;
                     if (Shape::kAMn) {
                         tma_load_pair(sa, &map_a, bar, ma, k);
@@ -302,7 +306,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     }
                     if (Shape::kBMn) {
                         tma_load_pair(sb, &map_b, bar, nb, args.b_offset + k);
-                        tma_load_pair(sb + kOperandBytes / 2, &map_b, bar, nb + 64, args.b_offset + k);
+                        if (!narrow(t))
+                            tma_load_pair(sb + kOperandBytes / 2, &map_b, bar, nb + 64, args.b_offset + k);
                     } else {
                         tma_load_pair(sb, &map_b, bar, k, args.b_offset + nb);
                     }
@@ -325,6 +330,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             for (int u = pair_id; u < units && !*stop; u += pairs) {
                 const Unit t = unit(u);
                 if (t.k0 == t.k1) continue;
+                const uint32_t idesc = narrow(t) ? args.idesc - ((NT / 2 >> 3) << 17) : args.idesc;
                 if (!mbar_wait(acc_empty0 + 8 * acc, acc_phase ^ 1, stop)) break;
                 tc_fence_after();
                 bool ok = true;
@@ -335,10 +341,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     if (leader) {
                         const uint64_t da = desc_a + stage * (Shape::kStageBytes >> 4);
                         const uint64_t db = desc_b + stage * (Shape::kStageBytes >> 4);
-                        umma_pair(tmem + acc * NT, da, db, args.idesc, kb != t.k0);
+                        umma_pair(tmem + acc * NT, da, db, idesc, kb != t.k0);
 #pragma unroll
                         for (int k = 1; k < kBlockK / 16; ++k)
-                            umma_pair(tmem + acc * NT, da + k * step_a, db + k * step_b, args.idesc, true);
+                            umma_pair(tmem + acc * NT, da + k * step_a, db + k * step_b, idesc, true);
                         umma_commit_pair(empty0 + 8 * stage);
                     }
                     __syncwarp();
@@ -381,7 +387,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 continue;
             }
             const int row0 = t.m * kTile + rank * kHalfTile + q * 32, row = row0 + lane;
-            const int col0 = t.n * kTile + h * kHalfTile;
+            const int width = narrow(t) ? NT / 4 : NT / 2;  // columns of this warp's half
+            const int col0 = t.n * NT + h * width;
             // a warp whose rows are all past the end has nothing to write, except that dz is
             // defined (zero) on whole 64-row blocks: the weight gradient sums over those
             const bool busy = EPI == kEpiGradZ ? row0 < max(64, (rows + 63) & ~63) : row0 < m_ext;
@@ -403,16 +410,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             if (!mbar_wait(acc_full0 + 8 * acc, acc_phase, stop)) break;
             tc_fence_after();
             if (busy) {
-                const uint32_t base = tmem + acc * kTile + h * kHalfTile + (static_cast<uint32_t>(q * 32) << 16);
+                const uint32_t base = tmem + acc * NT + h * width + (static_cast<uint32_t>(q * 32) << 16);
                 float m = -INFINITY, s = 0.0f;
                 // not unrolled: four copies of this code measured 9.6 us for a kernel's first
                 // tile (instruction fetches) against 3.7
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < width / 32; ++c) {
                     uint32_t r[32];
                     tmem_ld32(base + 32 * c, r);
                     tmem_wait_ld(r);
-                    if (c == 3) release();  // all is read: the next tile may have the accumulator
+                    if (c == width / 32 - 1) release();  // all is read: the next tile may have the accumulator
                     const int cc = col0 + 32 * c;
                     const bool here = tcol >= 32 * c && tcol < 32 * c + 32;  // the target's column
                     if (EPI == kEpiStats) {
@@ -624,7 +631,8 @@ __global__ void __launch_bounds__(256) copy_rows16_kernel(const uint16_t* __rest
 // ---------------------------------------------------------------------------
 // Forward: merge a row's pieces, form its value, reduce
 // ---------------------------------------------------------------------------
-// WARPS warps of a CTA share a row: all eight of them above 64 pieces.
+// WARPS warps of a CTA share a row: all eight for long rows that fit the SMs at once
+// (6061 rows of 600 pieces: 28 us that way, 8 us a warp to a row).
 template <int WARPS>
 __global__ void __launch_bounds__(256) finish_forward_kernel(
     const float2* __restrict__ part, int pieces, const float* __restrict__ zt,
@@ -751,35 +759,53 @@ __global__ void __launch_bounds__(1024) coefficients_kernel(
     }
 }
 
-template <bool BF16>
+// LANES neighbouring lanes share four columns of a row, each a part of the slabs: 8 of
+// them where few columns have many slabs (49 x 176 in 64 slabs: 12.6 us with one).
+template <bool BF16, int LANES>
 __global__ void __launch_bounds__(256) finish_hidden_kernel(const float* __restrict__ slabs, int splits,
                                                             int64_t slab_elems, const int* __restrict__ pos,
                                                             const int* __restrict__ meta,
-                                                            const float* __restrict__ inv_scale, int D,
-                                                            int ld, uint16_t* __restrict__ out) {
+                                                            const float* __restrict__ inv_scale, int64_t N,
+                                                            int D, int ld, uint16_t* __restrict__ out) {
     pdl_wait();
     pdl_launch_dependents();
-    const int64_t row = blockIdx.x;
-    const int64_t p = pos ? pos[row] : row;
     const float scale = meta[kMetaStop] ? __int_as_float(0x7fc00000) : inv_scale ? *inv_scale : 1.0f;
-    uint16_t* o = out + row * D;
-    const float* s = slabs + p * ld;
+    const int groups = (D + 3) / 4;
     const bool wide = D % 4 == 0;
-    for (int j = 4 * (blockIdx.y * 256 + threadIdx.x); j < D; j += 4 * 256 * gridDim.y) {
+    const int part = threadIdx.x % LANES;
+    constexpr int kPerBlock = 256 / LANES;
+    const int64_t total = N * groups;
+    // a block's bound is the same for all its threads: the shuffles are whole
+    for (int64_t first = (int64_t)blockIdx.x * kPerBlock; first < total; first += (int64_t)gridDim.x * kPerBlock) {
+        const int64_t i = min(first + threadIdx.x / LANES, total - 1);
+        const int64_t row = i < UINT32_MAX ? static_cast<uint32_t>(i) / static_cast<uint32_t>(groups) : i / groups;
+        const int j = 4 * static_cast<int>(i - row * groups);
+        const int64_t p = pos ? pos[row] : row;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (p >= 0) {
-            for (int k = 0; k < splits; ++k) {  // in the order of the vocabulary
-                const float4 w = __ldg(reinterpret_cast<const float4*>(s + k * slab_elems + j));
+            const float* s = slabs + p * ld + j;
+#pragma unroll 8
+            for (int k = part; k < splits; k += LANES) {
+                const float4 w = __ldg(reinterpret_cast<const float4*>(s + k * slab_elems));
                 v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
             }
-            v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
         }
+#pragma unroll
+        for (int off = LANES / 2; off > 0; off /= 2) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, off);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, off);
+            v.z += __shfl_xor_sync(0xffffffffu, v.z, off);
+            v.w += __shfl_xor_sync(0xffffffffu, v.w, off);
+        }
+        if (part != 0 || first + threadIdx.x / LANES >= total) continue;
+        if (p >= 0) v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
+        uint16_t* o = out + row * D + j;
         const uint32_t lo = pack16<BF16>(v.x, v.y), hi = pack16<BF16>(v.z, v.w);
         if (wide) {
-            *reinterpret_cast<uint2*>(o + j) = make_uint2(lo, hi);
+            *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
         } else {
             const uint32_t w[2] = {lo, hi};
-            for (int i = 0; i < 4 && j + i < D; ++i) o[j + i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+            for (int e = 0; e < 4 && j + e < D; ++e) o[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
         }
     }
 }
@@ -1058,7 +1084,7 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group
     else
         st = launch_product<kEpiFew, 128>(w_map, h_map, h_map, g, tiles_v, bf16, s, what);
     if (st) return st;
-    const bool wide = pieces > 64;
+    const bool wide = pieces > 64 && N <= 8ll * sm_count();
     auto finish = wide ? finish_forward_kernel<8> : finish_forward_kernel<1>;
     LaunchCfg lc(dim3((unsigned)std::min<int64_t>(wide ? N : (N + 7) / 8, 32ll * sm_count())), dim3(256), 0, s);
     FL_CUDA(cudaLaunchKernelEx(&lc.cfg, finish, (const float2*)part, g.pieces, (const float*)zt, target,
@@ -1189,12 +1215,16 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
         }
     }
     if (grad_hidden) {
-        auto kern = bf16 ? finish_hidden_kernel<true> : finish_hidden_kernel<false>;
-        const int64_t gy = std::min<int64_t>(8, (D + 1023) / 1024);
-        LaunchCfg lc(dim3((unsigned)N, (unsigned)gy), dim3(256), 0, s);
+        const int64_t groups = N * ((D + 3) / 4);
+        const bool shared = plan.splits >= 8 && groups < 1024ll * sm_count();
+        auto kern = shared ? (bf16 ? finish_hidden_kernel<true, 8> : finish_hidden_kernel<false, 8>)
+                           : (bf16 ? finish_hidden_kernel<true, 1> : finish_hidden_kernel<false, 1>);
+        const int64_t per_block = shared ? 32 : 256;
+        const int64_t grid = std::min<int64_t>((groups + per_block - 1) / per_block, 32ll * sm_count());
+        LaunchCfg lc(dim3((unsigned)grid), dim3(256), 0, s);
         FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, (const float*)slabs, plan.splits,
                                    plan.slab_rows * packed_ld(D), (const int*)keep.pos, (const int*)keep.meta,
-                                   (const float*)inv_scale, (int)D, (int)packed_ld(D), grad_hidden));
+                                   (const float*)inv_scale, N, (int)D, (int)packed_ld(D), grad_hidden));
         return check_launch(what);
     }
     return FL_OK;
