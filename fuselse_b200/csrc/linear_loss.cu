@@ -342,9 +342,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                         const uint64_t da = desc_a + stage * (Shape::kStageBytes >> 4);
                         const uint64_t db = desc_b + stage * (Shape::kStageBytes >> 4);
                         umma_pair(tmem + acc * NT, da, db, idesc, kb != t.k0);
+                        const int left = k_ext - kb * kBlockK;  // the last block may hold less than 64
 #pragma unroll
                         for (int k = 1; k < kBlockK / 16; ++k)
-                            umma_pair(tmem + acc * NT, da + k * step_a, db + k * step_b, idesc, true);
+                            if (16 * k < left)
+                                umma_pair(tmem + acc * NT, da + k * step_a, db + k * step_b, idesc, true);
                         umma_commit_pair(empty0 + 8 * stage);
                     }
                     __syncwarp();
