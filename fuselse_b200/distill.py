@@ -17,21 +17,29 @@ _REDUCTIONS = {"none": 1, "sum": 2, "mean": 3}
 
 
 class TopkDistillation(torch.autograd.Function):
-    """Student logits whose rows are read in place -> loss."""
+    """Student logits whose rows are read in place -> loss.
+    config: (temperature, reduce, err_flag)."""
 
     @staticmethod
-    def forward(ctx, logits, teacher_logits, teacher_index, temperature, reduce, err_flag):
+    def forward(ctx, logits, teacher_logits, teacher_index, config):
+        temperature, reduce, err_flag = config
         out, saved = ext.topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature,
                                                       reduce, err_flag)
-        ctx.save_for_backward(*saved)
-        ctx.config = temperature, reduce
+        ctx.save_for_backward(*saved[:3])
+        ctx.config = saved[3], temperature, reduce
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        return (ext.topk_distill_backward(grad_output, *ctx.saved_tensors, *ctx.config),
-                None, None, None, None, None)
+        return (_grads_once if torch.is_grad_enabled() else _grads)(ctx, grad_output)
+
+
+def _grads(ctx, grad_output):
+    return ext.topk_distill_backward(grad_output, *ctx.saved_tensors, *ctx.config), None, None, None
+
+
+# a second derivative is refused; the wrapper's cost is paid only where one could be asked for
+_grads_once = torch.autograd.function.once_differentiable(_grads)
 
 
 def topk_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
@@ -56,7 +64,7 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, t
     err = torch.zeros(1, dtype=torch.int32, device=logits.device) if check_index else None
     reduce = _REDUCTIONS[reduction]
     if torch.is_grad_enabled() and logits.requires_grad:
-        out = TopkDistillation.apply(logits, teacher_logits.detach(), teacher_index, temperature, reduce, err)
+        out = TopkDistillation.apply(logits, teacher_logits.detach(), teacher_index, (temperature, reduce, err))
     else:
         out, _ = ext.topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err)
     if check_index and int(err.item()):

@@ -25,26 +25,32 @@ _LOGP = 0
 
 
 class LinearLoss(torch.autograd.Function):
-    """hidden (..., D), weight (V, D), target (...) -> loss or log-probabilities."""
+    """hidden (..., D), weight (V, D), target (...) -> loss or log-probabilities.
+    config: (reduce, ignore_index, z_loss, vocab_chunk, err_flag)."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err_flag):
+    def forward(ctx, hidden, weight, target, config):
+        reduce, ignore_index, z_loss, vocab_chunk, err_flag = config
         out, saved = ext.linear_loss_forward_checked(hidden, weight, target, reduce, ignore_index, z_loss,
                                                      err_flag, True)
         # an operand that is used as it lies is saved as the input it is
-        ctx.save_for_backward(*saved[:4])
-        ctx.config = hidden.shape, reduce, z_loss, vocab_chunk, saved[4]
+        ctx.save_for_backward(*saved[:3])
+        ctx.config = saved[3], saved[4], hidden.shape, reduce, z_loss, vocab_chunk
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        shape, reduce, z_loss, vocab_chunk, pack = ctx.config
-        want_hidden, want_weight = ctx.needs_input_grad[:2]
-        grad_hidden, grad_weight = ext.linear_loss_backward(
-            grad_output, *ctx.saved_tensors, pack, shape, reduce, z_loss, vocab_chunk, want_hidden,
-            want_weight)
-        return grad_hidden, grad_weight, None, None, None, None, None, None
+        return (_grads_once if torch.is_grad_enabled() else _grads)(ctx, grad_output)
+
+
+def _grads(ctx, grad_output):
+    want_hidden, want_weight = ctx.needs_input_grad[:2]
+    return (*ext.linear_loss_backward(grad_output, *ctx.saved_tensors, *ctx.config, want_hidden, want_weight),
+            None, None)
+
+
+# a second derivative is refused; the wrapper's cost is paid only where one could be asked for
+_grads_once = torch.autograd.function.once_differentiable(_grads)
 
 
 def _apply(what, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, check_index):
@@ -55,7 +61,7 @@ def _apply(what, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chu
     ext.check_linear_loss(what, hidden, weight, target)
     err = torch.zeros(1, dtype=torch.int32, device=hidden.device) if check_index else None
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        out = LinearLoss.apply(hidden, weight, target, reduce, ignore_index, z_loss, vocab_chunk, err)
+        out = LinearLoss.apply(hidden, weight, target, (reduce, ignore_index, z_loss, vocab_chunk, err))
     else:
         out, _ = ext.linear_loss_forward_checked(hidden, weight, target, reduce, ignore_index, z_loss, err, False)
     if check_index and int(err.item()):

@@ -244,6 +244,21 @@ def test_equal_calls_give_equal_bits_and_backward_twice():
     assert torch.equal(first[0], second[0]) and torch.equal(first[1], second[1])
 
 
+def test_second_derivatives_are_refused():
+    h, w, t, _ = make(20, 32, 90, BF16)
+    hg, wg = h.requires_grad_(), w.requires_grad_()
+    plain = torch.autograd.grad(linear_cross_entropy(hg, wg, t), (hg, wg))
+    again = torch.autograd.grad(linear_cross_entropy(hg, wg, t), (hg, wg), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+    with pytest.raises(RuntimeError, match="does not require grad"):
+        torch.autograd.grad(again[0].float().sum(), (hg,))
+    # with an upstream gradient that is itself differentiated through
+    up = torch.ones((), device="cuda", requires_grad=True)
+    again = torch.autograd.grad(linear_cross_entropy(hg, wg, t), (hg, wg), up, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        again[0].float().sum().backward()
+
+
 def test_gradient_against_differences():
     """Central differences of the 64-bit loss along random directions."""
     h, w, t, _ = make(20, 32, 90, BF16)
@@ -348,6 +363,23 @@ def test_fresh_host_threads():
         worker.join()
     assert torch.equal(got["out"], want[0])
     assert torch.equal(got["grads"][0], want[1]) and torch.equal(got["grads"][1], want[2])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_a_call_that_gave_up_marks_its_outputs(dtype):
+    """The word that a kernel sets when one of its waits ran out makes the kernels after it
+    return at once, with NaN for every output."""
+    from fuselse_b200 import ext
+    h, w, t, up = make(300, 128, 1000, dtype)
+    out, saved = ext.linear_loss_forward(h, w, t, 0)
+    saved[3].view(torch.int32)[2] = 1
+    gh, gw = ext.linear_loss_backward(up, *saved, h.shape, 0)
+    torch.cuda.synchronize()
+    assert gh.isnan().all() and gw.isnan().all() and torch.isfinite(out).all()
+    # a new call starts clean
+    again, saved = ext.linear_loss_forward(h, w, t, 0)
+    gh, gw = ext.linear_loss_backward(up, *saved, h.shape, 0)
+    assert torch.equal(again, out) and torch.isfinite(gh).all() and torch.isfinite(gw).all()
 
 
 def test_captured_step_replays_on_new_data():
