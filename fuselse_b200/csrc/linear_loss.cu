@@ -878,7 +878,15 @@ int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
                    int64_t units, bool bf16, cudaStream_t stream, const char* what) {
     auto kern = bf16 ? product_kernel<EPI, true, NT> : product_kernel<EPI, false, NT>;
     constexpr uint32_t smem = GemmShape<EPI, NT>::kSmem;
-    FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // once per kernel and device (concurrent first calls set the same value)
+    static std::atomic<uint64_t> ready[2];
+    int dev = 0;
+    FL_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev > 63 || !(ready[bf16].load(std::memory_order_acquire) & bit)) {
+        FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev <= 63) ready[bf16].fetch_or(bit, std::memory_order_release);
+    }
     args.group = group_rows(args.k_extent < 0 ? args.rows : args.k_extent);
     const int64_t pairs = std::max<int64_t>(1, std::min<int64_t>(units, sm_count() / 2));
     LaunchCfg lc(dim3((unsigned)(2 * pairs)), dim3(kGemmThreads), smem, stream);
