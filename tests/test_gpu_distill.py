@@ -270,6 +270,23 @@ def test_no_rows():
     assert topk_distillation_loss(z, t, i, reduction="none").shape == (2, 0)
 
 
+@pytest.mark.slow
+def test_logits_past_32_bit_offsets():
+    """2.2e9 logits: the first and the last rows."""
+    N, V, K = 17001, 128256, 8
+    z = torch.empty(N, V, device="cuda", dtype=torch.bfloat16)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    z.normal_(0, 2, generator=g)
+    index = torch.randint(0, V, (N, K), device="cuda", generator=g)
+    t = torch.randn(N, K, device="cuda", generator=g)
+    loss, got = run(z, t, index, 1.0, "none", torch.ones(N, device="cuda"))
+    for part in (slice(0, 4), slice(N - 4, N)):
+        coef = torch.ones(4, dtype=F64, device="cuda")
+        value, verr, grad, gerr, _ = reference(z[part].detach(), t[part], index[part], 1.0, coef, torch.bfloat16)
+        close(loss[part], value, verr, "loss")
+        close(got[part], grad, gerr, "gradient")
+
+
 def test_streams_and_graphs():
     a, b = make(50, 3000, 30, torch.bfloat16, seed=1), make(50, 3000, 30, torch.bfloat16, seed=9)
     z, t, index = (x.clone() for x in a)

@@ -295,17 +295,88 @@ def test_extreme_logits():
     assert torch.isfinite(gh).all() and torch.isfinite(gw).all()
 
 
-def test_nan_and_inf_rows_stay_in_their_rows():
-    h, w, t, up = make(300, 64, 700, BF16)
+@pytest.mark.parametrize("n", [20, 100, 300])
+def test_nan_and_inf_rows_stay_in_their_rows(n):
+    h, w, t, up = make(n, 64, 700, BF16)
     clean = linear_selective_log_softmax(h, w, t)
     h2 = h.clone()
     h2[3, 5] = float("nan")
-    h2[200] = float("inf")
+    h2[n - 2] = float("inf")
     out = linear_selective_log_softmax(h2, w, t)
-    keep = torch.ones(300, dtype=torch.bool, device="cuda")
-    keep[3] = keep[200] = False
-    assert out[3].isnan() and out[200].isnan()
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[3] = keep[n - 2] = False
+    assert out[3].isnan() and out[n - 2].isnan()
     assert torch.equal(out[keep], clean[keep])
+
+
+@pytest.mark.parametrize("n", [5, 200])
+def test_vocabulary_entries_of_minus_infinity(n):
+    """Logits of -inf (a weight row that makes them so) carry no probability; a target there
+    has a log-probability of -inf."""
+    h = torch.ones(n, 16, device="cuda", dtype=BF16)
+    h[:, 1] = torch.arange(n, device="cuda") / n
+    w = torch.zeros(400, 16, device="cuda", dtype=BF16)
+    w[:, 1] = torch.linspace(-2, 2, 400, device="cuda")
+    w[::3, 0] = -float("inf")
+    t = torch.full((n,), 1, device="cuda")
+    t[0] = 3
+    out = linear_selective_log_softmax(h, w, t)
+    z = h.to(F64) @ torch.where(w == -float("inf"), torch.zeros_like(w), w).to(F64).t()
+    z[:, ::3] = -float("inf")
+    want = z.log_softmax(-1)[torch.arange(n, device="cuda"), t]
+    assert out[0] == -float("inf")
+    assert ((out[1:].to(F64) - want[1:]).abs() <= 1e-5 * want[1:].abs().clamp_min(1)).all()
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_shapes(seed):
+    import random
+    rng = random.Random(seed)
+    N, D, V = rng.randint(1, 700), rng.randint(1, 400), rng.randint(1, 3000)
+    dtype = rng.choice([BF16, FP16])
+    chunk = rng.choice([None, 256, 512, 1024])
+    h, w, t, up = make(N, D, V, dtype, seed=seed)
+    if rng.random() < 0.5:
+        _check_logp(h, w, t, up, _logp_case(h, w, t, up, vocab_chunk=chunk), rms=False)
+        return
+    z_loss = rng.choice([0.0, 1e-3])
+    drop = torch.rand(N, generator=torch.Generator().manual_seed(seed)).cuda() < rng.choice([0.0, 0.5, 0.95])
+    drop[N - 1] = False
+    target, live = t.masked_fill(drop, -1), ~drop
+    hg, wg = h.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(hg, wg, target, ignore_index=-1, reduction="none", z_loss=z_loss, vocab_chunk=chunk)
+    gh, gw = torch.autograd.grad(loss, (hg, wg), up)
+    ref = reference(h.detach()[live], w.detach(), t[live], up[live].to(F64), z_loss=z_loss)
+    within(loss[live], ref["value"], ref["value_err"], "loss")
+    within(gh[live], ref["grad_hidden"], ref["grad_hidden_err"], "grad_hidden")
+    within(gw, ref["grad_weight"], ref["grad_weight_err"], "grad_weight")
+    assert (gh[drop] == 0).all() and (loss[drop] == 0).all()
+
+
+@pytest.mark.slow
+@pytest.mark.parametrize("n", [3, 140])
+def test_weights_past_32_bit_offsets(n):
+    """2.2e9 weights: values, and gradients of the first and the last vocabulary entries."""
+    V, D = 270001, 8192
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.empty(V, D, device="cuda", dtype=BF16).normal_(0, 0.02, generator=g)
+    h = torch.randn(n, D, device="cuda", generator=g).to(BF16)
+    t = torch.randint(0, V, (n,), device="cuda", generator=g)
+    t[0], t[1] = V - 1, 0
+    up = torch.randn(n, device="cuda", generator=g)
+    logp, gh, gw = _logp_case(h, w, t, up)
+    hd = h.to(F64)
+    z = torch.cat([hd @ w[lo:lo + 30000].to(F64).t() for lo in range(0, V, 30000)], 1)
+    lse = torch.logsumexp(z, -1)
+    rows = torch.arange(n, device="cuda")
+    bound = 2 * D * 2.0 ** -23 * 0.02 * hd.abs().sum(-1) + 1e-5 * lse.abs().clamp_min(1)
+    assert ((logp.to(F64) - (z[rows, t] - lse)).abs() <= bound).all()
+    dz = -up.to(F64)[:, None] * torch.exp(z - lse[:, None])
+    dz[rows, t] += up.to(F64)
+    for part in (slice(0, 300), slice(V - 300, V)):
+        rms_close(gw[part], dz[:, part].t() @ hd, BF16, "grad_weight")
+    dh = sum(dz[:, lo:lo + 30000] @ w[lo:lo + 30000].to(F64) for lo in range(0, V, 30000))
+    rms_close(gh, dh, BF16, "grad_hidden")
 
 
 def test_int32_targets_and_shapes():
