@@ -24,7 +24,7 @@ class TopkDistillation(torch.autograd.Function):
     def forward(ctx, logits, teacher_logits, teacher_index, config):
         temperature, reduce, err_flag = config
         out, saved = ext.topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature,
-                                                      reduce, err_flag)
+                                                      reduce, err_flag, True)
         ctx.save_for_backward(*saved[:3])
         ctx.config = saved[3], temperature, reduce
         return out
@@ -66,7 +66,8 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, t
     if torch.is_grad_enabled() and logits.requires_grad:
         out = TopkDistillation.apply(logits, teacher_logits.detach(), teacher_index, (temperature, reduce, err))
     else:
-        out, _ = ext.topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err)
+        out, _ = ext.topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err,
+                                                  False)
     if check_index and int(err.item()):
         raise RuntimeError(f"topk_distillation_loss: index out of range for {logits.shape[-1]} classes")
     return out

@@ -23,7 +23,6 @@ row_layout / *_strided (rows read in place) and logsumexp_dim* (dim != -1).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 
@@ -183,12 +182,23 @@ _DTYPE16 = {torch.float16: 0, torch.bfloat16: 1}
 _INDEX = (torch.int64, torch.int32)
 
 
-def _on_device(dev: torch.device):
-    """The guard of a call on `dev`: workspace sizes and outputs follow the current device."""
-    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _on_device(f):
+    """Runs f(t, ...) with t's device current: workspace sizes and outputs follow it."""
+    @functools.wraps(f)
+    def guarded(t, *args, **kwargs):
+        if torch.cuda.current_device() == t.device.index:
+            return f(t, *args, **kwargs)
+        with torch.cuda.device(t.device):
+            return f(t, *args, **kwargs)
+    return guarded
 
 
-_NO_GUARD = contextlib.nullcontext()
+def _dense_or_layout(x: torch.Tensor):
+    """row_layout, at once for dense rows."""
+    if x.is_contiguous():
+        N = x.shape[-1]
+        return x.numel() // N, N, -1, 0, N
+    return row_layout(x)
 
 
 def _addr(t):
@@ -203,9 +213,9 @@ def _raw_stream(dev: torch.device) -> int:
 
 def check_linear_loss(what: str, hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor) -> None:
     """The argument checks of linear_cross_entropy and linear_selective_log_softmax."""
-    for t, name in ((hidden, "hidden"), (weight, "weight"), (target, "target")):
-        if not isinstance(t, torch.Tensor):
-            raise RuntimeError(f"{what}: {name} must be a tensor")
+    if not (isinstance(hidden, torch.Tensor) and isinstance(weight, torch.Tensor)
+            and isinstance(target, torch.Tensor)):
+        raise RuntimeError(f"{what}: hidden, weight and the targets: each must be a tensor")
     hs, ws = hidden.shape, weight.shape
     if hidden.dtype not in _DTYPE16 or weight.dtype != hidden.dtype:
         raise RuntimeError(f"{what}: hidden and weight must both be fp16 or both bf16 "
@@ -260,10 +270,10 @@ def linear_loss_sizes(N: int, V: int, D: int, pack: int = PACK_KEPT, vocab_chunk
 def _hidden_rows(hidden: torch.Tensor):
     """(hidden, rows_per_group, group_stride, row_stride, whether the products can read
     it as it lies); a copy where the rows have no layout that row_layout names."""
-    lay = row_layout(hidden)
+    lay = _dense_or_layout(hidden)
     if lay is None:
         hidden = hidden.contiguous()
-        lay = row_layout(hidden)
+        lay = _dense_or_layout(hidden)
     N, D, rpg, gs, rs = lay
     plain = (D % 8 == 0 and rs % 8 == 0 and rs >= D and (rpg < 0 or rpg >= N)
              and hidden.data_ptr() % 16 == 0)
@@ -286,38 +296,39 @@ def linear_loss_forward(hidden: torch.Tensor, weight: torch.Tensor, target: torc
     return linear_loss_forward_checked(hidden, weight, target, reduce, ignore_index, z_loss, err_flag, keep)
 
 
+@_on_device
 def linear_loss_forward_checked(hidden, weight, target, reduce, ignore_index, z_loss, err_flag, keep):
     """linear_loss_forward of arguments that check_linear_loss has passed."""
     V, D = weight.shape
     shape, dev = target.shape, hidden.device
-    with _on_device(dev):
-        stream = _raw_stream(dev)
-        N = target.numel()
-        if target.dtype != torch.int64 or not target.is_contiguous():
-            target = target.to(torch.int64).contiguous()
-        w, ldw = _weight_rows(weight)
-        rows, rpg, gs, rs, plain = _hidden_rows(hidden)
-        pack = PACK_KEPT if ignore_index is not None else PACK_NONE if plain and rows is hidden else PACK_ALL
-        out = torch.empty(shape if reduce < 2 else (), dtype=torch.float32, device=dev)
-        if N == 0:
-            if reduce >= 2:
-                out.fill_(float("nan") if reduce == 3 else 0.0)
-            return out, (None, w, target, None, pack)
-        need_state, need, _ = linear_loss_sizes(N, V, D, pack)
-        if keep:
-            state = torch.empty(need_state, dtype=torch.uint8, device=dev)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            at_state, at_ws = state.data_ptr(), ws.data_ptr()
-        else:  # one scratch buffer holds both (sizes are multiples of 256 bytes)
-            ws = torch.empty(need_state + need, dtype=torch.uint8, device=dev)
-            at_state = ws.data_ptr()
-            at_ws = at_state + need_state
-        call("fl_linear_loss_fwd", rows.data_ptr(), rpg, gs, rs, w.data_ptr(), ldw, _DTYPE16[hidden.dtype],
-             target.data_ptr(), pack, 0 if ignore_index is None else ignore_index, N, V, D, reduce, z_loss,
-             at_state, need_state, out.data_ptr(), at_ws, need, _addr(err_flag), stream)
+    stream = _raw_stream(dev)
+    N = target.numel()
+    if target.dtype != torch.int64 or not target.is_contiguous():
+        target = target.to(torch.int64).contiguous()
+    w, ldw = _weight_rows(weight)
+    rows, rpg, gs, rs, plain = _hidden_rows(hidden)
+    pack = PACK_KEPT if ignore_index is not None else PACK_NONE if plain and rows is hidden else PACK_ALL
+    out = torch.empty(shape if reduce < 2 else (), dtype=torch.float32, device=dev)
+    if N == 0:
+        if reduce >= 2:
+            out.fill_(float("nan") if reduce == 3 else 0.0)
+        return out, (None, w, target, None, pack)
+    need_state, need, _ = linear_loss_sizes(N, V, D, pack)
+    if keep:
+        state = torch.empty(need_state, dtype=torch.uint8, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        at_state, at_ws = state.data_ptr(), ws.data_ptr()
+    else:  # one scratch buffer holds both (sizes are multiples of 256 bytes)
+        ws = torch.empty(need_state + need, dtype=torch.uint8, device=dev)
+        at_state = ws.data_ptr()
+        at_ws = at_state + need_state
+    call("fl_linear_loss_fwd", rows.data_ptr(), rpg, gs, rs, w.data_ptr(), ldw, _DTYPE16[hidden.dtype],
+         target.data_ptr(), pack, 0 if ignore_index is None else ignore_index, N, V, D, reduce, z_loss,
+         at_state, need_state, out.data_ptr(), at_ws, need, _addr(err_flag), stream)
     return out, None if not keep else (hidden if pack == PACK_NONE else None, w, target, state, pack)
 
 
+@_on_device
 def linear_loss_backward(grad_output: torch.Tensor, hidden, weight: torch.Tensor, target: torch.Tensor, state,
                          pack: int, shape, reduce: int, z_loss: float = 0.0, vocab_chunk: int = 0,
                          want_hidden: bool = True, want_weight: bool = True):
@@ -328,28 +339,27 @@ def linear_loss_backward(grad_output: torch.Tensor, hidden, weight: torch.Tensor
     D = shape[-1]
     V, Dp = weight.shape[0], (D + 7) // 8 * 8
     N, dev, dtype = target.numel(), weight.device, weight.dtype
-    with _on_device(dev):
-        stream = _raw_stream(dev)
-        g = grad_output
-        if g.dtype != torch.float32 or not g.is_contiguous():
-            g = g.to(torch.float32).contiguous()
-        _check(g.numel() == (1 if reduce >= 2 else N), "grad_output does not match the forward's output")
-        grad_hidden = torch.empty(shape, dtype=dtype, device=dev) if want_hidden else None
-        grad_weight = torch.empty((V, Dp), dtype=dtype, device=dev) if want_weight else None
-        if N:
-            rpg, gs, rs = row_layout(hidden)[2:] if hidden is not None else (-1, 0, 0)
-            need_state, _, need = linear_loss_sizes(N, V, D, pack, vocab_chunk, want_hidden)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            call("fl_linear_loss_bwd", g.data_ptr(), _addr(hidden), rpg, gs, rs, weight.data_ptr(),
-                 weight.stride(0) if V > 1 else Dp, _DTYPE16[dtype], target.data_ptr(), pack, N, V, D, reduce,
-                 z_loss, vocab_chunk, state.data_ptr(), need_state, _addr(grad_hidden), _addr(grad_weight),
-                 ws.data_ptr(), need, stream)
-        elif want_weight:
-            grad_weight.zero_()
-        if want_weight and Dp != D:
-            cut = torch.empty((V, D), dtype=dtype, device=dev)
-            call("fl_copy_rows16", grad_weight.data_ptr(), cut.data_ptr(), V, Dp, D, -1, 0, 0, stream)
-            grad_weight = cut
+    stream = _raw_stream(dev)
+    g = grad_output
+    if g.dtype != torch.float32 or not g.is_contiguous():
+        g = g.to(torch.float32).contiguous()
+    _check(g.numel() == (1 if reduce >= 2 else N), "grad_output does not match the forward's output")
+    grad_hidden = torch.empty(shape, dtype=dtype, device=dev) if want_hidden else None
+    grad_weight = torch.empty((V, Dp), dtype=dtype, device=dev) if want_weight else None
+    if N:
+        rpg, gs, rs = _dense_or_layout(hidden)[2:] if hidden is not None else (-1, 0, 0)
+        need_state, _, need = linear_loss_sizes(N, V, D, pack, vocab_chunk, want_hidden)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        call("fl_linear_loss_bwd", g.data_ptr(), _addr(hidden), rpg, gs, rs, weight.data_ptr(),
+             weight.stride(0) if V > 1 else Dp, _DTYPE16[dtype], target.data_ptr(), pack, N, V, D, reduce,
+             z_loss, vocab_chunk, state.data_ptr(), need_state, _addr(grad_hidden), _addr(grad_weight),
+             ws.data_ptr(), need, stream)
+    elif want_weight:
+        grad_weight.zero_()
+    if want_weight and Dp != D:
+        cut = torch.empty((V, D), dtype=dtype, device=dev)
+        call("fl_copy_rows16", grad_weight.data_ptr(), cut.data_ptr(), V, Dp, D, -1, 0, 0, stream)
+        grad_weight = cut
     return grad_hidden, grad_weight
 
 
@@ -363,10 +373,9 @@ MAX_TOP = 1024
 def check_topk_distill(what: str, logits: torch.Tensor, teacher_logits: torch.Tensor,
                        teacher_index: torch.Tensor, temperature: float) -> None:
     """The argument checks of topk_distillation_loss."""
-    for t, name in ((logits, "logits"), (teacher_logits, "teacher_logits"),
-                    (teacher_index, "teacher_index")):
-        if not isinstance(t, torch.Tensor):
-            raise RuntimeError(f"{what}: {name} must be a tensor")
+    if not (isinstance(logits, torch.Tensor) and isinstance(teacher_logits, torch.Tensor)
+            and isinstance(teacher_index, torch.Tensor)):
+        raise RuntimeError(f"{what}: logits, teacher_logits and teacher_index: each must be a tensor")
     zs, ts = logits.shape, teacher_logits.shape
     if logits.dtype not in _DTYPE or teacher_logits.dtype not in _DTYPE:
         raise RuntimeError(f"{what}: logits must be fp32, fp16 or bf16 "
@@ -407,58 +416,66 @@ def topk_distill_workspace_bytes(N: int, V: int, dtype: torch.dtype) -> int:
 
 
 def topk_distill_forward(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
-                         temperature: float = 1.0, reduce: int = 1, err_flag=None):
+                         temperature: float = 1.0, reduce: int = 1, err_flag=None, keep: bool = True):
     """(out, saved): reduce 1 per-row losses (logits.shape[:-1]), 2 their sum, 3 their
     mean over the rows that keep a teacher entry.  logits rows are read in place
     (row_layout must address them); saved is what topk_distill_backward takes:
-    (logits, teacher_logits, teacher_index, state)."""
+    (logits, teacher_logits, teacher_index, state); without `keep` there is none (None)."""
     check_topk_distill("topk_distill_forward", logits, teacher_logits, teacher_index, temperature)
-    return topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err_flag)
+    return topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err_flag,
+                                        keep)
 
 
-def topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err_flag):
+@_on_device
+def topk_distill_forward_checked(logits, teacher_logits, teacher_index, temperature, reduce, err_flag, keep):
     """topk_distill_forward of arguments that check_topk_distill has passed."""
-    lay = row_layout(logits)
+    lay = _dense_or_layout(logits)
     _check(lay is not None, "logits rows cannot be addressed in place (more than two leading stride levels)")
     N, V, rpg, gs, rs = lay
     K, dev = teacher_logits.shape[-1], logits.device
-    with _on_device(dev):
-        tl, ti = _teacher(teacher_logits, teacher_index)
-        # the result shares no storage with what the backward keeps: a caller may change it in place
-        out = torch.empty(logits.shape[:-1] if reduce == 1 else (), dtype=torch.float32, device=dev)
-        state = torch.empty(2 * N + 1 + (0 if reduce == 1 else N), dtype=torch.float32, device=dev)
-        if N == 0:
-            if reduce >= 2:
-                out.fill_(float("nan") if reduce == 3 else 0.0)
-        else:
-            need = topk_distill_workspace_bytes(N, V, logits.dtype)
+    tl, ti = _teacher(teacher_logits, teacher_index)
+    # the result shares no storage with what the backward keeps: a caller may change it in place
+    out = torch.empty(logits.shape[:-1] if reduce == 1 else (), dtype=torch.float32, device=dev)
+    kept = 4 * (2 * N + 1 + (0 if reduce == 1 else N))  # lse, teacher_lse, count, values of a reduced loss
+    state = None
+    if N == 0:
+        if reduce >= 2:
+            out.fill_(float("nan") if reduce == 3 else 0.0)
+    else:
+        need = topk_distill_workspace_bytes(N, V, logits.dtype)
+        if keep:
+            state = torch.empty(kept, dtype=torch.uint8, device=dev)
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            at = state.data_ptr()  # lse, teacher_lse, count, values of a reduced loss
-            values = out.data_ptr() if reduce == 1 else at + 4 * (2 * N + 1)
-            call("fl_topk_distill_fwd", logits.data_ptr(), _DTYPE[logits.dtype], tl.data_ptr(),
-                 _DTYPE[tl.dtype], ti.data_ptr(), N, V, K, rpg, gs, rs, temperature, reduce, at, at + 4 * N,
-                 values, out.data_ptr(), at + 8 * N, ws.data_ptr(), need, _addr(err_flag), _raw_stream(dev))
-    return out, (logits, tl, ti, state)
+            at, at_ws = state.data_ptr(), ws.data_ptr()
+        else:  # one scratch buffer holds both
+            ws = torch.empty((need + 255) // 256 * 256 + kept, dtype=torch.uint8, device=dev)
+            at_ws = ws.data_ptr()
+            at = at_ws + (need + 255) // 256 * 256
+        values = out.data_ptr() if reduce == 1 else at + 4 * (2 * N + 1)
+        call("fl_topk_distill_fwd", logits.data_ptr(), _DTYPE[logits.dtype], tl.data_ptr(),
+             _DTYPE[tl.dtype], ti.data_ptr(), N, V, K, rpg, gs, rs, temperature, reduce, at, at + 4 * N,
+             values, out.data_ptr(), at + 8 * N, at_ws, need, _addr(err_flag), _raw_stream(dev))
+    return out, (logits, tl, ti, state) if keep else None
 
 
+@_on_device
 def topk_distill_backward(grad_output: torch.Tensor, logits: torch.Tensor, teacher_logits: torch.Tensor,
                           teacher_index: torch.Tensor, state: torch.Tensor, temperature: float = 1.0,
                           reduce: int = 1) -> torch.Tensor:
     """Dense gradient of logits, of their shape and dtype."""
-    N, V, rpg, gs, rs = row_layout(logits)
+    N, V, rpg, gs, rs = _dense_or_layout(logits)
     K, dev = teacher_logits.shape[-1], logits.device
-    with _on_device(dev):
-        g = grad_output
-        if g.dtype != torch.float32 or not g.is_contiguous():
-            g = g.to(torch.float32).contiguous()
-        _check(g.numel() == (N if reduce == 1 else 1), "grad_output does not match the forward's output")
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        if N:
-            at = state.data_ptr()
-            call("fl_topk_distill_bwd", g.data_ptr(), logits.data_ptr(), _DTYPE[logits.dtype],
-                 teacher_logits.data_ptr(), _DTYPE[teacher_logits.dtype], teacher_index.data_ptr(), N, V, K,
-                 rpg, gs, rs, temperature, reduce, at, at + 4 * N, at + 8 * N, grad.data_ptr(),
-                 _raw_stream(dev))
+    g = grad_output
+    if g.dtype != torch.float32 or not g.is_contiguous():
+        g = g.to(torch.float32).contiguous()
+    _check(g.numel() == (N if reduce == 1 else 1), "grad_output does not match the forward's output")
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    if N:
+        at = state.data_ptr()
+        call("fl_topk_distill_bwd", g.data_ptr(), logits.data_ptr(), _DTYPE[logits.dtype],
+             teacher_logits.data_ptr(), _DTYPE[teacher_logits.dtype], teacher_index.data_ptr(), N, V, K,
+             rpg, gs, rs, temperature, reduce, at, at + 4 * N, at + 8 * N, grad.data_ptr(),
+             _raw_stream(dev))
     return grad
 
 

@@ -453,6 +453,27 @@ def test_a_call_that_gave_up_marks_its_outputs(dtype):
     assert torch.equal(again, out) and torch.isfinite(gh).all() and torch.isfinite(gw).all()
 
 
+def test_logits_are_not_kept():
+    """What a step holds beside its operands and gradients: a piece of the vocabulary's logit
+    gradients and figures of each row, far below the logits."""
+    N, D, V = 4096, 64, 50304
+    h, w, t, _ = make(N, D, V, BF16)
+    hg, wg = h.requires_grad_(), w.requires_grad_()
+    torch.autograd.grad(linear_cross_entropy(hg, wg, t, vocab_chunk=1024), (hg, wg))
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    loss = linear_cross_entropy(hg, wg, t, vocab_chunk=1024)
+    held = torch.cuda.memory_allocated() - base
+    torch.autograd.grad(loss, (hg, wg))
+    peak = torch.cuda.max_memory_allocated() - base
+    logits = N * V * 2
+    # kept for the backward: the packed rows and three words a row; on top of it at the most
+    # the rows' partial states (16 bytes for 256 logits) or a piece, and the gradients
+    assert held <= 2 * N * D * 2 + 64 * N
+    assert peak <= held + max(N * 1024 * 2, logits // 16) + 4 * (N + V) * D + (8 << 20) < logits // 4
+
+
 def test_captured_step_replays_on_new_data():
     h, w, t, _ = make(300, 128, 1500, BF16, seed=1)
     h2, w2, t2, _ = make(300, 128, 1500, BF16, seed=2)
