@@ -220,6 +220,14 @@ __device__ __forceinline__ void few_rows_piece(uint32_t addr, int row0, int v0, 
     if ((lane & 1) == 0 && row < rows) args.part[(int64_t)row * args.pieces + piece] = make_float2(top, sum);
 }
 
+// The product kernel.  A tile of 256 x 256 over a CTA pair is the largest that leaves room
+// in tensor memory (512 columns) for a second accumulator; it asks 64 KB of operands for
+// every 64 of K, 512 cycles of the tensor pipe (32 KB per SM: half of what one CTA would
+// need for its 128 x 256 alone).  Bound by the tensor pipe from D = 512 up: a step of 64 of
+// K takes 512 cycles, 2048 x 2048 x 50257 240-250 us (1690-1757 TFLOP/s, pipe 92 % active)
+// where the 1000 W cap does not hold it, about 1400 TFLOP/s where it does.  Below, by the
+// epilogue (exponentials: 2048 cycles of a tile's 2900, 4000 with dz written); with few
+// rows or a short K by HBM (1 x 4096 x 128256: 162 us, 6.4 TB/s).
 template <int EPI, bool BF16, int NT = kTile>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -569,7 +577,8 @@ __device__ __forceinline__ int block_sum(int v, int* sh) {
 
 // Each CTA takes a contiguous range of rows; it counts the kept rows before the
 // range itself (the targets are a few KB that L2 serves), so one launch does it.
-// pos[row] = packed position or -1, src[position] = row.
+// pos[row] = packed position or -1, src[position] = row.  Bound by memory (6144 rows of
+// 4096: 24 us for 100 MB) and, when small, by the count's latency (1023 rows: 6 us).
 __global__ void __launch_bounds__(kPackThreads) pack_rows_kernel(
     const uint16_t* __restrict__ hidden, const int64_t* __restrict__ target, int64_t ignore,
     uint16_t* __restrict__ packed, int* __restrict__ src, int* __restrict__ pos, int* __restrict__ meta,
@@ -724,7 +733,8 @@ __global__ void __launch_bounds__(256) finish_forward_kernel(
 // fp16 only: the coefficients of dz = a softmax - b onehot, scaled by a power of two
 // that brings the largest to [2^13, 2^14): fp16 keeps its relative accuracy down to
 // probabilities of 1e-9 of it instead of flushing them.  bf16 has fp32's range and
-// forms its coefficients where it uses them.
+// forms its coefficients where it uses them.  One CTA, two passes over the rows: 3-5 us up
+// to 2048 of them, bound by its latency.
 __global__ void __launch_bounds__(1024) coefficients_kernel(
     const float* __restrict__ g, int reduce, float z_loss, const float* __restrict__ lse,
     const int* __restrict__ src, const int* __restrict__ meta, int64_t N, float* __restrict__ a,
@@ -761,6 +771,8 @@ __global__ void __launch_bounds__(1024) coefficients_kernel(
     }
 }
 
+// The hidden gradient: a row's slabs summed in the order of the vocabulary's K pieces, in
+// fp32, and rounded once.  Bound by the slabs' bytes (2048 x 2048: 8-10 us).
 // LANES neighbouring lanes share four columns of a row, each a part of the slabs: 8 of
 // them where few columns have many slabs (49 x 176 in 64 slabs: 12.6 us with one).
 template <bool BF16, int LANES>
@@ -823,7 +835,8 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // lines takes two requests (products of 1000-element rows measured 1.8x as long).
 int64_t packed_ld(int64_t D) { return round_up(D, 64); }
 
-// K pieces of the hidden gradient: as many as fill the CTA pairs best, at least
+// K pieces of the hidden gradient, whose tiles are few (2048 x 2048: 64 for 74 CTA pairs;
+// 1 x 4096: 16): as many as fill the CTA pairs best, at least
 // 8 blocks deep each and slabs of at most 64 MB in all (one slab is needed anyway).
 int choose_splits(int64_t tiles, int64_t kb, int64_t slab_bytes, int pairs) {
     int best = 1;
