@@ -100,9 +100,6 @@ struct Unit {
     int m, n, k0, k1, slab;
 };
 
-// Work unit u: K piece by K piece, tiles of a piece in groups of `group` tile rows,
-// so that the tiles in flight share operand rows through L2 (group_rows).
-
 // Division by a number known for the whole kernel: the quotient from the high half of a
 // product is at most one too small.  (The divide instruction sequence took the two
 // threads that feed the tensor cores 0.4 us at every tile.)
@@ -116,6 +113,8 @@ struct Divisor {
     }
 };
 
+// Work unit u: K piece by K piece, tiles of a piece in groups of `group` tile rows,
+// so that the tiles in flight share operand rows through L2 (group_rows).
 struct Schedule {
     int mt, nt, splits, kb, tiles, group;
     Divisor by_tiles, by_group, by_full, by_last;
@@ -863,9 +862,9 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidd
     // 512 MB of dz by default: the hidden gradient is added to once per piece
     if (chunk <= 0) chunk = (256ll << 20) / std::max<int64_t>(N, 1);
     p.chunk = std::min(all, std::max<int64_t>(kTile, chunk / kTile * kTile));
-    p.slab_rows = round_up(N, kTile);
+    p.slab_rows = round_up(N, 32);  // a warp's box of rows
     const int64_t slab = p.slab_rows * packed_ld(Dp) * 4;
-    p.splits = want_hidden ? choose_splits((p.slab_rows / kTile) * ((Dp + kTile - 1) / kTile),
+    p.splits = want_hidden ? choose_splits(((N + kTile - 1) / kTile) * ((Dp + kTile - 1) / kTile),
                                            p.chunk / kBlockK, slab, pairs)
                            : 0;
     p.coef_off = 256;

@@ -257,6 +257,7 @@ def test_gradient_against_differences():
         d = torch.randn(6, 40, generator=g, device="cuda", dtype=F64)
         e = 1e-5
         want = (f(z.detach().to(F64) + e * d) - f(z.detach().to(F64) - e * d)) / (2 * e)
+        # every element is within 1e-4 of its value (the bounds above: 1e-5 |lse| and a few 2^-22)
         assert ((grad.to(F64) * d).sum() - want).abs() <= 1e-4 * (grad.to(F64) * d).abs().sum()
 
 
@@ -341,5 +342,7 @@ def test_together_with_the_vocabulary_losses():
     # moves a KL of their softmax by no more than twice the largest such step times T
     zmax = z.detach().abs().max().item()
     assert abs(loss.item() - want.item()) <= 0.5 * 2 * 2 * 2.0 ** -8 * zmax + 1e-4
+    # and their softmax by a factor of 2 2^-8 zmax / T at most, 4 % here, beside the roundings
+    # of the gradients themselves (a few 2^-9)
     for got, ref in ((h.grad, hd.grad), (w.grad, wd.grad)):
         assert (got.to(F64) - ref).norm() <= 0.05 * ref.norm()
