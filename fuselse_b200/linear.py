@@ -58,6 +58,10 @@ def _apply(what, hidden, weight, target, reduce, ignore_index, z_loss, vocab_chu
         vocab_chunk = 0
     elif isinstance(vocab_chunk, bool) or not isinstance(vocab_chunk, int) or not 1 <= vocab_chunk < 1 << 62:
         raise RuntimeError(f"{what}: vocab_chunk must be a positive int or None")
+    if torch.is_autocast_enabled("cuda"):  # as for a linear layer
+        dtype = torch.get_autocast_dtype("cuda")
+        hidden, weight = (t.to(dtype) if isinstance(t, torch.Tensor) and t.is_cuda and t.is_floating_point()
+                          else t for t in (hidden, weight))
     ext.check_linear_loss(what, hidden, weight, target)
     err = torch.zeros(1, dtype=torch.int32, device=hidden.device) if check_index else None
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
@@ -74,8 +78,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
                          vocab_chunk: int | None = None, check_index: bool = False) -> torch.Tensor:
     """Cross entropy of softmax(hidden @ weight.T) against `target`, fp32.
 
-    hidden (..., D) and weight (V, D) are CUDA fp16 or bf16 (the same), target
-    (...) integer.  Per token lse - z[target] + z_loss * lse^2; tokens whose
+    hidden (..., D) and weight (V, D) are CUDA fp16 or bf16 (the same; under
+    torch.autocast any floating type, cast to autocast's as for a linear layer),
+    target (...) integer.  Per token lse - z[target] + z_loss * lse^2; tokens whose
     target is `ignore_index` give 0, take no part in the mean and are left out
     of every product (their hidden states may hold anything).  reduction "mean"
     (over the other tokens; NaN without any), "sum" or "none" (target.shape).
@@ -100,8 +105,8 @@ def linear_selective_log_softmax(hidden: torch.Tensor, weight: torch.Tensor, ind
     """Log-probabilities of `index` under softmax(hidden @ weight.T), fp32, shape
     index.shape: selective_log_softmax(hidden @ weight.T, index) without the logits.
 
-    hidden (..., D) and weight (V, D) are CUDA fp16 or bf16 (the same), index
-    (...) integer.  An index outside [0, V) yields NaN; with `check_index=True`
+    hidden (..., D) and weight (V, D) are CUDA fp16 or bf16 (the same; under
+    torch.autocast any floating type), index (...) integer.  An index outside [0, V) yields NaN; with `check_index=True`
     it raises RuntimeError instead (one device sync).  Gradients and
     `vocab_chunk` as in linear_cross_entropy."""
     return _apply("linear_selective_log_softmax", hidden, weight, index, _LOGP, None, 0.0,

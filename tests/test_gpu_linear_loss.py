@@ -222,6 +222,23 @@ def test_weight_layouts(case):
     _check_logp(h, w, t, up, _logp_case(h, view, t, up))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_autocast(dtype):
+    """fp32 master weights under autocast: the cast operands' values, fp32 gradients."""
+    h, w, t, up = make(60, 64, 500, dtype)
+    h32, w32 = h.float().requires_grad_(), w.float().requires_grad_()
+    with torch.autocast("cuda", dtype=dtype):
+        out = linear_selective_log_softmax(h32, w32, t)
+        loss = linear_cross_entropy(h, w32, t)
+    gh, gw = torch.autograd.grad(out, (h32, w32), up)
+    want = _logp_case(h, w, t, up)
+    assert torch.equal(out, want[0]) and gh.dtype == gw.dtype == torch.float32
+    assert torch.equal(gh, want[1].float()) and torch.equal(gw, want[2].float())
+    assert torch.equal(loss, linear_cross_entropy(h, w, t))
+    with pytest.raises(RuntimeError, match="fp16 or both bf16"):
+        linear_selective_log_softmax(h32, w32, t)
+
+
 def test_only_one_gradient_wanted():
     h, w, t, up = make(90, 64, 500, BF16)
     _, gh, gw = _logp_case(h, w, t, up)
