@@ -46,13 +46,15 @@ enum Epi {
     kEpiOut16 = 2,   // scaled, in 16 bits
     kEpiSlab = 3,    // fp32 partial sums (stored, or added to what is there)
     kEpiFew = 4,     // as kEpiStats with the operands exchanged: few rows, vocabulary in M
+    kEpiGrads = 5,   // kEpiSlab's and kEpiOut16's units in one launch
 };
 
 // NT: columns of a tile (256; fewer for kEpiFew).
 template <int EPI, int NT>
 struct GemmShape {
-    static constexpr bool kAMn = EPI == kEpiOut16;                    // A given as [k][m]
-    static constexpr bool kBMn = EPI == kEpiOut16 || EPI == kEpiSlab;  // B given as [k][n]
+    // A given as [k][m] (kEpiGrads: as its unit's kind says), B given as [k][n]
+    static constexpr bool kAMn = EPI == kEpiOut16;
+    static constexpr bool kBMn = EPI == kEpiOut16 || EPI == kEpiSlab || EPI == kEpiGrads;
     static constexpr bool kStores = EPI != kEpiStats && EPI != kEpiFew;
     static constexpr uint32_t kBBytes = NT / 2 * kBlockK * 2;
     static constexpr uint32_t kStageBytes = kOperandBytes + kBBytes;
@@ -96,8 +98,15 @@ struct GemmArgs {
     int64_t out_elems;
 };
 
+// A product's operands and output; kEpiGrads has its kEpiSlab maps in 0-2, its kEpiOut16
+// maps in 3-5.
+struct alignas(64) Maps {
+    CUtensorMap a, b, out, a1, b1, out1;
+};
+
 struct Unit {
     int m, n, k0, k1, slab;
+    int kind;  // kEpiGrads: 0 a unit of kEpiSlab, 1 of kEpiOut16
 };
 
 // Division by a number known for the whole kernel: the quotient from the high half of a
@@ -124,6 +133,7 @@ struct Schedule {
           by_last(mt_ % group_ ? mt_ % group_ : group_) {}
     __device__ __forceinline__ Unit operator()(int u) const {
         Unit t;
+        t.kind = 0;
         t.slab = 0;
         t.k0 = 0;
         t.k1 = kb;
@@ -142,6 +152,40 @@ struct Schedule {
         t.n = last ? by_last(u) : by_full(u);
         t.m = m0 + u - t.n * (last ? mt - m0 : min(mt, group));
         return t;
+    }
+};
+
+// kEpiGrads: the long units of the hidden gradient go to the pairs in turn, first; the
+// last round of them leaves some pairs out (64 units for 74 pairs), and those run ahead on
+// the weight gradient's units meanwhile; then all pairs share the rest in turn.
+
+// What a weight-gradient unit of `blocks` K blocks costs, in blocks: its 256 columns are
+// stored beside the next unit's products, which cannot take less than about 6 of them
+// (4 x 6416 x 34866: 2 us a unit where a block of the hidden gradient takes 0.4).
+__host__ __device__ constexpr int weight_unit_cost(int blocks) { return blocks + 2 > 6 ? blocks + 2 : 6; }
+
+struct GradsWalk {
+    int pair, pairs, longs, shorts, busy, ahead, mine_long, mine_ahead;
+    __device__ __forceinline__ GradsWalk(int pair_, int pairs_, int longs_, int long_blocks, int shorts_,
+                                         int short_blocks)
+        : pair(pair_), pairs(pairs_), longs(longs_), shorts(shorts_) {
+        busy = longs % pairs;  // pairs that have a unit of the last round
+        const int idle = pairs - busy;
+        const int rounds = busy ? long_blocks / weight_unit_cost(short_blocks) : 0;
+        ahead = static_cast<int>(min((int64_t)shorts, (int64_t)rounds * idle));
+        mine_long = longs > pair ? (longs - pair + pairs - 1) / pairs : 0;
+        mine_ahead = pair >= busy && ahead > pair - busy ? (ahead - (pair - busy) + idle - 1) / idle : 0;
+    }
+    // The i-th unit of this pair: its kind and index, or kind -1 at the end.
+    __device__ __forceinline__ int operator()(int i, int& kind) const {
+        kind = 0;
+        if (i < mine_long) return pair + i * pairs;
+        kind = 1;
+        i -= mine_long;
+        if (i < mine_ahead) return pair - busy + i * (pairs - busy);
+        const int64_t u = ahead + pair + (int64_t)(i - mine_ahead) * pairs;
+        if (u >= shorts) kind = -1;
+        return static_cast<int>(u);
     }
 };
 
@@ -229,8 +273,7 @@ __device__ __forceinline__ void few_rows_piece(uint32_t addr, int row0, int v0, 
 // rows or a short K by HBM (1 x 4096 x 128256: 162 us, 6.4 TB/s).
 template <int EPI, bool BF16, int NT = kTile>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
-    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const __grid_constant__ CUtensorMap map_out, const GemmArgs args) {
+    product_kernel(const __grid_constant__ Maps maps, const GemmArgs args, const GemmArgs args1) {
     using Shape = GemmShape<EPI, NT>;
     constexpr int kStages = Shape::kStages;
     extern __shared__ uint8_t smem_raw[];
@@ -255,9 +298,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             mbar_init(acc_empty0 + 8 * s, 2 * kEpiWarps);
         }
         mbar_init_fence();
-        tma_prefetch_map(&map_a);
-        tma_prefetch_map(&map_b);
-        if (Shape::kStores) tma_prefetch_map(&map_out);
+        tma_prefetch_map(&maps.a);
+        tma_prefetch_map(&maps.b);
+        if (Shape::kStores) tma_prefetch_map(&maps.out);
+        if (EPI == kEpiGrads) {
+            tma_prefetch_map(&maps.a1);
+            tma_prefetch_map(&maps.b1);
+            tma_prefetch_map(&maps.out1);
+        }
     }
     if (warp == 2) tmem_alloc_pair(smem_u32(&tmem_slot), Shape::kTmemCols);
     pdl_wait();
@@ -274,49 +322,74 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
-    const int m_ext = args.m_extent < 0 ? rows : args.m_extent;
-    const int k_ext = args.k_extent < 0 ? rows : args.k_extent;
-    const int mt = max(1, (m_ext + kTile - 1) / kTile);
-    const int n_ext = args.n_extent < 0 ? rows : args.n_extent;
+    const int m_ext0 = args.m_extent < 0 ? rows : args.m_extent;
+    const int k_ext0 = args.k_extent < 0 ? rows : args.k_extent;
+    const int mt = max(1, (m_ext0 + kTile - 1) / kTile);
+    const int n_ext = args.n_extent < 0 ? rows : args.n_extent;  // both kinds' in kEpiGrads
     const int nt = EPI == kEpiFew ? 1 : (n_ext + NT - 1) / NT;
-    const int kb_total = max(1, (k_ext + kBlockK - 1) / kBlockK);
+    const int kb_total = max(1, (k_ext0 + kBlockK - 1) / kBlockK);
     const int units = mt * nt * args.splits;
     const Schedule unit(mt, nt, args.splits, kb_total, args.group);
     // a last column of tiles with at most 128 columns left is done 128 wide (MN-major B:
     // 64 columns staged by each CTA)
     auto narrow = [&](const Unit& t) { return Shape::kBMn && n_ext - t.n * NT <= NT / 2; };
     const int pair_id = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    // kEpiGrads: the weight gradient's units, and both kinds' figures by the unit's kind
+    const int kb1 = max(1, (rows + kBlockK - 1) / kBlockK);
+    const int mt1 = EPI == kEpiGrads ? (args1.m_extent + kTile - 1) / kTile : 1;
+    const Schedule unit1(mt1, nt, 1, kb1, EPI == kEpiGrads ? args1.group : 1);
+    const GradsWalk walk(pair_id, pairs, units, max(1, kb_total / args.splits), mt1 * nt, kb1);
+    auto second = [&](const Unit& t) { return EPI == kEpiGrads && t.kind == 1; };
+    // the i-th unit of this pair, false at the end
+    auto unit_at = [&](int i, Unit& t) {
+        if constexpr (EPI == kEpiGrads) {
+            int kind;
+            const int u = walk(i, kind);
+            if (kind < 0) return false;
+            t = kind ? unit1(u) : unit(u);
+            t.kind = kind;
+        } else {
+            const int64_t u = pair_id + (int64_t)i * pairs;
+            if (u >= units) return false;
+            t = unit(static_cast<int>(u));
+        }
+        return true;
+    };
 
     if (warp == 0) {
         // ---- copies ----
         const bool leader = elect_one();
-        const uint32_t stage_tx = 2 * Shape::kBBytes + (args.one_half ? 1 : 2) * args.a_rows * (kBlockK * 2);
         const uint32_t full_leader = map_to_rank(full0, 0);  // the pair counts on one barrier
-        const bool has_a = rank == 0 || !args.one_half;
         uint32_t stage = 0, phase = 0;
-        for (int u = pair_id; u < units && !*stop; u += pairs) {
-            const Unit t = unit(u);
+        Unit t;
+        for (int i = 0; unit_at(i, t) && !*stop; ++i) {
+            const GemmArgs& job = second(t) ? args1 : args;
+            const bool a_mn = Shape::kAMn || second(t);
+            const CUtensorMap* map_a = second(t) ? &maps.a1 : &maps.a;
+            const CUtensorMap* map_b = second(t) ? &maps.b1 : &maps.b;
+            const bool has_a = rank == 0 || !job.one_half;
+            const uint32_t stage_tx = (narrow(t) ? 1 : 2) * Shape::kBBytes +
+                                      (job.one_half ? 1 : 2) * job.a_rows * (kBlockK * 2);
             const int ma = t.m * kTile + rank * kHalfTile, nb = t.n * NT + rank * (narrow(t) ? NT / 4 : NT / 2);
             for (int kb = t.k0; kb < t.k1; ++kb) {
                 if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, stop)) break;
                 if (leader) {
                     const uint32_t bar = full_leader + 8 * stage;
                     const uint32_t sa = smem + stage * Shape::kStageBytes, sb = sa + kOperandBytes;
-                    if (rank == 0)
-                        mbar_expect_tx(full0 + 8 * stage, narrow(t) ? stage_tx - Shape::kBBytes : stage_tx);
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * stage, stage_tx);
                     const int k = kb * kBlockK;
-                    if (Shape::kAMn) {
-                        tma_load_pair(sa, &map_a, bar, ma, k);
-                        tma_load_pair(sa + kOperandBytes / 2, &map_a, bar, ma + 64, k);
+                    if (a_mn) {
+                        tma_load_pair(sa, map_a, bar, ma, k);
+                        tma_load_pair(sa + kOperandBytes / 2, map_a, bar, ma + 64, k);
                     } else if (has_a) {
-                        tma_load_pair(sa, &map_a, bar, k, ma);
+                        tma_load_pair(sa, map_a, bar, k, ma);
                     }
                     if (Shape::kBMn) {
-                        tma_load_pair(sb, &map_b, bar, nb, args.b_offset + k);
+                        tma_load_pair(sb, map_b, bar, nb, job.b_offset + k);
                         if (!narrow(t))
-                            tma_load_pair(sb + kOperandBytes / 2, &map_b, bar, nb + 64, args.b_offset + k);
+                            tma_load_pair(sb + kOperandBytes / 2, map_b, bar, nb + 64, job.b_offset + k);
                     } else {
-                        tma_load_pair(sb, &map_b, bar, k, args.b_offset + nb);
+                        tma_load_pair(sb, map_b, bar, k, job.b_offset + nb);
                     }
                 }
                 __syncwarp();
@@ -327,17 +400,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         // ---- products, issued by the pair's first CTA for both ----
         if (rank == 0) {
             const bool leader = elect_one();
-            constexpr uint32_t lead_a = Shape::kAMn ? kOperandBytes / 2 : 16;
             constexpr uint32_t lead_b = Shape::kBMn ? kOperandBytes / 2 : 16;
             // 16 deep in K: 32 bytes along a K-major row, two 8-row groups of an MN-major tile
-            constexpr uint32_t step_a = Shape::kAMn ? 2048 >> 4 : 32 >> 4;
             constexpr uint32_t step_b = Shape::kBMn ? 2048 >> 4 : 32 >> 4;
-            const uint64_t desc_a = umma_desc(smem, lead_a), desc_b = umma_desc(smem + kOperandBytes, lead_b);
+            const uint64_t desc_b = umma_desc(smem + kOperandBytes, lead_b);
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-            for (int u = pair_id; u < units && !*stop; u += pairs) {
-                const Unit t = unit(u);
+            Unit t;
+            for (int i = 0; unit_at(i, t) && !*stop; ++i) {
                 if (t.k0 == t.k1) continue;
-                const uint32_t idesc = narrow(t) ? args.idesc - ((NT / 2 >> 3) << 17) : args.idesc;
+                const bool a_mn = Shape::kAMn || second(t);
+                const uint32_t step_a = a_mn ? 2048 >> 4 : 32 >> 4;
+                const uint64_t desc_a = umma_desc(smem, a_mn ? kOperandBytes / 2 : 16);
+                const uint32_t whole = second(t) ? args1.idesc : args.idesc;
+                const uint32_t idesc = narrow(t) ? whole - ((NT / 2 >> 3) << 17) : whole;
+                const int k_ext = second(t) ? rows : k_ext0;
                 if (!mbar_wait(acc_empty0 + 8 * acc, acc_phase ^ 1, stop)) break;
                 tc_fence_after();
                 bool ok = true;
@@ -372,7 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         const uint32_t srow = lane * 128, sxor = lane & 7;
         const uint32_t empty_leader = map_to_rank(acc_empty0, 0);
         float scale = 1.0f;
-        if (EPI == kEpiOut16 && args.inv_scale) scale = __ldg(args.inv_scale);
+        if ((EPI == kEpiOut16 || EPI == kEpiGrads) && args.inv_scale) scale = __ldg(args.inv_scale);
         uint32_t acc = 0, acc_phase = 0;
         // This warp has read its part of the accumulator.
         auto release = [&] {
@@ -381,8 +457,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             if (lane == 0) mbar_arrive_cluster(empty_leader + 8 * acc);
             if ((acc ^= 1) == 0) acc_phase ^= 1;
         };
-        for (int u = pair_id; u < units; u += pairs) {
-            const Unit t = unit(u);
+        Unit t;
+        for (int i = 0; unit_at(i, t); ++i) {
             if (t.k0 == t.k1) continue;
             if constexpr (EPI == kEpiFew) {
                 if (!mbar_wait(acc_full0 + 8 * acc, acc_phase, stop)) break;
@@ -396,6 +472,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 continue;
             }
             const int row0 = t.m * kTile + rank * kHalfTile + q * 32, row = row0 + lane;
+            const int m_ext = second(t) ? args1.m_extent : m_ext0;
+            const bool out16 = EPI == kEpiOut16 || second(t);
+            const CUtensorMap* map_out = second(t) ? &maps.out1 : &maps.out;
             const int width = narrow(t) ? NT / 4 : NT / 2;  // columns of this warp's half
             const int col0 = t.n * NT + h * width;
             // a warp whose rows are all past the end has nothing to write, except that dz is
@@ -448,7 +527,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                             if (col0 + tcol < args.n_extent) args.zt[row] = z;
                         }
                         fold_pairs<32>(m, s, v, max_of<32>(m, v), kLog2e);
-                    } else if (EPI == kEpiGradZ || EPI == kEpiOut16) {
+                    } else if (EPI == kEpiGradZ || out16) {
                         float v[32];
                         if (EPI == kEpiGradZ) {
 #pragma unroll
@@ -493,7 +572,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                             // a box that starts past the edge is not stored at all
                             const int x = col0 + 64 * (c >> 1);
                             if (lane == 0 && (EPI == kEpiGradZ ? row0 < args.rows : x < args.n_extent))
-                                tma_store(&map_out, staging, x, args.out_row + row0);
+                                tma_store(map_out, staging, x, (second(t) ? args1 : args).out_row + row0);
                             if (lane == 0) tma_store_commit();
                         }
                     } else {
@@ -509,9 +588,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                             const int y = t.slab * args.slab_rows + row0;
                             if (cc < args.n_extent) {
                                 if (args.add)
-                                    tma_reduce_add(&map_out, staging, cc, y);
+                                    tma_reduce_add(map_out, staging, cc, y);
                                 else
-                                    tma_store(&map_out, staging, cc, y);
+                                    tma_store(map_out, staging, cc, y);
                             }
                             tma_store_commit();
                         }
@@ -533,7 +612,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         const uint64_t t0 = global_ns();
         while (global_ns() - t0 < 2000000) __nanosleep(1000);
         if (threadIdx.x == 0) args.meta[kMetaStop] = 1;
-        if (EPI == kEpiOut16) {
+        if (EPI == kEpiOut16 || EPI == kEpiGrads) {
             const int64_t per = (args.out_elems + gridDim.x - 1) / gridDim.x;
             const int64_t e0 = per * blockIdx.x, e1 = min(args.out_elems, e0 + per);
             for (int64_t i = e0 + threadIdx.x; i < e1; i += kGemmThreads)
@@ -835,18 +914,27 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t packed_ld(int64_t D) { return round_up(D, 64); }
 
 // K pieces of the hidden gradient, whose tiles are few (2048 x 2048: 64 for 74 CTA pairs;
-// 1 x 4096: 16): as many as fill the CTA pairs best, at least
-// 8 blocks deep each and slabs of at most 64 MB in all (one slab is needed anyway).
-int choose_splits(int64_t tiles, int64_t kb, int64_t slab_bytes, int pairs) {
-    int best = 1;
-    double best_use = 0.0;
-    for (int s = 1; s <= 64; ++s) {
-        if (s > 1 && (kb / s < 8 || slab_bytes * s > (64 << 20))) break;
-        const int64_t units = tiles * s;
-        const double use = (double)units / (double)((units + pairs - 1) / pairs * pairs);
-        if (use > best_use * 1.02) best = s, best_use = use;
-    }
-    return best;
+// 1 x 4096: 16).  The end of GradsWalk's schedule is reckoned in blocks for each number of
+// pieces, with the slabs' traffic (a block's time moves about 2 MB through HBM): the fewest
+// pieces within 2 % of the earliest end, at least 8 blocks deep each, slabs of at most
+// 64 MB in all (one slab is needed anyway).
+int choose_splits(int64_t tiles, int64_t kb, int64_t weight_units, int64_t weight_blocks, int64_t slab_bytes,
+                  int64_t pairs) {
+    const int64_t cost = weight_unit_cost((int)std::min<int64_t>(weight_blocks, 1 << 20));
+    auto end = [&](int64_t s) {
+        const int64_t units = tiles * s, depth = (kb + s - 1) / s;
+        const int64_t busy = units % pairs, rounds = busy ? depth / cost : 0;
+        const int64_t ahead = std::min(weight_units, rounds * (pairs - busy));
+        const int64_t longs = units / pairs * depth + (busy ? std::max(depth, rounds * cost) : 0);
+        const int64_t rest = (weight_units - ahead + pairs - 1) / pairs;
+        return (double)(longs + rest * cost) + (double)(slab_bytes * s) * 1e-6;
+    };
+    auto fits = [&](int64_t s) { return s == 1 || (kb / s >= 8 && slab_bytes * s <= (64 << 20)); };
+    double earliest = end(1);
+    for (int s = 2; s <= 64 && fits(s); ++s) earliest = std::min(earliest, end(s));
+    for (int s = 1; s <= 64 && fits(s); ++s)
+        if (end(s) <= 1.02 * earliest) return s;
+    return 1;
 }
 
 struct BwdPlan {
@@ -856,7 +944,7 @@ struct BwdPlan {
     int64_t coef_off, slab_off, dz_off, bytes;
 };
 
-BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidden, int pairs) {
+BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidden, bool want_weight, int pairs) {
     BwdPlan p;
     const int64_t all = round_up(V, kTile);
     // 512 MB of dz by default: the hidden gradient is added to once per piece
@@ -864,8 +952,10 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidd
     p.chunk = std::min(all, std::max<int64_t>(kTile, chunk / kTile * kTile));
     p.slab_rows = round_up(N, 32);  // a warp's box of rows
     const int64_t slab = p.slab_rows * packed_ld(Dp) * 4;
-    p.splits = want_hidden ? choose_splits(((N + kTile - 1) / kTile) * ((Dp + kTile - 1) / kTile),
-                                           p.chunk / kBlockK, slab, pairs)
+    const int64_t dt = (Dp + kTile - 1) / kTile;
+    p.splits = want_hidden ? choose_splits((N + kTile - 1) / kTile * dt, p.chunk / kBlockK,
+                                           want_weight ? p.chunk / kTile * dt : 0, (N + kBlockK - 1) / kBlockK,
+                                           slab, pairs)
                            : 0;
     p.coef_off = 256;
     p.slab_off = p.coef_off + round_up(2 * N * 4, 256);
@@ -886,8 +976,8 @@ int staged_rows(int64_t rows) { return rows >= kHalfTile ? kHalfTile : (int)roun
 int group_rows(int64_t k) { return k <= 4096 ? 16 : 8; }
 
 template <int EPI, int NT = kTile>
-int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, GemmArgs args,
-                   int64_t units, bool bf16, cudaStream_t stream, const char* what) {
+int launch_product(const Maps& maps, GemmArgs args, GemmArgs args1, int64_t units, bool bf16,
+                   cudaStream_t stream, const char* what) {
     auto kern = bf16 ? product_kernel<EPI, true, NT> : product_kernel<EPI, false, NT>;
     constexpr uint32_t smem = GemmShape<EPI, NT>::kSmem;
     // once per kernel and device (concurrent first calls set the same value)
@@ -900,9 +990,10 @@ int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
         if (dev <= 63) ready[bf16].fetch_or(bit, std::memory_order_release);
     }
     args.group = group_rows(args.k_extent < 0 ? args.rows : args.k_extent);
+    args1.group = group_rows(args1.rows);
     const int64_t pairs = std::max<int64_t>(1, std::min<int64_t>(units, sm_count() / 2));
     LaunchCfg lc(dim3((unsigned)(2 * pairs)), dim3(kGemmThreads), smem, stream);
-    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, a, b, out, args));
+    FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, maps, args, args1));
     return check_launch(what);
 }
 
@@ -1011,7 +1102,7 @@ int check_call(Call* c, const uint16_t* hidden, int64_t rows_per_group, int64_t 
 using namespace fl;
 
 extern "C" int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int pack, int64_t vocab_chunk,
-                                    int want_hidden, int64_t* state, int64_t* forward, int64_t* backward) {
+                                    int want, int64_t* state, int64_t* forward, int64_t* backward) {
     clear_error();
     const char* what = "fl_linear_loss_sizes";
     Call c;
@@ -1022,7 +1113,7 @@ extern "C" int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int pack, i
                "%s: bad arguments", what);
     *state = lay_state(nullptr, N, D, pack).bytes;
     *forward = fwd_bytes(N, V);
-    *backward = plan_bwd(N, V, c.Dp, vocab_chunk, want_hidden != 0, sm_count() / 2).bytes;
+    *backward = plan_bwd(N, V, c.Dp, vocab_chunk, want & 1, want & 2, sm_count() / 2).bytes;
     return FL_OK;
 }
 
@@ -1082,7 +1173,8 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group
                                   : reinterpret_cast<float*>(reinterpret_cast<char*>(zt) + round_up(N * 4, 256));
     const bool bf16 = dtype == 1, exchanged = N <= kFewRows;
     const int64_t few_cols = N <= 32 ? 32 : N <= 64 ? 64 : 128;
-    CUtensorMap h_map, w_map;
+    Maps maps = {};  // the rows of hidden, or of weight where they are exchanged, as A
+    CUtensorMap &h_map = exchanged ? maps.b : maps.a, &w_map = exchanged ? maps.a : maps.b;
     if (int st = make_tensor_map(&h_map, kMap16[dtype], 2, h, c.Dp, N, ldh, kBlockK,
                                  exchanged ? (int)few_cols / 2 : kHalfTile))
         return st;
@@ -1105,13 +1197,13 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group
     g.zt = zt;
     int st;
     if (!exchanged)
-        st = launch_product<kEpiStats>(h_map, w_map, h_map, g, ((N + kTile - 1) / kTile) * tiles_v, bf16, s, what);
+        st = launch_product<kEpiStats>(maps, g, {}, ((N + kTile - 1) / kTile) * tiles_v, bf16, s, what);
     else if (few_cols == 32)
-        st = launch_product<kEpiFew, 32>(w_map, h_map, h_map, g, tiles_v, bf16, s, what);
+        st = launch_product<kEpiFew, 32>(maps, g, {}, tiles_v, bf16, s, what);
     else if (few_cols == 64)
-        st = launch_product<kEpiFew, 64>(w_map, h_map, h_map, g, tiles_v, bf16, s, what);
+        st = launch_product<kEpiFew, 64>(maps, g, {}, tiles_v, bf16, s, what);
     else
-        st = launch_product<kEpiFew, 128>(w_map, h_map, h_map, g, tiles_v, bf16, s, what);
+        st = launch_product<kEpiFew, 128>(maps, g, {}, tiles_v, bf16, s, what);
     if (st) return st;
     const bool wide = pieces > 64 && N <= 8ll * sm_count();
     auto finish = wide ? finish_forward_kernel<8> : finish_forward_kernel<1>;
@@ -1149,7 +1241,7 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     FL_REQUIRE(aligned_to(grad, 4) && aligned_to(workspace, 256), "%s: misaligned buffer", what);
     if (int st = bind_device(stream, workspace)) return st;
     const int pairs = sm_count() / 2;
-    const BwdPlan plan = plan_bwd(N, V, Dp, vocab_chunk, grad_hidden != nullptr, pairs);
+    const BwdPlan plan = plan_bwd(N, V, Dp, vocab_chunk, grad_hidden != nullptr, grad_weight != nullptr, pairs);
     FL_REQUIRE(workspace_bytes >= plan.bytes, "%s: workspace of %lld bytes, %lld needed", what,
                (long long)workspace_bytes, (long long)plan.bytes);
     FL_REQUIRE(plan.slab_rows * std::max(plan.splits, 1) <= kMaxExtent, "%s: shape too large", what);
@@ -1172,24 +1264,25 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
         inv_scale = ca = cb = nullptr;
     }
     // operand and output views: hidden and weight by rows and by columns, dz both ways
-    CUtensorMap h_k, w_k, dz_out, dz_mn, h_mn, dw_out, dz_k, w_mn, slab_out;
+    Maps dz_maps = {}, dw_maps = {}, dh_maps = {};
     const CUtensorMapDataType t16 = kMap16[dtype];
     const int a_rows = staged_rows(N);
-    if (int st = make_tensor_map(&h_k, t16, 2, h, Dp, N, ldh, kBlockK, a_rows)) return st;
-    if (int st = make_tensor_map(&w_k, t16, 2, weight, Dp, V, ldw, kBlockK, kHalfTile)) return st;
-    if (int st = make_tensor_map(&dz_out, t16, 2, dz, plan.chunk, N, plan.chunk, 64, 32)) return st;
+    if (int st = make_tensor_map(&dz_maps.a, t16, 2, h, Dp, N, ldh, kBlockK, a_rows)) return st;
+    if (int st = make_tensor_map(&dz_maps.b, t16, 2, weight, Dp, V, ldw, kBlockK, kHalfTile)) return st;
+    if (int st = make_tensor_map(&dz_maps.out, t16, 2, dz, plan.chunk, N, plan.chunk, 64, 32)) return st;
     if (grad_weight) {
-        if (int st = make_tensor_map(&dz_mn, t16, 2, dz, plan.chunk, N, plan.chunk, 64, kBlockK)) return st;
-        if (int st = make_tensor_map(&h_mn, t16, 2, h, Dp, N, ldh, 64, kBlockK)) return st;
-        if (int st = make_tensor_map(&dw_out, t16, 2, grad_weight, Dp, V, Dp, 64, 32)) return st;
+        if (int st = make_tensor_map(&dw_maps.a, t16, 2, dz, plan.chunk, N, plan.chunk, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&dw_maps.b, t16, 2, h, Dp, N, ldh, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&dw_maps.out, t16, 2, grad_weight, Dp, V, Dp, 64, 32)) return st;
     }
     if (grad_hidden) {
-        if (int st = make_tensor_map(&dz_k, t16, 2, dz, plan.chunk, N, plan.chunk, kBlockK, a_rows)) return st;
-        if (int st = make_tensor_map(&w_mn, t16, 2, weight, Dp, V, ldw, 64, kBlockK)) return st;
-        if (int st = make_tensor_map(&slab_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, slabs, Dp,
+        if (int st = make_tensor_map(&dh_maps.a, t16, 2, dz, plan.chunk, N, plan.chunk, kBlockK, a_rows)) return st;
+        if (int st = make_tensor_map(&dh_maps.b, t16, 2, weight, Dp, V, ldw, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&dh_maps.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, slabs, Dp,
                                      plan.slab_rows * plan.splits, packed_ld(D), 32, 32))
             return st;
     }
+    if (grad_hidden && grad_weight) dh_maps.a1 = dw_maps.a, dh_maps.b1 = dw_maps.b, dh_maps.out1 = dw_maps.out;
     GemmArgs base = {};
     base.rows = (int)N;
     base.packed = pack == kPackKept;
@@ -1214,34 +1307,39 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
         g.grad = grad;
         g.reduce = reduce;
         g.z_loss = z_loss;
-        if (int st = launch_product<kEpiGradZ>(h_k, w_k, dz_out, g, mt * ct, bf16, s, what)) return st;
-        if (grad_weight) {
-            g = base;
-            g.m_extent = (int)cv;
-            g.n_extent = (int)Dp;
-            g.k_extent = -1;
-            g.out_row = (int)v0;
-            g.idesc = umma_idesc(bf16, true, true);
-            g.a_rows = kHalfTile;
-            g.one_half = 0;
-            g.inv_scale = inv_scale;
-            g.out = grad_weight;
-            g.out_elems = V * Dp;
-            if (int st = launch_product<kEpiOut16>(dz_mn, h_mn, dw_out, g, ct * dt, bf16, s, what)) return st;
-        }
-        if (grad_hidden) {
-            g = base;
-            g.m_extent = -1;
-            g.n_extent = (int)Dp;
-            g.k_extent = (int)cv;
-            g.b_offset = (int)v0;
-            g.splits = plan.splits;
-            g.slab_rows = (int)plan.slab_rows;
-            g.add = v0 > 0;
-            g.idesc = umma_idesc(bf16, false, true);
-            if (int st = launch_product<kEpiSlab>(dz_k, w_mn, slab_out, g, mt * dt * plan.splits, bf16, s, what))
-                return st;
-        }
+        if (int st = launch_product<kEpiGradZ>(dz_maps, g, {}, mt * ct, bf16, s, what)) return st;
+        GemmArgs w = base;  // the weight gradient
+        w.m_extent = (int)cv;
+        w.n_extent = (int)Dp;
+        w.k_extent = -1;
+        w.out_row = (int)v0;
+        w.idesc = umma_idesc(bf16, true, true);
+        w.a_rows = kHalfTile;
+        w.one_half = 0;
+        w.inv_scale = inv_scale;
+        w.out = grad_weight;
+        w.out_elems = V * Dp;
+        g = base;  // the hidden gradient
+        g.m_extent = -1;
+        g.n_extent = (int)Dp;
+        g.k_extent = (int)cv;
+        g.b_offset = (int)v0;
+        g.splits = plan.splits;
+        g.slab_rows = (int)plan.slab_rows;
+        g.add = v0 > 0;
+        g.idesc = umma_idesc(bf16, false, true);
+        g.inv_scale = inv_scale;
+        g.out = grad_weight;
+        g.out_elems = V * Dp;
+        const int64_t w_units = ct * dt, h_units = mt * dt * plan.splits;
+        int st = FL_OK;
+        if (grad_weight && grad_hidden)
+            st = launch_product<kEpiGrads>(dh_maps, g, w, w_units + h_units, bf16, s, what);
+        else if (grad_weight)
+            st = launch_product<kEpiOut16>(dw_maps, w, {}, w_units, bf16, s, what);
+        else
+            st = launch_product<kEpiSlab>(dh_maps, g, {}, h_units, bf16, s, what);
+        if (st) return st;
     }
     if (grad_hidden) {
         const int64_t groups = N * ((D + 3) / 4);

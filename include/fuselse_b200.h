@@ -378,13 +378,14 @@ int fl_sparse_f32_bwd_workspace(int64_t num_nodes, int64_t batch, int64_t num_un
  *   taken to grad_hidden (N, D) dense, zero in rows left out, and grad_weight
  *   (V, Dp) dense; either may be NULL.  A target outside [0, V) contributes no
  *   one-hot term.  Sums run in a fixed order: equal calls give equal bits.
- * fl_linear_loss_sizes: bytes of state and of the two workspaces (256-byte
+ * fl_linear_loss_sizes: bytes of state and of the two workspaces, the backward's
+ *   for the gradients in `want` (1: hidden, 2: weight, 3: both) (256-byte
  *   aligned, contents undefined on entry, one call in flight each).
  * Waits between the kernels' own copies and products end after 4 s at most;
  * the call's outputs are NaN then.
  * ---------------------------------------------------------------------- */
 int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int pack, int64_t vocab_chunk,
-                         int want_hidden, int64_t* state, int64_t* forward, int64_t* backward);
+                         int want, int64_t* state, int64_t* forward, int64_t* backward);
 int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group, int64_t group_stride,
                        int64_t row_stride, const uint16_t* weight, int64_t ldw, int dtype,
                        const int64_t* target, int pack, int64_t ignore_index, int64_t N, int64_t V,
