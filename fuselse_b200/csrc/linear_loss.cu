@@ -155,15 +155,14 @@ struct Schedule {
     }
 };
 
-// kEpiGrads: the long units of the hidden gradient go to the pairs in turn, first; the
-// last round of them leaves some pairs out (64 units for 74 pairs), and those run ahead on
-// the weight gradient's units meanwhile; then all pairs share the rest in turn.
-
 // What a weight-gradient unit of `blocks` K blocks costs, in blocks: its 256 columns are
 // stored beside the next unit's products, which cannot take less than about 6 of them
 // (4 x 6416 x 34866: 2 us a unit where a block of the hidden gradient takes 0.4).
 __host__ __device__ constexpr int weight_unit_cost(int blocks) { return blocks + 2 > 6 ? blocks + 2 : 6; }
 
+// kEpiGrads: the long units of the hidden gradient go to the pairs in turn, first; the
+// last round of them leaves some pairs out (64 units for 74 pairs), and those run ahead on
+// the weight gradient's units meanwhile; then all pairs share the rest in turn.
 struct GradsWalk {
     int pair, pairs, longs, shorts, busy, ahead, mine_long, mine_ahead;
     __device__ __forceinline__ GradsWalk(int pair_, int pairs_, int longs_, int long_blocks, int shorts_,
