@@ -19,7 +19,9 @@ Reference bindings replaced (file:line):
 Additions without a reference counterpart: batched_logsumexp_q16_i32,
 lse_partial, lse_combine, sparse_log_weights, sparse_parent_index,
 sparse_backward_float, selective_logsoftmax_* (fused target gather + LSE),
-row_layout / *_strided (rows read in place) and logsumexp_dim* (dim != -1).
+row_layout / *_strided (rows read in place), logsumexp_dim* (dim != -1),
+linear_loss_* (losses from hidden states and the output projection) and
+topk_distill_* (distillation from a teacher's top logits).
 """
 from __future__ import annotations
 
