@@ -1060,7 +1060,8 @@ struct Call {
 // The checks that both directions share; forms the row layout.
 int check_call(Call* c, const uint16_t* hidden, int64_t rows_per_group, int64_t group_stride, int64_t row_stride,
                const uint16_t* weight, int64_t ldw, int dtype, const int64_t* target, int pack, int64_t N,
-               int64_t V, int64_t D, int reduce, const void* state, int64_t state_bytes, const char* what) {
+               int64_t V, int64_t D, int reduce, float z_loss, const void* state, int64_t state_bytes,
+               const char* what) {
     FL_REQUIRE(N >= 0 && V >= 1 && D >= 1, "%s: bad shape (%lld, %lld, %lld)", what, (long long)N, (long long)V,
                (long long)D);
     FL_REQUIRE(dtype == 0 || dtype == 1, "%s: dtype must be 0 (fp16) or 1 (bf16)", what);
@@ -1071,6 +1072,7 @@ int check_call(Call* c, const uint16_t* hidden, int64_t rows_per_group, int64_t 
     FL_REQUIRE(std::max({tn * tv, tv * td, tn * td}) <= INT32_MAX / 64, "%s: shape too large", what);
     FL_REQUIRE(pack >= kPackNone && pack <= kPackKept, "%s: unknown packing %d", what, pack);
     FL_REQUIRE(reduce >= kLogp && reduce <= kMean, "%s: unknown reduction %d", what, reduce);
+    FL_REQUIRE(reduce != kLogp || z_loss == 0.0f, "%s: z_loss belongs to a loss (reduce 1 to 3)", what);
     FL_REQUIRE(reduce < kSum || pack == kPackKept, "%s: a reduced loss needs packing 2", what);
     c->rows = RowMap::dense(D);
     c->ldh = D;
@@ -1106,7 +1108,7 @@ extern "C" int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int pack, i
     const char* what = "fl_linear_loss_sizes";
     Call c;
     if (int st = check_call(&c, nullptr, -1, 0, 0, nullptr, round_up(std::max<int64_t>(D, 1), 8), 0, nullptr, pack,
-                            0, V, D, kLogp, nullptr, 0, what))
+                            0, V, D, kLogp, 0.0f, nullptr, 0, what))
         return st;
     FL_REQUIRE(N >= 0 && N <= kMaxExtent && vocab_chunk >= 0 && state && forward && backward,
                "%s: bad arguments", what);
@@ -1143,7 +1145,7 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group
     const char* what = "fl_linear_loss_fwd";
     Call c;
     if (int st = check_call(&c, hidden, rows_per_group, group_stride, row_stride, weight, ldw, dtype, target, pack,
-                            N, V, D, reduce, state, state_bytes, what))
+                            N, V, D, reduce, z_loss, state, state_bytes, what))
         return st;
     if (N == 0) return FL_OK;
     FL_REQUIRE(hidden && out && workspace, "%s: NULL buffer", what);
@@ -1223,7 +1225,7 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     const char* what = "fl_linear_loss_bwd";
     Call c;
     if (int st = check_call(&c, hidden, rows_per_group, group_stride, row_stride, weight, ldw, dtype, target, pack,
-                            N, V, D, reduce, state, state_bytes, what))
+                            N, V, D, reduce, z_loss, state, state_bytes, what))
         return st;
     FL_REQUIRE(vocab_chunk >= 0, "%s: vocab_chunk is negative", what);
     if (!grad_hidden && !grad_weight) return FL_OK;

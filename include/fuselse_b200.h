@@ -364,7 +364,7 @@ int fl_sparse_f32_bwd_workspace(int64_t num_nodes, int64_t batch, int64_t num_un
  *   2: only the rows whose target differs from ignore_index are copied, in
  *      order; the others take no part in any product.
  * fl_linear_loss_fwd writes by `reduce`, with lse the row's log-sum-exp,
- *   0: out[row] = z[row, target] - lse                       (log-probabilities)
+ *   0: out[row] = z[row, target] - lse                       (log-probabilities; z_loss 0)
  *   1: out[row] = lse - z[row, target] + z_loss * lse^2, 0 for rows left out
  *   2, 3 (pack 2): out[0] = the sum of those, its mean over the rows kept
  *      (0 / 0 if none)

@@ -99,7 +99,7 @@ def _fwd(**kw):
 @pytest.mark.parametrize("kw,message", [
     (dict(N=-1), "bad shape"), (dict(V=0), "bad shape"), (dict(D=0), "bad shape"),
     (dict(dtype=2), "dtype"), (dict(pack=3), "packing"), (dict(reduce=4), "reduction"),
-    (dict(reduce=3), "needs packing 2"), (dict(N=1 << 31), "too large"), (dict(D=1 << 21, ldw=1 << 21), "too large"),
+    (dict(reduce=3), "needs packing 2"), (dict(z=1e-3), "z_loss belongs"), (dict(N=1 << 31), "too large"), (dict(D=1 << 21, ldw=1 << 21), "too large"),
     (dict(N=1 << 30, V=1 << 30), "too large"),
     (dict(ldw=60), "weight rows"), (dict(ldw=68), "weight rows"), (dict(weight=8200), "weight rows"),
     (dict(D=60), "unpacked hidden"), (dict(rpg=4, rs=60), "unpacked hidden"), (dict(rpg=2, rs=64), "unpacked hidden"),
@@ -129,6 +129,7 @@ def _bwd(**kw):
 
 @pytest.mark.parametrize("kw,message", [
     (dict(N=-1), "bad shape"), (dict(dtype=-1), "dtype"), (dict(reduce=2), "needs packing 2"),
+    (dict(z=-1.0), "z_loss belongs"),
     (dict(chunk=-1), "vocab_chunk"), (dict(grad=None), "NULL"), (dict(ws=None), "NULL"), (dict(hidden=None), "NULL"),
     (dict(gw=131080), "misaligned"), (dict(gh=65540), "misaligned"), (dict(grad=2050), "misaligned"),
     (dict(ws=262152), "misaligned"),
