@@ -719,21 +719,22 @@ __global__ void __launch_bounds__(256) copy_rows16_kernel(const uint16_t* __rest
 // ---------------------------------------------------------------------------
 // Forward: merge a row's pieces, form its value, reduce
 // ---------------------------------------------------------------------------
-// WARPS warps of a CTA share a row: all eight for long rows that fit the SMs at once
-// (6061 rows of 600 pieces: 28 us that way, 8 us a warp to a row).
+// WARPS warps of a CTA share a row: one of 8, all 8 for long rows that fit the SMs at once
+// (6061 rows of 600 pieces: 28 us that way, 8 us a warp to a row), 32 for few rows of
+// thousands of pieces (1 x 128256: 4008).  Bound by the latency of a row's loads and merges.
 template <int WARPS>
-__global__ void __launch_bounds__(256) finish_forward_kernel(
+__global__ void __launch_bounds__(WARPS > 8 ? WARPS * 32 : 256) finish_forward_kernel(
     const float2* __restrict__ part, int pieces, const float* __restrict__ zt,
     const int64_t* __restrict__ target, const int* __restrict__ pos, int* meta, int64_t N, int64_t V,
     float z_loss, int reduce, float* __restrict__ lse_out, float* values, float* __restrict__ out,
     int* err) {
-    __shared__ double sums[8];
-    __shared__ float2 states[8];
+    constexpr int kWarpsHere = WARPS > 8 ? WARPS : 8, kRows = kWarpsHere / WARPS;
+    __shared__ double sums[kWarpsHere];
+    __shared__ float2 states[kWarpsHere];
     __shared__ int last;
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int kRows = 8 / WARPS;
     const float nan = __int_as_float(0x7fc00000);
     for (int64_t row = (int64_t)blockIdx.x * kRows + warp / WARPS; row < N; row += (int64_t)gridDim.x * kRows) {
         const int64_t p = pos ? pos[row] : row;
@@ -761,13 +762,21 @@ __global__ void __launch_bounds__(256) finish_forward_kernel(
                 const float2 v = __ldg(pp + i);
                 ms_merge(m, s, v.x, v.y);
             }
-            ms_warp_allreduce(m, s);
+            // the warp's maximum first, then one rescaling and a sum
+            auto merge_lanes = [&] {
+                const float M = warp_max_nan(m);
+                s *= exp_from(m, safe_max(M));
+                m = M;
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+            };
+            merge_lanes();
             if (WARPS > 1) {
                 if (lane == 0) states[warp] = make_float2(m, s);
                 __syncthreads();
-                m = states[0].x, s = states[0].y;
-#pragma unroll
-                for (int w = 1; w < WARPS; ++w) ms_merge(m, s, states[w].x, states[w].y);
+                const float2 mine = lane < WARPS ? states[lane] : make_float2(-INFINITY, 0.0f);
+                m = mine.x, s = mine.y;
+                merge_lanes();
                 __syncthreads();
             }
             const float lse = ms_finalize(m, s, -INFINITY);
@@ -790,14 +799,14 @@ __global__ void __launch_bounds__(256) finish_forward_kernel(
     __threadfence();
     // one CTA sums all rows in a fixed order, in 64 bits (long sums of like values)
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < N; i += 256) sum += __ldcg(values + i);
+    for (int64_t i = threadIdx.x; i < N; i += kWarpsHere * 32) sum += __ldcg(values + i);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     if (lane == 0) sums[warp] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
         double total = 0.0;
-        for (int w = 0; w < 8; ++w) total += sums[w];
+        for (int w = 0; w < kWarpsHere; ++w) total += sums[w];
         if (reduce == kMean) total /= meta[kMetaRows];
         *out = static_cast<float>(total);
         meta[kMetaCount] = 0;
@@ -1206,9 +1215,10 @@ extern "C" int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group
     else
         st = launch_product<kEpiFew, 128>(maps, g, {}, tiles_v, bf16, s, what);
     if (st) return st;
-    const bool wide = pieces > 64 && N <= 8ll * sm_count();
-    auto finish = wide ? finish_forward_kernel<8> : finish_forward_kernel<1>;
-    LaunchCfg lc(dim3((unsigned)std::min<int64_t>(wide ? N : (N + 7) / 8, 32ll * sm_count())), dim3(256), 0, s);
+    const bool wide = pieces > 64 && N <= 8ll * sm_count(), widest = pieces > 1024 && N <= 2ll * sm_count();
+    auto finish = widest ? finish_forward_kernel<32> : wide ? finish_forward_kernel<8> : finish_forward_kernel<1>;
+    LaunchCfg lc(dim3((unsigned)std::min<int64_t>(wide ? N : (N + 7) / 8, 32ll * sm_count())),
+                 dim3(widest ? 1024 : 256), 0, s);
     FL_CUDA(cudaLaunchKernelEx(&lc.cfg, finish, (const float2*)part, g.pieces, (const float*)zt, target,
                                (const int*)keep.pos, keep.meta, N, V, z_loss, reduce, keep.lse, values, out,
                                err_flag));
