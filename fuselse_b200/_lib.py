@@ -68,7 +68,7 @@ SIGNATURES = {
     "fl_ipc_buffer_free": [c_int, c_void_p],
     # addresses as plain integers: these entry points are called once or twice per training step
     # of small batches, where forming typed pointers would be a good part of the call
-    "fl_linear_loss_sizes": [c_int64, c_int64, c_int64, c_int, c_int64, c_int, POINTER(c_int64),
+    "fl_linear_loss_sizes": [c_int64, c_int64, c_int64, c_int, c_int, c_int64, c_int, POINTER(c_int64),
                              POINTER(c_int64), POINTER(c_int64)],
     "fl_linear_loss_fwd": [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int,
                            c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_void_p, c_int64, c_void_p,

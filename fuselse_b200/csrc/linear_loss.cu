@@ -7,7 +7,9 @@
 //   backward  dz_iv = a_i softmax(z_i)_v - b_i [v = t_i], in pieces of the
 //             vocabulary: the product is recomputed, dz of the piece is written
 //             in 16 bits, and two more products take it to the gradients
-//             dW = dz^T hidden and dH = dz weight.
+//             dW = dz^T hidden and dH = dz weight.  With bf16 operands dW takes
+//             dz and hidden in fp16 (convert_rows_kernel): dz's eight bits are
+//             too few for the sums of often named vocabulary entries.
 //   Tokens without a target are packed away first, so every product runs over
 //   the remaining rows only.
 //
@@ -24,6 +26,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <type_traits>
 
 namespace fl {
 namespace {
@@ -50,7 +53,7 @@ enum Epi {
 };
 
 // NT: columns of a tile (256; fewer for kEpiFew).
-template <int EPI, int NT>
+template <int EPI, int NT, bool BF16>
 struct GemmShape {
     // A given as [k][m] (kEpiGrads: as its unit's kind says), B given as [k][n]
     static constexpr bool kAMn = EPI == kEpiOut16;
@@ -59,8 +62,10 @@ struct GemmShape {
     static constexpr uint32_t kBBytes = NT / 2 * kBlockK * 2;
     static constexpr uint32_t kStageBytes = kOperandBytes + kBBytes;
     // one 4 KB buffer per epilogue warp: a stage more for the operands measured 1 % faster
-    // than a second buffer (5 and 4 stages: 1 % and 6 % slower than 6)
-    static constexpr uint32_t kStaging = kStores ? kEpiWarps * kStagingBuf : 0;
+    // than a second buffer (5 and 4 stages: 1 % and 6 % slower than 6); dz has one for each type
+    // that it is stored in (128-byte rows of 64 columns: 5 stages, 0.5-1 % slower)
+    static constexpr uint32_t kBuffers = EPI == kEpiGradZ && BF16 ? 2 : kStores ? 1 : 0;
+    static constexpr uint32_t kStaging = kBuffers * kEpiWarps * kStagingBuf;
     static constexpr int kStages = (227 * 1024 - 1280 - kStaging) / kStageBytes;
     static constexpr uint32_t kSmem = kStages * kStageBytes + kStaging + 1024;
     static constexpr uint32_t kTmemCols = 2 * NT;  // two accumulators
@@ -89,11 +94,14 @@ struct GemmArgs {
     float2* part;          // [row][pieces] partial states
     int pieces;
     float* zt;
-    const float *lse, *a, *b;  // kEpiGradZ; without a and b (bf16) they are formed from
+    const float* lse;          // kEpiGradZ
     const float* grad;         // the upstream gradient
     int reduce;
     float z_loss;
-    const float* inv_scale;    // kEpiOut16 (none: 1)
+    int stores;                // dz in the operands' type (1), in fp16 for bf16 operands' dW (2)
+    const int* exponents;      // the latter: the powers of two in hidden's rows
+    float* residual;           // what the target's element of dz lost to its rounding
+    float* inv_scale;          // of fp16 dz: kEpiGradZ writes it, kEpiOut16 reads it
     void* out;             // kEpiOut16: filled with NaN when a wait ran out
     int64_t out_elems;
 };
@@ -198,6 +206,12 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return r;
 }
 
+// v rounded to the 16-bit type.
+template <bool BF16>
+__device__ __forceinline__ float round16(float v) {
+    return BF16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
+}
+
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                              uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
@@ -273,12 +287,14 @@ __device__ __forceinline__ void few_rows_piece(uint32_t addr, int row0, int v0, 
 template <int EPI, bool BF16, int NT = kTile>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     product_kernel(const __grid_constant__ Maps maps, const GemmArgs args, const GemmArgs args1) {
-    using Shape = GemmShape<EPI, NT>;
+    using Shape = GemmShape<EPI, NT, BF16>;
     constexpr int kStages = Shape::kStages;
     extern __shared__ uint8_t smem_raw[];
     __shared__ alignas(8) uint64_t bars[2 * kStages + 4];
     __shared__ uint32_t tmem_slot;
     __shared__ int stop_flag;
+    __shared__ float bigs[kEpiWarps];
+    __shared__ int leasts[kEpiWarps];
     volatile int* stop = &stop_flag;
 
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -299,12 +315,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         mbar_init_fence();
         tma_prefetch_map(&maps.a);
         tma_prefetch_map(&maps.b);
-        if (Shape::kStores) tma_prefetch_map(&maps.out);
+        if (Shape::kStores && (EPI != kEpiGradZ || (args.stores & 1))) tma_prefetch_map(&maps.out);
         if (EPI == kEpiGrads) {
             tma_prefetch_map(&maps.a1);
             tma_prefetch_map(&maps.b1);
-            tma_prefetch_map(&maps.out1);
         }
+        if (EPI == kEpiGrads || (EPI == kEpiGradZ && (args.stores & 2))) tma_prefetch_map(&maps.out1);
     }
     if (warp == 2) tmem_alloc_pair(smem_u32(&tmem_slot), Shape::kTmemCols);
     pdl_wait();
@@ -443,11 +459,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     } else if (warp >= 4) {
         // ---- epilogue: warp quarter q reads lanes (rows) 32q.., half h columns 128h.. ----
         const int q = warp & 3, h = (warp - 4) >> 2;
-        const uint32_t staging = smem + kStages * Shape::kStageBytes + (warp - 4) * kStagingBuf;
+        const uint32_t staging = smem + kStages * Shape::kStageBytes + (warp - 4) * Shape::kBuffers * kStagingBuf;
         const uint32_t srow = lane * 128, sxor = lane & 7;
         const uint32_t empty_leader = map_to_rank(acc_empty0, 0);
         float scale = 1.0f;
-        if ((EPI == kEpiOut16 || EPI == kEpiGrads) && args.inv_scale) scale = __ldg(args.inv_scale);
+        if (EPI == kEpiOut16 || EPI == kEpiGrads) scale = __ldg(args.inv_scale);
+        // dz in fp16 takes a power of two that brings the largest of its coefficients to
+        // [2^13, 2^14): it keeps its relative accuracy down to probabilities of 1e-9 of it
+        // instead of flushing them.  With bf16 operands a row also takes back the power that
+        // convert_rows_kernel gave hidden's, and the coefficients are compared after that.
+        // Every CTA looks at all rows, while the tensor cores are at its first tile: a kernel
+        // of one CTA for it took 4-5 us of its own.
+        int power = 0;
+        if (EPI == kEpiGradZ && (!BF16 || (args.stores & 2))) {
+            float big = 0.0f;
+            int least = 100;
+#pragma unroll 4
+            for (int r = threadIdx.x - 128; r < rows; r += 32 * kEpiWarps) {
+                float a, b;
+                row_coefficients(args.grad, args.reduce, args.z_loss, __ldg(args.lse + r), args.src, r, rows, a, b);
+                float most = fmaxf(fabsf(a), fabsf(b));
+                if (BF16) {
+                    const int e = __ldg(args.exponents + r);
+                    most = scalbnf(most, -e);
+                    least = min(least, e);
+                }
+                big = fmaxf(big, most);
+            }
+            big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));  // no NaN, not negative
+            least = __reduce_min_sync(0xffffffffu, least);
+            if (lane == 0) bigs[warp - 4] = big, leasts[warp - 4] = least;
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+#pragma unroll
+            for (int w = 0; w < kEpiWarps; ++w) big = fmaxf(big, bigs[w]), least = min(least, leasts[w]);
+            if (big > 0.0f && big < INFINITY) power = min(max(13 - ilogbf(big), -120), 120);
+            if (BF16) power = min(power, 126 + least);  // every row's factor is a finite power of two
+            if (blockIdx.x == 0 && threadIdx.x == 128) *args.inv_scale = scalbnf(1.0f, -power);
+        }
         uint32_t acc = 0, acc_phase = 0;
         // This warp has read its part of the accumulator.
         auto release = [&] {
@@ -480,18 +528,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             // defined (zero) on whole 64-row blocks: the weight gradient sums over those
             const bool busy = EPI == kEpiGradZ ? row0 < max(64, (rows + 63) & ~63) : row0 < m_ext;
             int64_t tcol = -1;
-            float lse = 0.0f, a = 0.0f, b = 0.0f;
+            float lse = 0.0f, a = 0.0f, b = 0.0f, factor = 0.0f;
             if ((EPI == kEpiStats || EPI == kEpiGradZ) && row < rows) {
                 tcol = __ldg(args.target + (args.src ? __ldg(args.src + row) : row));
                 tcol = tcol < 0 ? -1 : tcol - (EPI == kEpiGradZ ? args.b_offset : 0) - col0;
                 if (EPI == kEpiGradZ) {
                     lse = __ldg(args.lse + row);
-                    if (args.a) {
-                        a = __ldg(args.a + row);
-                        b = __ldg(args.b + row);
-                    } else {
-                        row_coefficients(args.grad, args.reduce, args.z_loss, lse, args.src, row, rows, a, b);
-                    }
+                    row_coefficients(args.grad, args.reduce, args.z_loss, lse, args.src, row, rows, a, b);
+                    if (!BF16) a = scalbnf(a, power), b = scalbnf(b, power);
+                    if (BF16 && (args.stores & 2)) factor = scalbnf(1.0f, power - __ldg(args.exponents + row));
                 }
             }
             if (!mbar_wait(acc_full0 + 8 * acc, acc_phase, stop)) break;
@@ -538,9 +583,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                                 v[j + 1] = o.y;
                             }
                             if (here) {
+                                float at = 0.0f;
 #pragma unroll
                                 for (int j = 0; j < 32; ++j)
-                                    if (tcol == 32 * c + j) v[j] -= b;
+                                    if (tcol == 32 * c + j) at = v[j] -= b;
+                                if (args.residual) args.residual[row] = at - round16<BF16>(at);
                             }
                             // rows and columns past the end are zero whatever was staged there
                             if (row >= rows || cc + 32 > n_ext) {
@@ -556,22 +603,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                             if (lane == 0) tma_store_wait_read<0>();
                             __syncwarp();
                         }
+                        // a row's 32 columns to a buffer, in the swizzle of the tensor map
+                        auto stage32 = [&](uint32_t buf, auto type) {
+                            constexpr bool kBf = decltype(type)::value;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t chunk = (c & 1) * 4 + j;
-                            st_shared_v4(staging + srow + ((chunk ^ sxor) << 4),
-                                         pack16<BF16>(v[8 * j], v[8 * j + 1]),
-                                         pack16<BF16>(v[8 * j + 2], v[8 * j + 3]),
-                                         pack16<BF16>(v[8 * j + 4], v[8 * j + 5]),
-                                         pack16<BF16>(v[8 * j + 6], v[8 * j + 7]));
+                            for (int j = 0; j < 4; ++j) {
+                                const uint32_t chunk = (c & 1) * 4 + j;
+                                st_shared_v4(buf + srow + ((chunk ^ sxor) << 4),
+                                             pack16<kBf>(v[8 * j], v[8 * j + 1]),
+                                             pack16<kBf>(v[8 * j + 2], v[8 * j + 3]),
+                                             pack16<kBf>(v[8 * j + 4], v[8 * j + 5]),
+                                             pack16<kBf>(v[8 * j + 6], v[8 * j + 7]));
+                            }
+                        };
+                        if (EPI != kEpiGradZ || (args.stores & 1))
+                            stage32(staging, std::integral_constant<bool, BF16>());
+                        if (EPI == kEpiGradZ && BF16 && (args.stores & 2)) {
+                            const f32x2 f2 = pair(factor, factor);
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2) {
+                                const float2 o = unpair(mul2(pair(v[j], v[j + 1]), f2));
+                                v[j] = o.x;
+                                v[j + 1] = o.y;
+                            }
+                            stage32(staging + kStagingBuf, std::false_type());
                         }
                         if ((c & 1) == 1) {
                             fence_async_smem();
                             __syncwarp();
                             // a box that starts past the edge is not stored at all
                             const int x = col0 + 64 * (c >> 1);
-                            if (lane == 0 && (EPI == kEpiGradZ ? row0 < args.rows : x < args.n_extent))
+                            if (EPI == kEpiGradZ) {
+                                if (lane == 0 && row0 < args.rows) {
+                                    if (args.stores & 1) tma_store(&maps.out, staging, x, row0);
+                                    if (BF16 && (args.stores & 2))
+                                        tma_store(&maps.out1, staging + kStagingBuf, x, row0);
+                                }
+                            } else if (lane == 0 && x < args.n_extent) {
                                 tma_store(map_out, staging, x, (second(t) ? args1 : args).out_row + row0);
+                            }
                             if (lane == 0) tma_store_commit();
                         }
                     } else {
@@ -816,57 +886,73 @@ __global__ void __launch_bounds__(WARPS > 8 ? WARPS * 32 : 256) finish_forward_k
 // ---------------------------------------------------------------------------
 // Backward: row coefficients of dz, and the hidden gradient from its slabs
 // ---------------------------------------------------------------------------
-// fp16 only: the coefficients of dz = a softmax - b onehot, scaled by a power of two
-// that brings the largest to [2^13, 2^14): fp16 keeps its relative accuracy down to
-// probabilities of 1e-9 of it instead of flushing them.  bf16 has fp32's range and
-// forms its coefficients where it uses them.  One CTA, two passes over the rows: 3-5 us up
-// to 2048 of them, bound by its latency.
-__global__ void __launch_bounds__(1024) coefficients_kernel(
-    const float* __restrict__ g, int reduce, float z_loss, const float* __restrict__ lse,
-    const int* __restrict__ src, const int* __restrict__ meta, int64_t N, float* __restrict__ a,
-    float* __restrict__ b, float* __restrict__ inv_scale) {
+// bf16 operands, where the weight gradient is wanted: hidden's rows in fp16.  bf16 has
+// fp32's range and needs no scales, but a sum over hundreds of tokens' dz h for one
+// vocabulary entry shows dz's eight bits: the worst elements of 8192 x 4096 x 128256 were
+// off by a third of the gradient's rms, with fp16's eleven bits by a twentieth (0.0017 of
+// the norm in all, what rounding the exact result gives, against 0.0024).  dz and hidden go to
+// one instruction, so both change; it costs 2.5-5 % of a training step, most of that for
+// writing dz twice.  A row is brought by a power of two to a largest element of [2^14, 2^15),
+// which is exact but for elements of 2^-29 of it and less; dz's row takes that power back.
+//
+// A warp per row, two passes, the second from L1 or L2.  Bound by memory when large
+// (6144 x 4096: 18 us, 5.5 TB/s), by latency when small (511 x 1000, 1022 x 2048: 3.6 us).
+__global__ void __launch_bounds__(256) convert_rows_kernel(
+    const uint16_t* __restrict__ h, int64_t ldh, int Dp, const int* __restrict__ src,
+    const int* __restrict__ meta, int64_t N, uint16_t* __restrict__ h16, int64_t ld16,
+    int* __restrict__ exponents) {
     pdl_wait();
     pdl_launch_dependents();
-    __shared__ float top[32];
+    const int lane = threadIdx.x & 31;
     const int64_t rows = src ? meta[kMetaRows] : N;
-    auto coef = [&](int64_t r, float& ca, float& cb) {
-        row_coefficients(g, reduce, z_loss, lse[r], src, r, rows, ca, cb);
-    };
-    float big = 0.0f;
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-        float ca, cb;
-        coef(r, ca, cb);
-        big = fmaxf(big, fmaxf(fabsf(ca), fabsf(cb)));
-    }
+    // the products run over whole blocks of 64 rows: those past the last one are zero
+    const int64_t end = min(N, max((int64_t)kBlockK, (rows + kBlockK - 1) / kBlockK * kBlockK));
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < end; r += (int64_t)gridDim.x * 8) {
+        uint4* to = reinterpret_cast<uint4*>(h16 + r * ld16);
+        if (r >= rows) {
+            for (int i = lane; i < Dp / 8; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        const uint4* from = reinterpret_cast<const uint4*>(h + r * ldh);
+        uint32_t most = 0;  // the largest magnitude's bits, two columns side by side
+        for (int i = lane; i < Dp / 8; i += 32) {
+            const uint4 v = __ldg(from + i);
+            most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                           __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+        }
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, max(most >> 16, most & 0xffffu));
+        // infinities and NaN stay what they are; a row of zeros must not set the scale of the others
+        const int e = bits >= 0x7f80u ? 0 : min(14 - (max((int)(bits >> 7), 1) - 127), 100);
+        const float scale = __int_as_float((e + 127) << 23);
+        for (int i = lane; i < Dp / 8; i += 32) {
+            const uint4 v = __ldg(from + i);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t o[4];
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = big;
-    __syncthreads();
-    big = top[threadIdx.x & 31];
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-    int e = 0;
-    if (big > 0.0f && big < INFINITY) e = min(max(14 - (ilogbf(big) + 1), -120), 120);
-    const float scale = scalbnf(1.0f, e);
-    if (threadIdx.x == 0) *inv_scale = scalbnf(1.0f, -e);
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-        float ca, cb;
-        coef(r, ca, cb);
-        a[r] = ca * scale;
-        b[r] = cb * scale;
+            for (int k = 0; k < 4; ++k)
+                o[k] = pack16<false>(__uint_as_float(w[k] << 16) * scale,
+                                     __uint_as_float(w[k] & 0xffff0000u) * scale);
+            to[i] = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        if (lane == 0) exponents[r] = e;
     }
 }
 
 // The hidden gradient: a row's slabs summed in the order of the vocabulary's K pieces, in
-// fp32, and rounded once.  Bound by the slabs' bytes (2048 x 2048: 8-10 us).
+// fp32, with what the rounding of dz took from its largest element, the target's, times
+// that weight row, and rounded once.  Bound by the slabs' bytes (2048 x 2048: 8-10 us).
 // LANES neighbouring lanes share four columns of a row, each a part of the slabs: 8 of
 // them where few columns have many slabs (49 x 176 in 64 slabs: 12.6 us with one).
 template <bool BF16, int LANES>
 __global__ void __launch_bounds__(256) finish_hidden_kernel(const float* __restrict__ slabs, int splits,
                                                             int64_t slab_elems, const int* __restrict__ pos,
                                                             const int* __restrict__ meta,
-                                                            const float* __restrict__ inv_scale, int64_t N,
-                                                            int D, int ld, uint16_t* __restrict__ out) {
+                                                            const float* __restrict__ inv_scale,
+                                                            const float* __restrict__ residual,
+                                                            const int64_t* __restrict__ target,
+                                                            const uint16_t* __restrict__ weight, int64_t ldw,
+                                                            int64_t V, int64_t N, int D, int ld,
+                                                            uint16_t* __restrict__ out) {
     pdl_wait();
     pdl_launch_dependents();
     const float scale = meta[kMetaStop] ? __int_as_float(0x7fc00000) : inv_scale ? *inv_scale : 1.0f;
@@ -898,7 +984,19 @@ __global__ void __launch_bounds__(256) finish_hidden_kernel(const float* __restr
             v.w += __shfl_xor_sync(0xffffffffu, v.w, off);
         }
         if (part != 0 || first + threadIdx.x / LANES >= total) continue;
-        if (p >= 0) v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
+        if (p >= 0) {
+            const int64_t tg = __ldg(target + row);
+            if (tg >= 0 && tg < V) {
+                const float r = __ldg(residual + p);
+                const uint2 w = __ldg(reinterpret_cast<const uint2*>(weight + tg * ldw + j));
+                auto wide16 = [](uint32_t x) {
+                    return BF16 ? __uint_as_float(x << 16) : __half2float(__ushort_as_half((unsigned short)x));
+                };
+                v.x += r * wide16(w.x & 0xffffu), v.y += r * wide16(w.x >> 16);
+                v.z += r * wide16(w.y & 0xffffu), v.w += r * wide16(w.y >> 16);
+            }
+            v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
+        }
         uint16_t* o = out + row * D + j;
         const uint32_t lo = pack16<BF16>(v.x, v.y), hi = pack16<BF16>(v.z, v.w);
         if (wide) {
@@ -949,13 +1047,14 @@ struct BwdPlan {
     int64_t chunk;      // columns of a vocabulary piece, a multiple of 256
     int splits;
     int64_t slab_rows;
-    int64_t coef_off, slab_off, dz_off, bytes;
+    int64_t exponents_off, residual_off, h16_off, slab_off, dz_off, dz16_off, bytes;
 };
 
-BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidden, bool want_weight, int pairs) {
+BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool bf16, bool want_hidden, bool want_weight,
+                 int pairs) {
     BwdPlan p;
     const int64_t all = round_up(V, kTile);
-    // 512 MB of dz by default: the hidden gradient is added to once per piece
+    // 512 MB of dz by default (of each type that is held): the hidden gradient is added to once per piece
     if (chunk <= 0) chunk = (256ll << 20) / std::max<int64_t>(N, 1);
     p.chunk = std::min(all, std::max<int64_t>(kTile, chunk / kTile * kTile));
     p.slab_rows = round_up(N, 32);  // a warp's box of rows
@@ -965,10 +1064,17 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t Dp, int64_t chunk, bool want_hidd
                                            want_weight ? p.chunk / kTile * dt : 0, (N + kBlockK - 1) / kBlockK,
                                            slab, pairs)
                            : 0;
-    p.coef_off = 256;
-    p.slab_off = p.coef_off + round_up(2 * N * 4, 256);
+    // bf16, weight gradient: the exponents, hidden in fp16 and dz in fp16; dz in the operands'
+    // type unless that is all
+    const bool convert = bf16 && want_weight;
+    const int64_t dz = round_up(N * p.chunk * 2, 256);
+    p.exponents_off = 256;
+    p.residual_off = p.exponents_off + (convert ? round_up(N * 4, 256) : 0);
+    p.h16_off = p.residual_off + (want_hidden ? round_up(N * 4, 256) : 0);
+    p.slab_off = p.h16_off + (convert ? round_up(N * packed_ld(Dp) * 2, 256) : 0);
     p.dz_off = p.slab_off + round_up(slab * p.splits, 256);
-    p.bytes = p.dz_off + round_up(N * p.chunk * 2, 256);
+    p.dz16_off = p.dz_off + (bf16 && !want_hidden ? 0 : dz);
+    p.bytes = p.dz16_off + (convert ? dz : 0);
     return p;
 }
 
@@ -987,7 +1093,7 @@ template <int EPI, int NT = kTile>
 int launch_product(const Maps& maps, GemmArgs args, GemmArgs args1, int64_t units, bool bf16,
                    cudaStream_t stream, const char* what) {
     auto kern = bf16 ? product_kernel<EPI, true, NT> : product_kernel<EPI, false, NT>;
-    constexpr uint32_t smem = GemmShape<EPI, NT>::kSmem;
+    const uint32_t smem = bf16 ? GemmShape<EPI, NT, true>::kSmem : GemmShape<EPI, NT, false>::kSmem;
     // once per kernel and device (concurrent first calls set the same value)
     static std::atomic<uint64_t> ready[2];
     int dev = 0;
@@ -1111,19 +1217,19 @@ int check_call(Call* c, const uint16_t* hidden, int64_t rows_per_group, int64_t 
 
 using namespace fl;
 
-extern "C" int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int pack, int64_t vocab_chunk,
+extern "C" int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int dtype, int pack, int64_t vocab_chunk,
                                     int want, int64_t* state, int64_t* forward, int64_t* backward) {
     clear_error();
     const char* what = "fl_linear_loss_sizes";
     Call c;
-    if (int st = check_call(&c, nullptr, -1, 0, 0, nullptr, round_up(std::max<int64_t>(D, 1), 8), 0, nullptr, pack,
+    if (int st = check_call(&c, nullptr, -1, 0, 0, nullptr, round_up(std::max<int64_t>(D, 1), 8), dtype, nullptr, pack,
                             0, V, D, kLogp, 0.0f, nullptr, 0, what))
         return st;
     FL_REQUIRE(N >= 0 && N <= kMaxExtent && vocab_chunk >= 0 && state && forward && backward,
                "%s: bad arguments", what);
     *state = lay_state(nullptr, N, D, pack).bytes;
     *forward = fwd_bytes(N, V);
-    *backward = plan_bwd(N, V, c.Dp, vocab_chunk, want & 1, want & 2, sm_count() / 2).bytes;
+    *backward = plan_bwd(N, V, c.Dp, vocab_chunk, dtype == 1, want & 1, want & 2, sm_count() / 2).bytes;
     return FL_OK;
 }
 
@@ -1252,7 +1358,7 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     FL_REQUIRE(aligned_to(grad, 4) && aligned_to(workspace, 256), "%s: misaligned buffer", what);
     if (int st = bind_device(stream, workspace)) return st;
     const int pairs = sm_count() / 2;
-    const BwdPlan plan = plan_bwd(N, V, Dp, vocab_chunk, grad_hidden != nullptr, grad_weight != nullptr, pairs);
+    const BwdPlan plan = plan_bwd(N, V, Dp, vocab_chunk, dtype == 1, grad_hidden != nullptr, grad_weight != nullptr, pairs);
     FL_REQUIRE(workspace_bytes >= plan.bytes, "%s: workspace of %lld bytes, %lld needed", what,
                (long long)workspace_bytes, (long long)plan.bytes);
     FL_REQUIRE(plan.slab_rows * std::max(plan.splits, 1) <= kMaxExtent, "%s: shape too large", what);
@@ -1261,29 +1367,39 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
     const int64_t ldh = pack == kPackNone ? c.ldh : packed_ld(D);
     char* ws = static_cast<char*>(workspace);
     float* inv_scale = reinterpret_cast<float*>(ws);
-    float* ca = reinterpret_cast<float*>(ws + plan.coef_off);
-    float* cb = ca + N;
+    int* exponents = reinterpret_cast<int*>(ws + plan.exponents_off);
+    float* residual = reinterpret_cast<float*>(ws + plan.residual_off);
+    uint16_t* h16 = reinterpret_cast<uint16_t*>(ws + plan.h16_off);
     float* slabs = reinterpret_cast<float*>(ws + plan.slab_off);
     uint16_t* dz = reinterpret_cast<uint16_t*>(ws + plan.dz_off);
-    const bool bf16 = dtype == 1;
-    if (!bf16) {
-        LaunchCfg lc(dim3(1), dim3(1024), 0, s);
-        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, coefficients_kernel, grad, reduce, z_loss, (const float*)keep.lse,
-                                   (const int*)keep.src, (const int*)keep.meta, N, ca, cb, inv_scale));
+    uint16_t* dz16 = reinterpret_cast<uint16_t*>(ws + plan.dz16_off);
+    const bool bf16 = dtype == 1, convert = bf16 && grad_weight;
+    if (convert) {
+        LaunchCfg lc(dim3((unsigned)std::min<int64_t>((N + 7) / 8, 8ll * sm_count())), dim3(256), 0, s);
+        FL_CUDA(cudaLaunchKernelEx(&lc.cfg, convert_rows_kernel, h, ldh, (int)Dp, (const int*)keep.src,
+                                   (const int*)keep.meta, N, h16, packed_ld(D), exponents));
         if (int st = check_launch(what)) return st;
-    } else {
-        inv_scale = ca = cb = nullptr;
     }
+    // dz for the hidden gradient, and its scale; for the weight gradient the same or in fp16
+    const float* h_inv_scale = bf16 ? nullptr : inv_scale;
+    const uint16_t* dz_w = convert ? dz16 : dz;
+    const uint16_t* h_w = convert ? h16 : h;
+    const int64_t ldh_w = convert ? packed_ld(D) : ldh;
+    const CUtensorMapDataType w16 = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     // operand and output views: hidden and weight by rows and by columns, dz both ways
     Maps dz_maps = {}, dw_maps = {}, dh_maps = {};
     const CUtensorMapDataType t16 = kMap16[dtype];
     const int a_rows = staged_rows(N);
     if (int st = make_tensor_map(&dz_maps.a, t16, 2, h, Dp, N, ldh, kBlockK, a_rows)) return st;
     if (int st = make_tensor_map(&dz_maps.b, t16, 2, weight, Dp, V, ldw, kBlockK, kHalfTile)) return st;
-    if (int st = make_tensor_map(&dz_maps.out, t16, 2, dz, plan.chunk, N, plan.chunk, 64, 32)) return st;
+    const bool store_dz = !bf16 || grad_hidden;
+    if (store_dz)
+        if (int st = make_tensor_map(&dz_maps.out, t16, 2, dz, plan.chunk, N, plan.chunk, 64, 32)) return st;
+    if (convert)
+        if (int st = make_tensor_map(&dz_maps.out1, w16, 2, dz16, plan.chunk, N, plan.chunk, 64, 32)) return st;
     if (grad_weight) {
-        if (int st = make_tensor_map(&dw_maps.a, t16, 2, dz, plan.chunk, N, plan.chunk, 64, kBlockK)) return st;
-        if (int st = make_tensor_map(&dw_maps.b, t16, 2, h, Dp, N, ldh, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&dw_maps.a, w16, 2, dz_w, plan.chunk, N, plan.chunk, 64, kBlockK)) return st;
+        if (int st = make_tensor_map(&dw_maps.b, w16, 2, h_w, Dp, N, ldh_w, 64, kBlockK)) return st;
         if (int st = make_tensor_map(&dw_maps.out, t16, 2, grad_weight, Dp, V, Dp, 64, 32)) return st;
     }
     if (grad_hidden) {
@@ -1313,18 +1429,20 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
         g.target = target;
         g.src = keep.src;
         g.lse = keep.lse;
-        g.a = ca;
-        g.b = cb;
         g.grad = grad;
         g.reduce = reduce;
         g.z_loss = z_loss;
+        g.stores = (store_dz ? 1 : 0) | (convert ? 2 : 0);
+        g.exponents = exponents;
+        g.inv_scale = inv_scale;
+        g.residual = grad_hidden ? residual : nullptr;
         if (int st = launch_product<kEpiGradZ>(dz_maps, g, {}, mt * ct, bf16, s, what)) return st;
         GemmArgs w = base;  // the weight gradient
         w.m_extent = (int)cv;
         w.n_extent = (int)Dp;
         w.k_extent = -1;
         w.out_row = (int)v0;
-        w.idesc = umma_idesc(bf16, true, true);
+        w.idesc = umma_idesc(false, true, true);  // fp16 operands, whatever the gradient's type
         w.a_rows = kHalfTile;
         w.one_half = 0;
         w.inv_scale = inv_scale;
@@ -1362,7 +1480,8 @@ extern "C" int fl_linear_loss_bwd(const float* grad, const uint16_t* hidden, int
         LaunchCfg lc(dim3((unsigned)grid), dim3(256), 0, s);
         FL_CUDA(cudaLaunchKernelEx(&lc.cfg, kern, (const float*)slabs, plan.splits,
                                    plan.slab_rows * packed_ld(D), (const int*)keep.pos, (const int*)keep.meta,
-                                   (const float*)inv_scale, N, (int)D, (int)packed_ld(D), grad_hidden));
+                                   h_inv_scale, (const float*)residual, target, weight, ldw, V, N, (int)D,
+                                   (int)packed_ld(D), grad_hidden));
         return check_launch(what);
     }
     return FL_OK;

@@ -261,11 +261,12 @@ PACK_NONE, PACK_ALL, PACK_KEPT = 0, 1, 2
 
 @functools.lru_cache(maxsize=256)
 def linear_loss_sizes(N: int, V: int, D: int, pack: int = PACK_KEPT, vocab_chunk: int = 0,
-                      want_hidden: bool = True, want_weight: bool = True) -> tuple[int, int, int]:
+                      want_hidden: bool = True, want_weight: bool = True,
+                      dtype: torch.dtype = torch.bfloat16) -> tuple[int, int, int]:
     """Bytes of the state that linear_loss_forward keeps and of the scratch that it and
     linear_loss_backward allocate."""
     out = [ctypes.c_int64() for _ in range(3)]
-    call("fl_linear_loss_sizes", N, V, D, pack, vocab_chunk, int(want_hidden) + 2 * int(want_weight),
+    call("fl_linear_loss_sizes", N, V, D, _DTYPE16[dtype], pack, vocab_chunk, int(want_hidden) + 2 * int(want_weight),
          *map(ctypes.byref, out))
     return tuple(v.value for v in out)
 
@@ -351,7 +352,7 @@ def linear_loss_backward(grad_output: torch.Tensor, hidden, weight: torch.Tensor
     grad_weight = torch.empty((V, Dp), dtype=dtype, device=dev) if want_weight else None
     if N:
         rpg, gs, rs = _dense_or_layout(hidden)[2:] if hidden is not None else (-1, 0, 0)
-        need_state, _, need = linear_loss_sizes(N, V, D, pack, vocab_chunk, want_hidden, want_weight)
+        need_state, _, need = linear_loss_sizes(N, V, D, pack, vocab_chunk, want_hidden, want_weight, dtype)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         call("fl_linear_loss_bwd", g.data_ptr(), _addr(hidden), rpg, gs, rs, weight.data_ptr(),
              weight.stride(0) if V > 1 else Dp, _DTYPE16[dtype], target.data_ptr(), pack, N, V, D, reduce,

@@ -87,7 +87,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     A target outside [0, V) gives NaN; with `check_index=True` it raises
     RuntimeError instead (one device sync).  Gradients have the dtype of their
     operands; the backward holds the logits' gradient of `vocab_chunk`
-    vocabulary entries at a time (None: at most 512 MB)."""
+    vocabulary entries at a time (None: at most 512 MB, twice that with bf16 operands)."""
     if reduction not in _REDUCTIONS:
         raise RuntimeError(f"linear_cross_entropy: unknown reduction {reduction!r}")
     ignore_index, z_loss = int(ignore_index), float(z_loss)

@@ -374,7 +374,8 @@ int fl_sparse_f32_bwd_workspace(int64_t num_nodes, int64_t batch, int64_t num_un
  * fl_linear_loss_bwd: with grad one float (reduce 2, 3) or (N,) by row,
  *   d z = grad * (softmax (1 + 2 z_loss lse) - onehot)   (reduce 0: grad * (onehot - softmax))
  *   is formed for `vocab_chunk` vocabulary columns at a time (0: a size that
- *   bounds the workspace; rounded down to a multiple of 256), in 16 bits, and
+ *   bounds the workspace; rounded down to a multiple of 256), in 16 bits (dtype
+ *   1: in bf16 for grad_hidden and in fp16, scaled, for grad_weight), and
  *   taken to grad_hidden (N, D) dense, zero in rows left out, and grad_weight
  *   (V, Dp) dense; either may be NULL.  A target outside [0, V) contributes no
  *   one-hot term.  Sums run in a fixed order: equal calls give equal bits.
@@ -384,7 +385,7 @@ int fl_sparse_f32_bwd_workspace(int64_t num_nodes, int64_t batch, int64_t num_un
  * Waits between the kernels' own copies and products end after 4 s at most;
  * the call's outputs are NaN then.
  * ---------------------------------------------------------------------- */
-int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int pack, int64_t vocab_chunk,
+int fl_linear_loss_sizes(int64_t N, int64_t V, int64_t D, int dtype, int pack, int64_t vocab_chunk,
                          int want, int64_t* state, int64_t* forward, int64_t* backward);
 int fl_linear_loss_fwd(const uint16_t* hidden, int64_t rows_per_group, int64_t group_stride,
                        int64_t row_stride, const uint16_t* weight, int64_t ldw, int dtype,

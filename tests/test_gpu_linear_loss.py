@@ -301,6 +301,89 @@ def test_gradient_against_differences():
         assert (got - want).abs() <= bound + 1e-8
 
 
+def _half_step(y, dtype):
+    """Half the spacing of the type's values at y."""
+    return torch.exp2(torch.floor(torch.log2(y.abs()))) * (torch.finfo(dtype).eps / 2)
+
+
+def test_weight_gradient_of_a_frequent_entry():
+    """bf16: the logits' gradients of a vocabulary entry named by many tokens keep more than the
+    eight bits of the result.  Zero weights make the softmax 1 / V, and every token of entry t
+    adds the same g (1 - 1 / V) h: in bf16, 257/256 would be 1, and a sum of 384 off by 1.5
+    where its rounding is off by 1 at most.  The bound: half a step of the result, 2^-11 of the
+    value for the rounding of dz (2^-12) and all fp32 steps (far below 2^-12)."""
+    N, D, V = 1000, 72, 4096
+    t = torch.full((N,), 7, device="cuda")
+    t[384:] = 9
+    h = (torch.arange(D, device="cuda") % 5 - 2.0).exp2().expand(N, D).to(BF16).contiguous()
+    w = torch.zeros(V, D, device="cuda", dtype=BF16)
+    g = torch.full((N,), 257 / 256, device="cuda")
+    g[384:] = 1 + 3 / 512
+    _, _, gw = _logp_case(h, w, t, g)
+    for entry in (7, 9, 11):
+        dz = g.to(F64) * ((t == entry).to(F64) - 1 / V)
+        want = dz @ h.to(F64)
+        err = (gw[entry].to(F64) - want).abs()
+        # an entry that no token names has its sum rounded only; 7 and 9 each the others' softmax too
+        assert (err <= _half_step(want, BF16) + 2.0 ** -11 * (dz.abs() @ h.to(F64))).all(), entry
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("N", [40, 300])
+def test_hidden_gradient_of_the_target_is_rounded_once(N, dtype):
+    """Zero hidden states make the softmax 1 / V; only the targets' weight rows are not zero.
+    The gradient g (1 - 1 / V) w is then within half a step of its value (a second rounding
+    would take up to a whole one), 2^-18 of it allowed for the fp32 steps: lse is known to
+    2^-23 of 9, exp to 2^-22, and 1 / V of the whole rests on them."""
+    D, V = 136, 8192
+    g = torch.Generator(device="cpu").manual_seed(N)
+    up = (torch.rand(N, generator=g) + 0.5).cuda()
+    t = torch.randint(0, 2, (N,), generator=g).cuda() * 5000  # entries 0 and 5000
+    w = torch.zeros(V, D, device="cuda", dtype=dtype)
+    w[0] = (torch.rand(D, generator=g) + 0.5).to(dtype).cuda()
+    h = torch.zeros(N, D, device="cuda", dtype=dtype)
+    _, gh, gw = _logp_case(h, w, t, up)
+    # entry 5000 has no weights: its tokens' gradients are - g / V w[0]
+    named = t == 0
+    want = (up.to(F64) * (1 - 1 / V))[named, None] * w[0].to(F64)
+    assert ((gh[named].to(F64) - want).abs() <= _half_step(want, dtype) + 2.0 ** -18 * want).all()
+    rest = (up.to(F64) / -V)[~named, None] * w[0].to(F64)
+    u = torch.finfo(dtype).eps / 2
+    assert ((gh[~named].to(F64) - rest).abs() <= (2 * u + 2.0 ** -18) * rest.abs() + 2.0 ** -24).all()
+    assert torch.equal(gw, torch.zeros_like(gw))
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e-25, 1e25])
+def test_weight_gradient_of_rows_of_any_size(scale):
+    """bf16 hidden rows from 2^-100 to 2^3 in size, rows of zeros, rows of subnormals, and
+    upstream gradients over twenty binades.  Beside the usual bound, fp16's smallest step: dz
+    and hidden are scaled so that the largest |g| |h| of a row, M, stands at 2^27 at least
+    (coefficients from 2^13, hidden from 2^14); 2^-25 of either is lost against at most 2^15
+    of the other, M 2^-37 each for every token."""
+    N, D, V = 200, 96, 700
+    h, w, t, up = make(N, D, V, BF16, seed=4)
+    g = torch.Generator(device="cpu").manual_seed(1)
+    power = torch.randint(-100, 1, (N, 1), generator=g).float()
+    power[::2] = 0
+    h = (h.float() * power.cuda().exp2()).to(BF16)
+    h[5] = 0
+    h[6] = 2.0 ** -130
+    up = up * torch.randint(-10, 11, (N,), generator=g).float().exp2().cuda() * scale
+    logp, gh, gw = _logp_case(h, w, t, up)
+    ref = reference(h, w, t, up.to(F64), sign=-1.0)
+    most = (up.to(F64).abs() * h.to(F64).abs().amax(-1)).max()
+    within(gh, ref["grad_hidden"], ref["grad_hidden_err"] + 2.0 ** -133, "grad_hidden")
+    within(gw, ref["grad_weight"], ref["grad_weight_err"] + N * 2.0 ** -36 * most + 2.0 ** -133, "grad_weight")
+    rms_close(gw, ref["grad_weight"], BF16, "grad_weight")
+
+
+def test_all_hidden_states_zero():
+    h, w, t, up = make(150, 64, 300, BF16)
+    h = torch.zeros_like(h)
+    _, gh, gw = _logp_case(h, w, t, up)
+    assert torch.equal(gw, torch.zeros_like(gw)) and torch.isfinite(gh).all() and gh.any()
+
+
 def test_extreme_logits():
     """Logits of +-1e4 and rows that one entry owns: finite losses, no overflow."""
     N, D, V = 64, 64, 1000
@@ -486,9 +569,10 @@ def test_logits_are_not_kept():
     peak = torch.cuda.max_memory_allocated() - base
     logits = N * V * 2
     # kept for the backward: the packed rows and three words a row; on top of it at the most
-    # the rows' partial states (16 bytes for 256 logits) or a piece, and the gradients
+    # the rows' partial states (16 bytes for 256 logits) or a piece in two types with the rows
+    # in fp16, and the gradients
     assert held <= 2 * N * D * 2 + 64 * N
-    assert peak <= held + max(N * 1024 * 2, logits // 16) + 4 * (N + V) * D + (8 << 20) < logits // 4
+    assert peak <= held + max(2 * N * 1024 * 2 + N * D * 2, logits // 16) + 4 * (N + V) * D + (8 << 20) < logits // 4
 
 
 def test_captured_step_replays_on_new_data():

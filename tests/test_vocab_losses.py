@@ -148,8 +148,14 @@ def test_sizes():
     assert ext.linear_loss_sizes(1000, 5000, 100, ext.PACK_NONE, 0, True)[0] == 256 + r(4000)
     assert fwd >= 1000 * 2 * 20 * 8 and bwd >= 1000 * 5120 * 2
     # a piece bounds the backward's scratch, whatever the vocabulary
-    small = ext.linear_loss_sizes(1000, 1 << 20, 100, ext.PACK_KEPT, 512, False)[2]
-    assert small <= 1000 * 512 * 2 + 3 * r(8000)
+    small = ext.linear_loss_sizes(1000, 1 << 20, 100, ext.PACK_KEPT, 512, False, True, torch.float16)[2]
+    assert small <= 1000 * 512 * 2 + 4 * r(8000)
+    # bf16: the rows again in fp16, and a piece in both types where both gradients are wanted
+    one = ext.linear_loss_sizes(1000, 1 << 20, 100, ext.PACK_KEPT, 512, False)[2]
+    assert one == small + r(4000) + r(1000 * 128 * 2)
+    both = ext.linear_loss_sizes(1000, 1 << 20, 100, ext.PACK_KEPT, 512)[2]
+    slabs = ext.linear_loss_sizes(1000, 1 << 20, 100, ext.PACK_KEPT, 512, True, True, torch.float16)[2] - small
+    assert both == one + slabs + r(1000 * 512 * 2)
     for bad in ((-1, 10, 10), (10, 0, 10), (10, 10, 0)):
         with pytest.raises(_lib.FuseLSEError):
             ext.linear_loss_sizes(*bad)
