@@ -306,6 +306,26 @@ def _half_step(y, dtype):
     return torch.exp2(torch.floor(torch.log2(y.abs()))) * (torch.finfo(dtype).eps / 2)
 
 
+@pytest.mark.parametrize("n", [1, 33, 100])
+def test_few_tokens_long_sums(n):
+    """Up to 128 tokens: a logit of 4096 positive products.  An accumulator that rounds toward
+    zero loses up to 2^-23 of itself at each of the 32 instructions (16 of K) of a piece, being
+    on average half the piece's sum: 16.5 x 2^-23 of z over all pieces; 8 additions of the
+    pieces, 2^-24 each, and the same again for the products of different sizes: 21 x 2^-23 in
+    all.  (In one piece of 256 instructions: up to 128.)  The other logits are zero, and lse and
+    the difference are single fp32 values below 16 (2^-21 each and for the sum of exponentials)."""
+    D, V = 4096, 131072
+    g = torch.Generator(device="cpu").manual_seed(n)
+    h = (torch.rand(n, D, generator=g) + 0.5).to(BF16).cuda()
+    w = torch.zeros(V, D, dtype=BF16, device="cuda")
+    w[70001] = ((torch.rand(D, generator=g) + 0.5) * (8.0 / D)).to(BF16).cuda()
+    t = torch.full((n,), 70001, device="cuda")
+    z = h.to(F64) @ w[70001].to(F64)
+    want = z - torch.log(torch.exp(z) + (V - 1))
+    err = (linear_selective_log_softmax(h, w, t).to(F64) - want).abs()
+    assert (err <= 21 * 2.0 ** -23 * z + 3 * 2.0 ** -21).all(), err.max()
+
+
 def test_weight_gradient_of_a_frequent_entry():
     """bf16: the logits' gradients of a vocabulary entry named by many tokens keep more than the
     eight bits of the result.  Zero weights make the softmax 1 / V, and every token of entry t
